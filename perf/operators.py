@@ -189,7 +189,8 @@ def _quantised(x, group):
     """fp32 rows [..., dim] -> (codes uint8 [..., dim / 2], params fp16 [..., dim / group, 2])."""
     g = x.unflatten(-1, (-1, group))
     lo = g.amin(-1).half()
-    step = ((g.amax(-1) - lo.float()) / 15.0).clamp_min(0.0).half()
+    span = g.amax(-1) - lo.float()
+    step = (span / torch.full_like(span, 15.0)).clamp_min(0.0).half()     # a tensor: by a number torch multiplies with its inverse
     inv = torch.where(step > 0, 1.0 / step.float(), torch.zeros((), device=x.device))
     codes = ((g - lo.float()[..., None]) * inv[..., None]).round().clamp(0.0, 15.0).to(torch.uint8).flatten(-2)
     return codes[..., 0::2] | (codes[..., 1::2] << 4), torch.stack([lo, step], -1)
