@@ -7,7 +7,7 @@
  *
  *   1. Device runtime   itexb_rt_*      - what ITEX's StreamExecutor callbacks do
  *   2. Kernel launches  itexb_quantize / itexb_dequantize / itexb_gemm / itexb_conv2d /
- *                       itexb_fp8_*     - raw device pointers + POD descriptors
+ *                       itexb_fp8_* / itexb_rope / itexb_kv4_*  - raw device pointers + POD descriptors
  *   3. Op layer         itexb_op_*      - ITEX's op names, attrs, input/output order,
  *                       HostMemory conventions and error behaviour; this is what a
  *                       TensorFlow PluggableDevice shim binds its create/compute/delete
@@ -455,6 +455,156 @@ ITEXB_API int itexb_fp8_layernorm(const void* x, int x_dtype, const void* gamma,
 ITEXB_API int itexb_fp8_amax_and_scale_update(float* amax_history, float* scale, float* scale_inv,
                                               int32_t history_len, int32_t n, float fp8_max, float margin,
                                               int32_t algo, itexb_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Decoder operators: what stands between a decoder's QKV linear and its output linear.  Rotary positions, per-head
+ * norms of queries and keys, a paged key/value cache held in 4 bits, and attention over it.  No counterpart in the
+ * reference, whose attention is a chain of (quantized) batched matmuls and a softmax over dense keys
+ * (itex/core/kernels/common/batch_matmul_op.h).  Strides count elements unless said otherwise; the innermost
+ * dimension is always dense.  All calls are asynchronous on `stream` and may be captured into a CUDA graph.           */
+/* ------------------------------------------------------------------------- */
+
+/* Written to a status word (as by itexb_gemm) by the kernels below. */
+#define ITEXB_STATUS_BAD_INDEX 6      /* a slot, page, length or row offset lies outside its tensor; it was skipped */
+#define ITEXB_STATUS_WAIT_EXPIRED 7   /* a bounded wait inside the kernel ran out; the output is incomplete */
+
+/* Rotary positions of q [tokens, q_heads, head_dim] and, with k_heads > 0, k [tokens, k_heads, head_dim]: the first
+ * rotary_dim elements of every head are rotated pair by pair, the rest is copied.  With angle = positions[t] *
+ * inv_freq[i] (radians, formed and reduced in 64 bits), i < rotary_dim / 2:
+ *   (a, b) -> mscale * (a cos - b sin, b cos + a sin)
+ * a, b = elements i and i + rotary_dim/2 (interleaved == 0) or 2i and 2i + 1 (interleaved != 0).  inverse != 0 turns by
+ * -angle, which (mscale unchanged) is the transpose of the forward map, hence its gradient.  Scaled positions are
+ * expressed in inv_freq and mscale.  An output may be its input (in place), else they must not overlap. */
+typedef struct itexb_rope_params {
+  int64_t tokens;
+  int32_t q_heads, k_heads;
+  int32_t head_dim;              /* even, up to 512 */
+  int32_t rotary_dim;            /* even, 0 .. head_dim */
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t dtype;                 /* FLOAT | BFLOAT16 | HALF, of q, k and the outputs */
+  int32_t positions_dtype;       /* INT32 | INT64 */
+  float mscale;
+  const void* positions;         /* device [tokens] */
+  const double* inv_freq;        /* device [rotary_dim / 2] */
+  const void* q; int64_t q_token_stride, q_head_stride;
+  const void* k; int64_t k_token_stride, k_head_stride;
+  void* q_out;   int64_t q_out_token_stride, q_out_head_stride;
+  void* k_out;   int64_t k_out_token_stride, k_out_head_stride;
+} itexb_rope_params_t;
+ITEXB_API int itexb_rope(const itexb_rope_params_t* p, itexb_stream_t stream);
+
+/* The same after a root-mean-square norm over each head: x -> x * rsqrt(mean(x^2) + epsilon) * weight, then the
+ * rotation, in one pass (statistics in fp32).  q_weight / k_weight: device [head_dim] of w_dtype.  r.inverse must be 0. */
+typedef struct itexb_qk_norm_rope_params {
+  itexb_rope_params_t r;
+  const void* q_weight;
+  const void* k_weight;
+  int32_t w_dtype;               /* FLOAT | BFLOAT16 | HALF */
+  float epsilon;
+} itexb_qk_norm_rope_params_t;
+ITEXB_API int itexb_qk_norm_rope(const itexb_qk_norm_rope_params_t* p, itexb_stream_t stream);
+
+/* Gradient of itexb_qk_norm_rope.  n describes the forward call (r.q, r.k its inputs); n.r.q_out / n.r.k_out receive the
+ * inputs' gradients, q_grad / k_grad are the outputs' gradients (dtype n.r.dtype), d_q_weight / d_k_weight the weights'
+ * gradients [head_dim] in w_dtype, summed over tokens and heads in a fixed order (equal calls give equal bits).
+ * workspace: device scratch of itexb_qk_norm_rope_grad_workspace_bytes(). */
+typedef struct itexb_qk_norm_rope_grad_params {
+  itexb_qk_norm_rope_params_t n;
+  const void* q_grad; int64_t q_grad_token_stride, q_grad_head_stride;
+  const void* k_grad; int64_t k_grad_token_stride, k_grad_head_stride;
+  void* d_q_weight;
+  void* d_k_weight;
+  void* workspace;
+} itexb_qk_norm_rope_grad_params_t;
+ITEXB_API size_t itexb_qk_norm_rope_grad_workspace_bytes(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim);
+ITEXB_API int itexb_qk_norm_rope_grad(const itexb_qk_norm_rope_grad_params_t* p, itexb_stream_t stream);
+
+/* A paged key/value cache held in 4 bits.  A row is one token of one key/value head: head_dim / 2 bytes of codes
+ * (element 2i in the low, 2i + 1 in the high nibble of byte i) and, for every `group` consecutive elements, a pair of
+ * halves (lo, step): element = lo + step * code.  Written as: lo = half(min), step = half(max(0, (max - lo) / 15)),
+ * code = clamp(rne((x - lo) * (1 / step)), 0, 15) in fp32 (step 0: code 0); a group that holds a NaN or an infinity, or
+ * whose lo or step does not fit a finite half, is stored as NaN.  Row `o` of page `g` for head `h` lies at
+ *   codes  + g * codes_page_stride + h * codes_head_stride + o * codes_token_stride              (bytes, multiples of 16)
+ *   params + g * params_page_stride + h * params_head_stride + o * params_token_stride           (pairs)
+ * so pages may be laid out head by head or token by token.  A row's pairs must be aligned to their size, up to 16
+ * bytes.  Slot s of the cache is row s % page_size of page s / page_size. */
+typedef struct itexb_kv4_cache {
+  int32_t num_pages, page_size, kv_heads;
+  int32_t head_dim;              /* 64 | 128 | 256 */
+  int32_t group;                 /* 32 | 64 | 128, at most head_dim */
+  int32_t reserved;
+  void* k_codes; void* k_params;
+  void* v_codes; void* v_params;
+  int64_t codes_page_stride, codes_head_stride, codes_token_stride;
+  int64_t params_page_stride, params_head_stride, params_token_stride;
+} itexb_kv4_cache_t;
+
+/* Quantizes k and v [tokens, kv_heads, head_dim] into the cache's rows slots[t]; a token whose slot is -1 is skipped, a
+ * slot past the cache is skipped and reported.  The slots of one call must differ.  With positions != NULL the keys are
+ * rotated on the way (as by itexb_rope, in fp32, cos and sin rounded from 64 bits). */
+typedef struct itexb_kv4_append_params {
+  itexb_kv4_cache_t cache;
+  int64_t tokens;
+  int32_t dtype;                 /* FLOAT | BFLOAT16 | HALF */
+  int32_t slots_dtype;           /* INT32 | INT64 */
+  const void* k; int64_t k_token_stride, k_head_stride;
+  const void* v; int64_t v_token_stride, v_head_stride;
+  const void* slots;             /* device [tokens] */
+  const void* positions;         /* device [tokens] or NULL: no rotation */
+  const double* inv_freq;
+  int32_t positions_dtype;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  float mscale;
+  int32_t* status_word;          /* optional */
+} itexb_kv4_append_params_t;
+ITEXB_API int itexb_kv4_append(const itexb_kv4_append_params_t* p, itexb_stream_t stream);
+
+/* The values that the cache's rows slots[t] stand for -> k and v [tokens, kv_heads, head_dim]; zeros for slot -1 and
+ * (reported) for a slot past the cache. */
+typedef struct itexb_kv4_gather_params {
+  itexb_kv4_cache_t cache;
+  int64_t tokens;
+  int32_t dtype;                 /* FLOAT | BFLOAT16 | HALF */
+  int32_t slots_dtype;           /* INT32 | INT64 */
+  void* k; int64_t k_token_stride, k_head_stride;
+  void* v; int64_t v_token_stride, v_head_stride;
+  const void* slots;
+  int32_t* status_word;
+} itexb_kv4_gather_params_t;
+ITEXB_API int itexb_kv4_gather(const itexb_kv4_gather_params_t* p, itexb_stream_t stream);
+
+/* Attention of new tokens over the cache: for query row i of sequence b and query head h (key/value head
+ * h / (q_heads / kv_heads)), out = sum_j softmax_j(scale * q . k_j) v_j over the visible cache rows j of the sequence:
+ * j < kept[b]; with `causal`, j <= place = kept[b] - new_b + i (the new tokens are the last of the sequence and already
+ * in the cache); with window > 0, j > place - window.  A row that sees nothing gets zeros.  Row j of sequence b is row
+ * j % page_size of page block_table[b * table_stride + j / page_size].
+ * new_b = q_starts[b + 1] - q_starts[b], its rows q_starts[b] .. of q and out; q_starts == NULL: new_b = max_new, rows
+ * b * max_new ...  Rows of `out` that belong to no sequence are left as they were.  max_new and max_kept are upper bounds
+ * the launch is sized by; a sequence beyond them (or beyond the table) is cut there and reported, a page outside the cache
+ * is not read: its rows count as not visible, and it is reported.
+ * workspace: device scratch of itexb_kv4_attention_workspace_bytes() for the same params (it depends on shapes and bounds
+ * only).  Calls that may run at the same time need workspaces of their own. */
+typedef struct itexb_kv4_attention_params {
+  itexb_kv4_cache_t cache;
+  int32_t dtype;                 /* BFLOAT16 | HALF, of q and out */
+  int32_t num_seqs, q_heads;
+  int32_t causal, window;
+  int32_t max_new, max_kept;
+  float scale;
+  int64_t total_rows;            /* rows of q and out */
+  const void* q; int64_t q_token_stride, q_head_stride;
+  void* out;     int64_t out_token_stride, out_head_stride;
+  const int32_t* block_table; int64_t table_stride;
+  int32_t table_cols;
+  const int32_t* kept;           /* device [num_seqs] */
+  const int32_t* q_starts;       /* device [num_seqs + 1] or NULL */
+  int32_t* status_word;          /* optional */
+  void* workspace; size_t workspace_bytes;
+} itexb_kv4_attention_params_t;
+ITEXB_API size_t itexb_kv4_attention_workspace_bytes(const itexb_kv4_attention_params_t* p);
+ITEXB_API int itexb_kv4_attention(const itexb_kv4_attention_params_t* p, itexb_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
 /* 3. Op layer.  One kernel object per graph node, created from the node's op name

@@ -99,6 +99,54 @@ class RewriteResult(C.Structure):
     _fields_ = [("new_op", C.c_char_p), ("num_added", C.c_int32), ("added", Attr * 4)]
 
 
+def _fields(text):
+    """'i32 a b; ptr c' -> ctypes fields."""
+    kinds = {"i32": C.c_int32, "i64": C.c_int64, "f32": C.c_float, "ptr": C.c_void_p, "size": C.c_size_t}
+    return [(n, kinds[part.split()[0]]) for part in text.split(";") for n in part.split()[1:]]
+
+
+class RopeParams(C.Structure):
+    _fields_ = _fields("i64 tokens; i32 q_heads k_heads head_dim rotary_dim interleaved inverse dtype positions_dtype; f32 mscale;"
+                       "ptr positions inv_freq q; i64 q_token_stride q_head_stride; ptr k; i64 k_token_stride k_head_stride;"
+                       "ptr q_out; i64 q_out_token_stride q_out_head_stride; ptr k_out; i64 k_out_token_stride k_out_head_stride")
+
+
+class QkNormRopeParams(C.Structure):
+    _fields_ = [("r", RopeParams)] + _fields("ptr q_weight k_weight; i32 w_dtype; f32 epsilon")
+
+
+class QkNormRopeGradParams(C.Structure):
+    _fields_ = [("n", QkNormRopeParams)] + _fields("ptr q_grad; i64 q_grad_token_stride q_grad_head_stride; ptr k_grad;"
+                                                   "i64 k_grad_token_stride k_grad_head_stride; ptr d_q_weight d_k_weight workspace")
+
+
+class Kv4CacheParams(C.Structure):
+    _fields_ = _fields("i32 num_pages page_size kv_heads head_dim group reserved; ptr k_codes k_params v_codes v_params;"
+                       "i64 codes_page_stride codes_head_stride codes_token_stride params_page_stride params_head_stride params_token_stride")
+
+
+class Kv4AppendParams(C.Structure):
+    _fields_ = [("cache", Kv4CacheParams)] + _fields(
+        "i64 tokens; i32 dtype slots_dtype; ptr k; i64 k_token_stride k_head_stride; ptr v; i64 v_token_stride v_head_stride;"
+        "ptr slots positions inv_freq; i32 positions_dtype rotary_dim interleaved; f32 mscale; ptr status_word")
+
+
+class Kv4GatherParams(C.Structure):
+    _fields_ = [("cache", Kv4CacheParams)] + _fields(
+        "i64 tokens; i32 dtype slots_dtype; ptr k; i64 k_token_stride k_head_stride; ptr v; i64 v_token_stride v_head_stride;"
+        "ptr slots status_word")
+
+
+class Kv4AttentionParams(C.Structure):
+    _fields_ = [("cache", Kv4CacheParams)] + _fields(
+        "i32 dtype num_seqs q_heads causal window max_new max_kept; f32 scale; i64 total_rows; ptr q; i64 q_token_stride q_head_stride;"
+        "ptr out; i64 out_token_stride out_head_stride; ptr block_table; i64 table_stride; i32 table_cols; ptr kept q_starts status_word"
+        " workspace; size workspace_bytes")
+
+
+# itexb_status words of the decoder operators
+STATUS_BAD_INDEX, STATUS_WAIT_EXPIRED = 6, 7
+
 ALLOC_OUTPUT_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.POINTER(Tensor))
 ALLOC_TEMP_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_size_t, C.c_int, C.POINTER(C.c_void_p))
 
@@ -139,6 +187,13 @@ def load():
     lib.itexb_peer_signal.argtypes = [C.POINTER(C.c_void_p), C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
     lib.itexb_peer_wait.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.itexb_peer_advance.argtypes = [C.c_void_p, C.c_void_p]
+    for name, params in (("rope", RopeParams), ("qk_norm_rope", QkNormRopeParams), ("qk_norm_rope_grad", QkNormRopeGradParams),
+                         ("kv4_append", Kv4AppendParams), ("kv4_gather", Kv4GatherParams), ("kv4_attention", Kv4AttentionParams)):
+        getattr(lib, "itexb_" + name).argtypes = [C.POINTER(params), C.c_void_p]
+    lib.itexb_qk_norm_rope_grad_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
+    lib.itexb_qk_norm_rope_grad_workspace_bytes.restype = C.c_size_t
+    lib.itexb_kv4_attention_workspace_bytes.argtypes = [C.POINTER(Kv4AttentionParams)]
+    lib.itexb_kv4_attention_workspace_bytes.restype = C.c_size_t
     _lib = lib
     return lib
 

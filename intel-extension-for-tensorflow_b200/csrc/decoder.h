@@ -1,0 +1,59 @@
+// Shared device helpers of the decoder operators (rotary positions, per-head norms, the 4-bit cache and attention).
+#ifndef ITEXB_CSRC_DECODER_H_
+#define ITEXB_CSRC_DECODER_H_
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.h"
+#include "gemm_sm100.h"  // FastDiv
+
+namespace itexb {
+
+__device__ __forceinline__ uint32_t QuickDiv(uint32_t x, const FastDiv& d) {  // x < 2^31
+  return d.mul == 0u ? x : __umulhi(x, d.mul) >> d.shift;
+}
+
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+__device__ __forceinline__ float ToFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float ToFloat(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T FromFloat(float v);
+template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half FromFloat<__half>(float v) { return __float2half_rn(v); }
+
+// VEC elements moved as one access of VEC * sizeof(T) bytes (1, 2, 4, 8 or 16); the caller guarantees the alignment.
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
+template <typename T, int VEC> __device__ __forceinline__ void LoadVec(const T* p, float (&f)[VEC]) {
+  const Vec<T, VEC> x = *reinterpret_cast<const Vec<T, VEC>*>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) f[i] = ToFloat(x.v[i]);
+}
+template <typename T, int VEC> __device__ __forceinline__ void StoreVec(T* p, const float (&f)[VEC]) {
+  Vec<T, VEC> x;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) x.v[i] = FromFloat<T>(f[i]);
+  *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+}
+
+__device__ __forceinline__ int64_t LoadIndex(const void* p, int is64, int64_t i) {
+  return is64 ? __ldg(static_cast<const long long*>(p) + i) : int64_t(__ldg(static_cast<const int*>(p) + i));
+}
+
+// Fraction of a turn of position * radians-per-position, in [-1/2, 1/2].  At position 10^6 a 32-bit product would be off
+// by 0.06 rad; the 64-bit one is off by 10^-10.
+__device__ __forceinline__ double TurnFraction(int64_t pos, double inv_freq) {
+  const double turns = double(pos) * (inv_freq * 0.15915494309189533577);  // 1 / (2 pi)
+  return turns - rint(turns);
+}
+
+__device__ __forceinline__ void ReportIndex(int32_t* status_word) {
+  if (status_word != nullptr) atomicCAS(status_word, 0, ITEXB_STATUS_BAD_INDEX);
+}
+
+}  // namespace itexb
+
+#endif  // ITEXB_CSRC_DECODER_H_

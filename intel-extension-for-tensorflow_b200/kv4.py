@@ -1,0 +1,180 @@
+"""A paged key/value cache held in 4 bits, attention over it, and the rotary frequencies of a decoder.
+
+A decoder layer's step between its QKV linear and its output linear, on columns of the QKV linear's output:
+
+    inv_freq, mscale = kv4.rope_frequencies(128, device="cuda")
+    cache = kv4.Kv4Cache.allocate(num_pages, 64, kv_heads, 128)
+    q = kernels.rope(q, positions, inv_freq, mscale=mscale)        # or kernels.qk_norm_rope
+    cache.append(k, v, slots, positions=positions, inv_freq=inv_freq, mscale=mscale)
+    out = cache.attention(q, block_table, kept, max_new=1, max_kept=8192)
+
+Every method is one call into the C-ABI (layer 2 of include/itexb200.h, where the row format is defined) on torch's current
+stream; none of them synchronises, and all may be captured into a CUDA graph.  Kernels report indexes outside the cache
+through an optional device int32 `status` (STATUS_BAD_INDEX) instead of following them.
+"""
+import math
+
+import torch
+
+from . import _lib as L
+from . import kernels as K
+
+STATUS_BAD_INDEX = L.STATUS_BAD_INDEX
+STATUS_WAIT_EXPIRED = L.STATUS_WAIT_EXPIRED
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, trained=8192, fast=32.0, slow=1.0, device="cuda"):
+    """-> (inv_freq, mscale): radians per position for each of the rotary_dim / 2 pairs (float64 on `device`) and the factor on
+    cos and sin, for kernels.rope, kernels.qk_norm_rope and Kv4Cache.append.  scaling stretches a model trained on `trained`
+    positions to `factor` times as many:
+      None        base ** (-2 i / rotary_dim)
+      "linear"    all frequencies divided by factor
+      "base"      base raised so that the slowest pair is divided by factor, the fastest kept
+      "by_parts"  pairs that turn fewer than `slow` times over `trained` positions divided by factor, those that turn more
+                  than `fast` times kept, a linear ramp over the pair's index between; mscale = 0.1 ln(factor) + 1
+      "by_length" the same two ends with the ramp linear in the number of turns; mscale = 1"""
+    if rotary_dim < 2 or rotary_dim % 2 != 0:
+        raise ValueError("rotary_dim must be even and positive, got %r" % (rotary_dim,))
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError("base must be above 1 and factor at least 1, got %r and %r" % (base, factor))
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / rotary_dim)
+    mscale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "base":
+        if rotary_dim < 4:
+            raise ValueError("scaling='base' needs more than one pair")
+        f = (base * factor ** (rotary_dim / (rotary_dim - 2.0))) ** (-2.0 * i / rotary_dim)
+    elif scaling in ("by_parts", "by_length"):
+        if not fast > slow > 0.0 or trained <= 0:
+            raise ValueError("fast > slow > 0 and trained > 0 are needed, got %r, %r, %r" % (fast, slow, trained))
+        if scaling == "by_parts":
+            at = [rotary_dim * math.log(trained / (turns * 2.0 * math.pi)) / (2.0 * math.log(base)) for turns in (fast, slow)]
+            low, high = max(0.0, math.floor(at[0])), min(rotary_dim / 2.0 - 1.0, math.ceil(at[1]))
+            stretch = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+            mscale = 0.1 * math.log(factor) + 1.0
+        else:
+            stretch = ((fast - trained * f / (2.0 * math.pi)) / (fast - slow)).clamp(0.0, 1.0)
+        f = f * (1.0 - stretch) + f / factor * stretch
+    elif scaling is not None:
+        raise ValueError("unknown scaling %r" % (scaling,))
+    return f.to(device), mscale
+
+
+class Kv4Cache:
+    """The cache's four tensors: codes uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16
+    [pages, kv_heads, page_size, head_dim / group, 2], for keys and for values.  The first three dimensions may have any
+    strides (a token-major cache is passed as its transpose(1, 2)); keys and values share them.  The object holds no state
+    besides the tensors: which page belongs to which sequence is the caller's block table."""
+
+    def __init__(self, k_codes, k_params, v_codes, v_params):
+        self.device = K.on_device_of(k_codes, k_params, v_codes, v_params)
+        if k_codes.dim() != 4 or k_params.dim() != 5 or k_codes.dtype != torch.uint8 or k_params.dtype != torch.float16:
+            raise ValueError("codes must be uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16 [.., head_dim / group, 2]")
+        cs, ps, ct, pt = k_codes.shape, k_params.shape, k_codes.stride(), k_params.stride()
+        if v_codes.shape != cs or v_codes.stride() != ct or v_codes.dtype != torch.uint8 or v_params.shape != ps or v_params.stride() != pt \
+                or v_params.dtype != torch.float16:
+            raise ValueError("keys and values must agree in shapes, strides and types")
+        if ps[:3] != cs[:3] or ps[4] != 2 or ps[3] < 1 or ct[3] != 1 or pt[4] != 1 or (ps[3] > 1 and pt[3] != 2) or any(s % 2 for s in pt[:3]) \
+                or cs[3] * 2 % ps[3] != 0:
+            raise ValueError("codes %s and params %s do not describe one cache with dense rows" % (tuple(cs), tuple(ps)))
+        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.group = cs[0], cs[1], cs[2], cs[3] * 2, cs[3] * 2 // ps[3]
+        self._c = L.Kv4CacheParams(cs[0], cs[2], cs[1], cs[3] * 2, self.group, 0, k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(),
+                                   v_params.data_ptr(), ct[0], ct[1], ct[2], pt[0] // 2, pt[1] // 2, pt[2] // 2)
+
+    @classmethod
+    def allocate(cls, num_pages, page_size, kv_heads, head_dim, group=64, device="cuda", token_major=False):
+        """An empty cache; token_major lays a page out token by token instead of head by head."""
+        dims = (num_pages, page_size, kv_heads) if token_major else (num_pages, kv_heads, page_size)
+        made = []
+        for _ in range(2):
+            made.append(torch.zeros(dims + (head_dim // 2,), dtype=torch.uint8, device=device))
+            made.append(torch.zeros(dims + (head_dim // group, 2), dtype=torch.float16, device=device))
+        return cls(*[t.transpose(1, 2) if token_major else t for t in made])
+
+    def _kv(self, k, v, what):
+        kp, vp = K._rows(k, "k"), K._rows(v, "v", k)
+        if k.shape[1] != self.kv_heads or k.shape[2] != self.head_dim:
+            raise ValueError("%s: rows %s for a cache of %d heads of %d" % (what, tuple(k.shape), self.kv_heads, self.head_dim))
+        return kp, vp
+
+    def append(self, k, v, slots, *, positions=None, inv_freq=None, interleaved=False, mscale=1.0, status=None):
+        """Writes k, v [tokens, kv_heads, head_dim] (strided views are fine) into rows slots[t] = page * page_size + offset; -1
+        skips a token; the other slots of a call must differ.  With positions and inv_freq the keys are rotated on the way."""
+        K.on_device_of(self.k_codes, k, v, slots, positions, inv_freq, status)
+        if (positions is None) != (inv_freq is None):
+            raise ValueError("positions and inv_freq go together")
+        kp, vp = self._kv(k, v, "append")
+        n = k.shape[0]
+        sp = K._vector(slots, "slots", K._INDEX_DT, n)
+        pos = freq = pdt = rot = 0
+        if positions is not None:
+            pos, pdt = K._vector(positions, "positions", K._INDEX_DT, n), K._INDEX_DT[positions.dtype]
+            freq, rot = K._vector(inv_freq, "inv_freq", (torch.float64,)), 2 * inv_freq.shape[0]
+        K.launch(L.load().itexb_kv4_append, L.Kv4AppendParams(self._c, n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
+                                                              int(interleaved), mscale, _status(status)), self.device)
+
+    def gather(self, slots, dtype=torch.bfloat16, *, out_k=None, out_v=None, status=None):
+        """-> (k, v) [len(slots), kv_heads, head_dim]: the values that rows `slots` stand for, zeros for slot -1."""
+        K.on_device_of(self.k_codes, slots, out_k, out_v, status)
+        sp = K._vector(slots, "slots", K._INDEX_DT)
+        shape = (slots.shape[0], self.kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device) if out_k is None else out_k
+        v = torch.empty(shape, dtype=dtype, device=self.device) if out_v is None else out_v
+        kp, vp = self._kv(k, v, "gather")
+        if k.shape[0] != shape[0]:
+            raise ValueError("gather: %d rows for %d slots" % (k.shape[0], shape[0]))
+        K.launch(L.load().itexb_kv4_gather, L.Kv4GatherParams(self._c, shape[0], K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status)),
+                 self.device)
+        return k, v
+
+    def attention(self, q, block_table, kept, *, q_starts=None, max_new=None, max_kept=None, causal=True, window=0, scale=None, out=None,
+                  status=None, workspace=None):
+        """Attention of the new tokens q [rows, q_heads, head_dim] over the cache (itexb_kv4_attention): block_table int32
+        [sequences, pages each], kept int32 [sequences] = rows of each sequence in the cache, the new tokens' included.
+        q_starts int32 [sequences + 1] gives each sequence's rows of q; without it every sequence has max_new rows.  max_new and
+        max_kept are upper bounds of a sequence's new and kept tokens (by default as many as q and the table can hold); a tight
+        bound saves work.  -> out, whose rows behind the last sequence stay as they were (uninitialised without `out`).
+        workspace: a uint8 tensor of workspace_bytes(...) to use instead of a fresh one."""
+        K.on_device_of(self.k_codes, q, block_table, kept, q_starts, out, status, workspace)
+        qp = K._rows(q, "q")
+        seqs = kept.shape[0]
+        kp = K._vector(kept, "kept", (torch.int32,))
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != seqs or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+            raise ValueError("block_table must be int32 [sequences, pages] with dense rows, got %s %s" % (block_table.dtype, tuple(block_table.shape)))
+        rows, heads, dim = q.shape
+        if dim != self.head_dim or heads % self.kv_heads != 0:
+            raise ValueError("q %s for a cache of %d heads of %d" % (tuple(q.shape), self.kv_heads, self.head_dim))
+        sp = 0
+        if q_starts is not None:
+            sp = K._vector(q_starts, "q_starts", (torch.int32,), seqs + 1)
+            max_new = rows if max_new is None else max_new
+        elif max_new is None:
+            max_new = rows // max(1, seqs)
+        if q_starts is None and max_new * seqs > rows:
+            raise ValueError("%d sequences of %d new tokens, but q has %d rows" % (seqs, max_new, rows))
+        cols = block_table.shape[1]
+        max_kept = min(cols * self.page_size, (1 << 31) - 1) if max_kept is None else max_kept
+        o = torch.empty(q.shape, dtype=q.dtype, device=self.device) if out is None else out
+        p = L.Kv4AttentionParams(self._c, K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
+                                 rows, *qp, *K._rows(o, "out", q), block_table.data_ptr(), block_table.stride(0), cols, kp, sp, _status(status), 0, 0)
+        lib = L.load()
+        need = lib.itexb_kv4_attention_workspace_bytes(p)
+        if need:
+            if workspace is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+                raise ValueError("workspace must be a dense uint8 tensor")
+            p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        K.launch(lib.itexb_kv4_attention, p, self.device)
+        return o
+
+
+def _status(t):
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.numel() != 1:
+        raise ValueError("status must be one int32")
+    return t.data_ptr()
