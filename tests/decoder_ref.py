@@ -60,14 +60,21 @@ def dequantize(codes, params):
 
 
 def cache_rows(cache, table_row, kept, head):
-    """-> k, v float64 [kept, dim] of one sequence and head."""
+    """-> k, v and what the rounding of a weight may multiply: |v|, or v's distance from the middle of its group's range, lo + 8
+    step, where the middle is added unrounded.  There the fp32 sums are of products with 128 + code and with 136, up to 143
+    steps, taken from each other: two sums over the tokens of a warp (a quarter of them, 16 at a time, and the joins), each
+    addition off by up to 2^-23 of the sum, in units of the weights' 2^-8: 143 * 2 * 2^-15 steps times their number.
+    float64 [kept, dim] of one sequence and head."""
     j = torch.arange(kept, device=table_row.device)
     page, off = table_row.long()[j // cache.page_size], j % cache.page_size
-    return tuple(dequantize(c[page, head, off], p[page, head, off]).double() for c, p in ((cache.k_codes, cache.k_params), (cache.v_codes, cache.v_params)))
+    k, v = (dequantize(c[page, head, off], p[page, head, off]).double() for c, p in ((cache.k_codes, cache.k_params), (cache.v_codes, cache.v_params)))
+    pars = cache.v_params[page, head, off].double()
+    lo, step = (pars[..., i].repeat_interleave(cache.group, -1) for i in (0, 1))
+    return k, v, torch.maximum(v.abs(), (v - lo - 8.0 * step).abs()) + step * (143.0 * 2.0 ** -14 * (kept / 64 + 8))
 
 
 def attention(cache, q, table, kept, starts, causal=True, window=0, scale=None, hidden=None):
-    """-> (out, bound's parts A = sum p |v| and D = scale * sum |q| |k| at its largest), float64; rows behind the last sequence NaN.
+    """-> (out, bound's parts A = sum p |what weights multiply| and D = scale * sum |q| |k| at its largest), float64; rows behind the last sequence NaN.
     hidden: bool [seqs, rows] of cache rows that do not count."""
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     share = q.shape[1] // cache.kv_heads
@@ -87,21 +94,20 @@ def attention(cache, q, table, kept, starts, causal=True, window=0, scale=None, 
             if n_kept == 0:
                 out[lo:hi] = 0.0
                 break
-            k, v = cache_rows(cache, table[b].clamp_min(0), n_kept, h)
             clean = seen.any(0)[:, None]
-            k, v = torch.where(clean, k, 0.0), torch.where(clean, v, 0.0)
+            k, v, far = (torch.where(clean, x, 0.0) for x in cache_rows(cache, table[b].clamp_min(0), n_kept, h))
             for g in range(h * share, (h + 1) * share):
                 x = q[lo:hi, g].double()
                 a = (x @ k.T * scale).masked_fill(~seen, -math.inf)
                 p = torch.softmax(a, -1)
                 p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
-                out[lo:hi, g], size[lo:hi, g] = p @ v, p @ v.abs()
+                out[lo:hi, g], size[lo:hi, g] = p @ v, p @ far
                 dots[lo:hi, g, 0] = (x.abs() @ k.abs().T * scale).masked_fill(~seen, 0.0).amax(-1)
     return out, size, dots
 
 
 def check_attention(got, want, size, dots, rows, context):
-    """Elementwise: the weights' rounding (bf16 at worst, 2^-8), the values' (fp16, 2^-11), the output's, and twice a score's error
+    """Elementwise: the weights' rounding (bf16 at worst, 2^-8 of what a weight multiplies, see cache_rows), the values' (fp16, 2^-11), the output's, and twice a score's error
     (keys rounded to fp16, 2^-11, fp32 sums over the dimension, 2^-16) in the exponent, since it enters weights and their sum.
     In the 2-norm: the roundings are independent, each uniform within half a step (a factor 3^-1/2), so weights, output and
     scores add up to less than 6e-3 of the output for bf16 (2^-8 / 3^1/2 = 0.0023 each), where the scores stay moderate."""
