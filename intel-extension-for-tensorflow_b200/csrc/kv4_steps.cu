@@ -4,11 +4,13 @@
 // codes into operands stays cheap.  The codes themselves are multiplied, and the groups' ranges enter behind the products:
 //     q . k_t = sum_g step_tg (sum_{d in g} q_d c_td) + lo_tg (sum_{d in g} q_d)
 //     o_d     = sum_t (p_t step_tg) (c_td - 8) + sum_t p_t (lo_tg + 8 step_tg)
-// A code becomes a half by or-ing it into the low mantissa bits of a constant where it lies: 1024 + c at bits 0-3, 64 + c at
-// bits 4-7.  The keys' products take the constants along and their share, constant * sum q, is taken back in fp32.  The
-// values' constants are subtracted before the product (exact), because there the sums run over all tokens: left in, they
-// cost an 128 Ki context three digits.  Codes count from the middle of their range so that the rounding of (p step) is
-// relative to what a value differs from it.
+// A code needs no conversion: masked out where it lies, the word's low byte of each half reads as a subnormal half,
+// c 2^-24 at bits 0-3 and 16 c 2^-24 at bits 4-7, which the tensor cores multiply exactly.  That is one mask per two codes
+// and one shift per four.  The 16 is taken out of q beforehand and out of the output afterwards, the 2^24 is part of the scale.
+// Codes count from the middle of their range (8 sum p step, by the same rounded weights, comes off at the end), so that
+// the rounding of (p step) is relative to what a value differs from it.
+// (A constant's mantissa or-ed around the code, 1024 + c, costs as much, and taking the constant out again either three
+// digits, in sums over 128 Ki tokens, or an addition per two codes.)
 // q enters as half: for bf16 inputs each row is scaled by a power of two to at most 2, so that elements within 2^-14 of the
 // row's largest stay exact and the others are off by 2^-25 of it.  p is kept at most 4 (see kRescale), p * step is then
 // below 2^15.1 for every step a half can hold; small products lose bits only where they are 2^-11 of the largest or less.
@@ -35,7 +37,7 @@ constexpr int kStages = 4;
 constexpr int kMaxChunk = kTile * kWarps * 32;  // a lane of each warp holds the page of one of its tiles
 constexpr float kRescale = 4.f;                 // scores may pass the running maximum by 4 before it moves,
 constexpr float kShift = 2.f;                   // so weights are 2^(score - maximum - 2), at most 4
-constexpr float kNone = -INFINITY;
+constexpr float kNone = -3.0e38f;               // the maximum of no scores
 
 struct StepArgs {
   AttnArgs a;
@@ -59,31 +61,39 @@ template <int BYTES> __device__ __forceinline__ void CpAsync(uint32_t dst, const
 }
 
 __device__ __forceinline__ void Mma(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t Transpose8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-// The codes of a word's nibbles 0 and 4 as 1024 + c, of 1 and 5 as 64 + c (pairs of halves); nibbles 2, 6, 3, 7: of w >> 8.
-__device__ __forceinline__ uint32_t AndOr(uint32_t x, uint32_t mask, uint32_t constant) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(constant));
-  return r;
+template <int WORDS> __device__ __forceinline__ void Lds(uint32_t (&w)[WORDS], const uint8_t* at) {
+  if constexpr (WORDS == 1) w[0] = *reinterpret_cast<const uint32_t*>(at);
+  else if constexpr (WORDS == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(at);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(at + 4 * i);
+      w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+    }
+  }
 }
-__device__ __forceinline__ uint32_t EvenCodes(uint32_t w) { return AndOr(w, 0x000F000Fu, 0x64006400u); }
-__device__ __forceinline__ uint32_t OddCodes(uint32_t w) { return AndOr(w, 0x00F000F0u, 0x54005400u); }
-__device__ __forceinline__ uint32_t AddHalf2(uint32_t x, uint32_t y) {
-  uint32_t r;
-  asm("add.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
-  return r;
+__device__ __forceinline__ float2 Pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ void MmaFromZero(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-// c - 8 from the above
-__device__ __forceinline__ uint32_t EvenCentred(uint32_t w) { return AddHalf2(EvenCodes(w), 0xE408E408u); }   // - 1032
-__device__ __forceinline__ uint32_t OddCentred(uint32_t w) { return AddHalf2(OddCodes(w), 0xD480D480u); }    // - 72
+// The codes of a word's nibbles 0 and 4 as halves c 2^-24, of 1 and 5 as 16 c 2^-24; nibbles 2, 6, 3, 7: of w >> 8.
+__device__ __forceinline__ uint32_t EvenCodes(uint32_t w) { return w & 0x000F000Fu; }
+__device__ __forceinline__ uint32_t OddCodes(uint32_t w) { return w & 0x00F000F0u; }
+constexpr uint32_t kMiddle = 0x00080008u;      // the code 8
+constexpr float kUnit = 16777216.f;            // 2^24
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -94,14 +104,14 @@ __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) {
 struct F2 { uint64_t v; };
 __device__ __forceinline__ F2 Make2(float x, float y) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
 __device__ __forceinline__ F2 Same2(float x) { return Make2(x, x); }
-__device__ __forceinline__ float X(F2 a) { float x, y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); return x; }
-__device__ __forceinline__ float Y(F2 a) { float x, y; asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); return y; }
+__device__ __forceinline__ float X(F2 a) { return __uint_as_float(uint32_t(a.v)); }
+__device__ __forceinline__ float Y(F2 a) { return __uint_as_float(uint32_t(a.v >> 32)); }
 __device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
 __device__ __forceinline__ F2 Mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 __device__ __forceinline__ F2 Add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 
 // Partial results of four warps (or of several chunks) with maxima m and sums l: what the part's values are weighed with.
-__device__ __forceinline__ float PartWeight(float m, float l, float top) { return m == kNone ? (isnan(l) ? l : 0.f) : Exp2(m - top); }
+__device__ __forceinline__ float PartWeight(float m, float l, float top) { return m <= kNone ? (isnan(l) ? l : 0.f) : Exp2(m - top); }
 
 __device__ __forceinline__ void StoreOut(const AttnArgs& a, int bf16, int64_t at, float v) {
   if (bf16) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
@@ -118,7 +128,8 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
   constexpr int kW = GROUP / 32;                 // words of codes per lane, group and row (keys); halves (values)
   const AttnArgs& a = s.a;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t s_ok[kWarps][kStages];
+  __shared__ uint32_t s_ok[kWarps][kStages];          // !PAGE16: rows of a tile that are there
+  __shared__ longlong2 s_from[kWarps][32];            // PAGE16: where a tile's codes and params begin, from a page on
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   const int kvh = int(blockIdx.y) / s.row_tiles, rt = int(blockIdx.y) - kvh * s.row_tiles, b = blockIdx.z;
@@ -144,9 +155,9 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
     return;
   }
 
-  // ---- query rows as the 8-column operand; per group the sums sum q and the constants' share in the products
+  // ---- query rows as the 8-column operand, and their sums per group times 2^-24
   uint32_t qf[NT][DIM / 16][2];
-  F2 qs[NT][NG], qc[NT][NG], scale[NT];  // of columns 2c, 2c + 1
+  F2 qs[NT][NG], scale[NT];              // of columns 2c, 2c + 1
   int lo[NT][2], hi[NT][2];              // visible tokens of those columns
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -170,29 +181,31 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
 #pragma unroll
           for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x[g][w].e[e]) << 16)));
       }
-    float down = 1.f, up = a.scale_log2;     // powers of two: q * down is exact
+    // q * down is exact but for underflow; scores are (codes' product) * up, up > 0
+    float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f), up = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
     if (s.bf16) {
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
       if (most > 0.f && most < INFINITY) {
-        down = __uint_as_float(uint32_t(254 - e) << 23);
-        up = __uint_as_float(uint32_t(e) << 23) * a.scale_log2;
+        down *= __uint_as_float(uint32_t(254 - e) << 23);
+        up = fmaxf(up * __uint_as_float(uint32_t(e) << 23), 1e-37f);
       }
     }
+    up *= kUnit;
     scale[nt] = Make2(__shfl_sync(0xffffffffu, up, (2 * c) * 4), __shfl_sync(0xffffffffu, up, (2 * c + 1) * 4));
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float sum = 0.f, share = 0.f;
+      float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kW; ++w) {
         Piece& y = x[g][w];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (s.bf16) y.e[e] = __half_as_ushort(__float2half_rn(__uint_as_float(uint32_t(y.e[e]) << 16) * down));
-          const float f = __half2float(__ushort_as_half(y.e[e]));
+          const float raw = s.bf16 ? __uint_as_float(uint32_t(y.e[e]) << 16) : __half2float(__ushort_as_half(y.e[e]));
+          const float f = raw * down;
           sum += f;
-          share += f * ((e & 1) ? 64.f : 1024.f);
+          y.e[e] = __half_as_ushort(__float2half_rn(e & 1 ? f * 0.0625f : f));
         }
         // a word's codes come out in pairs (j, j + 4)
         const int ks = (g * kW + w) * 2;
@@ -203,10 +216,8 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      share += __shfl_xor_sync(0xffffffffu, share, 1);
-      share += __shfl_xor_sync(0xffffffffu, share, 2);
+      sum *= 1.f / kUnit;
       qs[nt][g] = Make2(__shfl_sync(0xffffffffu, sum, (2 * c) * 4), __shfl_sync(0xffffffffu, sum, (2 * c + 1) * 4));
-      qc[nt][g] = Make2(-__shfl_sync(0xffffffffu, share, (2 * c) * 4), -__shfl_sync(0xffffffffu, share, (2 * c + 1) * 4));
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -217,46 +228,58 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
   }
 
   // ---- tiles: w, w + 4, ...
-  uint8_t* ring = smem + warp * (kStages * kStage);
-  const uint32_t ring_addr = uint32_t(__cvta_generic_to_shared(ring));
+  const uint32_t ring = warp * (kStages * kStage), ring_addr = uint32_t(__cvta_generic_to_shared(smem)) + ring;
   const int mine = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
-  int my_page = -1;
-  if (PAGE16 && lane < mine) {
-    my_page = __ldg(table + QuickDiv(uint32_t(begin + (warp + lane * kWarps) * kTile), a.c.div_page));
-    if (my_page < 0 || my_page >= a.c.num_pages) {
-      ReportIndex(a.status_word);
-      my_page = -1;
+  uint32_t there = 0;   // PAGE16: tiles whose page exists
+  if (PAGE16) {
+    longlong2 from = make_longlong2(0, 0);
+    bool ok = false;
+    if (lane < mine) {
+      const int j0 = begin + (warp + lane * kWarps) * kTile;
+      const int col = int(QuickDiv(uint32_t(j0), a.c.div_page)), off = j0 - col * a.c.page_size;
+      const int page = __ldg(table + col);
+      ok = page >= 0 && page < a.c.num_pages;
+      if (ok) from = make_longlong2(int64_t(page) * a.c.cp + int64_t(off) * a.c.ct, (int64_t(page) * a.c.pp + int64_t(off) * a.c.pt) * 4);
+      else ReportIndex(a.status_word);
     }
+    s_from[warp][lane] = from;
+    there = __ballot_sync(0xffffffffu, ok);
+    __syncwarp();
   }
   const uint8_t* kcodes = a.c.k_codes + int64_t(kvh) * a.c.ch;
   const uint8_t* vcodes = a.c.v_codes + int64_t(kvh) * a.c.ch;
-  const int64_t lane_at = int64_t(lane / kPieces) * a.c.ct + (lane % kPieces) * 16;   // this lane's first piece in a tile
+  const uint8_t* pars = reinterpret_cast<const uint8_t*>((lane < 16 ? a.c.k_params : a.c.v_params) + int64_t(kvh) * a.c.ph);
+  if (PAGE16) {  // this lane's first piece of a tile, its row's params
+    kcodes += int64_t(lane / kPieces) * a.c.ct + (lane % kPieces) * 16;
+    vcodes += int64_t(lane / kPieces) * a.c.ct + (lane % kPieces) * 16;
+    pars += int64_t(lane & 15) * a.c.pt * 4;
+  }
   const int64_t lane_step = int64_t(32 / kPieces) * a.c.ct;
-  const __half2* pars = (lane < 16 ? a.c.k_params : a.c.v_params) + int64_t(kvh) * a.c.ph;
+  constexpr int kCopies = kPieces * kTile / 32;
+  uint32_t put[kCopies];
+#pragma unroll
+  for (int x = 0; x < kCopies; ++x) put[x] = PieceAt<DIM>((x * 32 + lane) / kPieces, (x * 32 + lane) % kPieces);
+  const uint32_t put_pars = 2 * kCodes + lane * (NG * 4);   // keys' rows, then values'
 
   auto issue = [&](int n) {
     const int stage = n & (kStages - 1);
     const int j0 = begin + (warp + n * kWarps) * kTile;
     const uint32_t dst = ring_addr + stage * kStage;
     if (PAGE16) {
-      const int page = __shfl_sync(0xffffffffu, my_page, n);
-      if (page >= 0) {
-        const int off = j0 - int(QuickDiv(uint32_t(j0), a.c.div_page)) * a.c.page_size;
-        int64_t from = int64_t(page) * a.c.cp + int64_t(off) * a.c.ct + lane_at;
+      if ((there >> n) & 1u) {
+        const longlong2 from = s_from[warp][n];
+        const uint8_t *k = kcodes + from.x, *v = vcodes + from.x, *p = pars + from.y;
 #pragma unroll
-        for (int x = 0; x < kPieces * kTile; x += 32) {
-          const int row = (x + lane) / kPieces, piece = (x + lane) % kPieces;
-          CpAsync<16>(dst + PieceAt<DIM>(row, piece), kcodes + from);
-          CpAsync<16>(dst + kCodes + PieceAt<DIM>(row, piece), vcodes + from);
-          from += lane_step;
+        for (int x = 0; x < kCopies; ++x) {
+          CpAsync<16>(dst + put[x], k);
+          CpAsync<16>(dst + kCodes + put[x], v);
+          k += lane_step;
+          v += lane_step;
         }
-        const __half2* p = pars + int64_t(page) * a.c.pp + int64_t(off + (lane & 15)) * a.c.pt;
-        const uint32_t pd = dst + 2 * kCodes + lane * (NG * 4);   // keys' rows, then values'
-        if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(pd, p);
-        else { CpAsync<16>(pd, p); CpAsync<16>(pd + 16, p + 4); }
+        if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(dst + put_pars, p);
+        else { CpAsync<16>(dst + put_pars, p); CpAsync<16>(dst + put_pars + 16, p + 16); }
       }
-      if (lane == 0) s_ok[warp][stage] = page >= 0 ? 0xffffu : 0u;
     } else {
       int page = -1, off = 0;
       const int j = j0 + (lane & 15);
@@ -271,37 +294,197 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
       }
       const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
 #pragma unroll
-      for (int x = 0; x < kPieces * kTile; x += 32) {
-        const int row = (x + lane) / kPieces, piece = (x + lane) % kPieces;
+      for (int x = 0; x < kCopies; ++x) {
+        const int row = (x * 32 + lane) / kPieces, piece = (x * 32 + lane) % kPieces;
         const int pg = __shfl_sync(0xffffffffu, page, row), of = __shfl_sync(0xffffffffu, off, row);
         if (pg >= 0) {
           const int64_t from = int64_t(pg) * a.c.cp + int64_t(of) * a.c.ct + piece * 16;
-          CpAsync<16>(dst + PieceAt<DIM>(row, piece), kcodes + from);
-          CpAsync<16>(dst + kCodes + PieceAt<DIM>(row, piece), vcodes + from);
+          CpAsync<16>(dst + put[x], kcodes + from);
+          CpAsync<16>(dst + kCodes + put[x], vcodes + from);
         }
       }
       if (page >= 0) {
-        const __half2* p = pars + int64_t(page) * a.c.pp + int64_t(off) * a.c.pt;
-        const uint32_t pd = dst + 2 * kCodes + lane * (NG * 4);
-        if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(pd, p);
-        else { CpAsync<16>(pd, p); CpAsync<16>(pd + 16, p + 4); }
+        const uint8_t* p = pars + (int64_t(page) * a.c.pp + int64_t(off) * a.c.pt) * 4;
+        if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(dst + put_pars, p);
+        else { CpAsync<16>(dst + put_pars, p); CpAsync<16>(dst + put_pars + 16, p + 16); }
       }
       if (lane == 0) s_ok[warp][stage] = ok;
     }
   };
 
-  float o[NT][DIM / 16][4];
+  float o[NT][DIM / 16][4], middle[NT][NG][4];   // sums times 2^-24; the odd channels' (2, 3) are 16 times as large
   F2 zsum[NT][NG], l[NT];
-  float m[NT][2];
+  F2 down[NT];                 // -(running maximum) - kShift
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int x = 0; x < DIM / 16; ++x) o[nt][x][0] = o[nt][x][1] = o[nt][x][2] = o[nt][x][3] = 0.f;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) zsum[nt][g] = Same2(0.f);
-    m[nt][0] = m[nt][1] = kNone;
+    for (int g = 0; g < NG; ++g) {
+      zsum[nt][g] = Same2(0.f);
+      middle[nt][g][0] = middle[nt][g][1] = middle[nt][g][2] = middle[nt][g][3] = 0.f;
+    }
+    down[nt] = Same2(-kNone - kShift);
     l[nt] = Same2(0.f);
   }
+
+  // where this lane reads in a tile; a group further is another piece of the same row (an xor, see PieceAt)
+  const uint32_t key_at = PieceAt<DIM>(r, c * (GROUP / 8) / 16) + c * (GROUP / 8) % 16;
+  const uint32_t value_at0 = kCodes + PieceAt<DIM>(2 * c, r * (GROUP / 16) / 16) + r * (GROUP / 16) % 16;
+  const uint32_t value_at1 = kCodes + PieceAt<DIM>(2 * c + 1, r * (GROUP / 16) / 16) + r * (GROUP / 16) % 16;
+  const uint32_t pars_at = 2 * kCodes + r * (NG * 4);
+  auto compute = [&](auto part, const uint32_t st, const int j0, const uint32_t ok) {
+    // ---- scores of tokens r, r + 8 and columns 2c, 2c + 1
+    float t[NT][4];
+    uint32_t kp0[NG], kp1[NG];
+    Lds<NG>(kp0, smem + st + pars_at);
+    Lds<NG>(kp1, smem + st + pars_at + 8 * NG * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint32_t w0[kW], w1[kW];
+      const uint8_t* from = smem + ((st + key_at) ^ (g * (GROUP / 2)));
+      Lds<kW>(w0, from);
+      Lds<kW>(w1, from + 8 * kRow);
+      float acc[NT][4];
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t u0 = half ? w0[w] >> 8 : w0[w], u1 = half ? w1[w] >> 8 : w1[w];
+          const uint32_t x[4] = {EvenCodes(u0), EvenCodes(u1), OddCodes(u0), OddCodes(u1)};
+          const int ks = (g * kW + w) * 2 + half;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (w == 0 && half == 0) MmaFromZero(acc[nt], x, qf[nt][ks][0], qf[nt][ks][1]);
+            else Mma(acc[nt], x, qf[nt][ks][0], qf[nt][ks][1]);
+          }
+        }
+      }
+      const float2 p0 = Pair(kp0[g]), p1 = Pair(kp1[g]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float qsum = e & 1 ? Y(qs[nt][g]) : X(qs[nt][g]);
+          const float2 p = e < 2 ? p0 : p1;
+          t[nt][e] = fmaf(p.y, acc[nt][e], g == 0 ? p.x * qsum : fmaf(p.x, qsum, t[nt][e]));
+        }
+    }
+
+    // ---- masks
+    uint32_t seen = 0xffffffffu;     // bit 4 nt + 2 * (token r + 8) + column
+    if constexpr (decltype(part)::value) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int in = r + 8 * k, j = j0 + in;
+          const bool there = ((ok >> in) & 1u) != 0u;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!there || j < lo[nt][e] || j >= hi[nt][e]) {
+              seen &= ~(1u << (4 * nt + 2 * k + e));
+              t[nt][2 * k + e] = -INFINITY;
+            }
+        }
+    }
+    // ---- the running maximum, moved only when a score passes it by more than kRescale
+    F2 d[NT][2];
+    float over = -INFINITY;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      d[nt][0] = Fma2(Make2(t[nt][0], t[nt][1]), scale[nt], down[nt]);
+      d[nt][1] = Fma2(Make2(t[nt][2], t[nt][3]), scale[nt], down[nt]);
+      over = fmaxf(over, fmaxf(fmaxf(X(d[nt][0]), Y(d[nt][0])), fmaxf(X(d[nt][1]), Y(d[nt][1]))));
+    }
+    if (__any_sync(0xffffffffu, over > kRescale - kShift)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2], to[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float was = e ? Y(down[nt]) : X(down[nt]);
+          float top = fmaxf(t[nt][e], t[nt][e + 2]) * (e ? Y(scale[nt]) : X(scale[nt]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          to[e] = fminf(was, -kShift - top);
+          f[e] = Exp2(to[e] - was);
+        }
+        down[nt] = Make2(to[0], to[1]);
+        const F2 f2 = Make2(f[0], f[1]);
+        l[nt] = Mul2(l[nt], f2);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          zsum[nt][g] = Mul2(zsum[nt][g], f2);
+          middle[nt][g][0] *= f[0]; middle[nt][g][1] *= f[1];   // all its rows are alike; (2, 3) are never read
+        }
+#pragma unroll
+        for (int x = 0; x < DIM / 16; ++x) { o[nt][x][0] *= f[0]; o[nt][x][1] *= f[1]; o[nt][x][2] *= f[0]; o[nt][x][3] *= f[1]; }
+        d[nt][0] = Fma2(Make2(t[nt][0], t[nt][1]), scale[nt], down[nt]);
+        d[nt][1] = Fma2(Make2(t[nt][2], t[nt][3]), scale[nt], down[nt]);
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      t[nt][0] = Exp2(X(d[nt][0])); t[nt][1] = Exp2(Y(d[nt][0]));
+      t[nt][2] = Exp2(X(d[nt][1])); t[nt][3] = Exp2(Y(d[nt][1]));
+      l[nt] = Add2(l[nt], Add2(Make2(t[nt][0], t[nt][1]), Make2(t[nt][2], t[nt][3])));
+    }
+
+    // ---- values: weights times the group's steps as the 8-column operand, codes of 16 channels as rows
+    uint32_t vp0[NG], vp1[NG];
+    Lds<NG>(vp0, smem + st + pars_at + kPars);
+    Lds<NG>(vp1, smem + st + pars_at + kPars + 8 * NG * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float2 p0 = Pair(vp0[g]), p1 = Pair(vp1[g]);
+      uint32_t b0[NT], b1[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float mid[2] = {fmaf(8.f, p0.y, p0.x), fmaf(8.f, p1.y, p1.x)};
+        float w[4], z[2] = {X(zsum[nt][g]), Y(zsum[nt][g])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float step = e < 2 ? p0.y : p1.y;
+          if constexpr (decltype(part)::value) {  // an unseen row's lo and step may be anything
+            const bool on = ((seen >> (4 * nt + e)) & 1u) != 0u;
+            w[e] = on ? t[nt][e] * step : 0.f;
+            z[e & 1] = on ? fmaf(t[nt][e], mid[e >> 1], z[e & 1]) : z[e & 1];
+          } else {
+            w[e] = t[nt][e] * step;
+            z[e & 1] = fmaf(t[nt][e], mid[e >> 1], z[e & 1]);
+          }
+        }
+        zsum[nt][g] = Make2(z[0], z[1]);
+        b0[nt] = Transpose8x8(PackHalf(w[0], w[1]));
+        b1[nt] = Transpose8x8(PackHalf(w[2], w[3]));
+        const uint32_t eights[4] = {kMiddle, kMiddle, kMiddle, kMiddle};
+        Mma(middle[nt][g], eights, b0[nt], b1[nt]);
+      }
+      const uint8_t *fa = smem + ((st + value_at0) ^ (g * (GROUP / 2))), *fb = smem + ((st + value_at1) ^ (g * (GROUP / 2)));
+      uint32_t x[4][kW > 1 ? kW / 2 : 1];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
+      if constexpr (kW == 1) {
+        x[0][0] = *reinterpret_cast<const uint16_t*>(fa); x[1][0] = *reinterpret_cast<const uint16_t*>(fb);
+        x[2][0] = *reinterpret_cast<const uint16_t*>(fa + 8 * kRow); x[3][0] = *reinterpret_cast<const uint16_t*>(fb + 8 * kRow);
+      } else {
+        Lds<kW / 2>(x[0], fa); Lds<kW / 2>(x[1], fb); Lds<kW / 2>(x[2], fa + 8 * kRow); Lds<kW / 2>(x[3], fb + 8 * kRow);
+      }
+#pragma unroll
+      for (int hh = 0; hh < kW; ++hh) {
+        // four codes of each of two tokens, token pairs in the word's halves
+        const uint32_t sel = (hh & 1) ? 0x7632 : 0x5410;
+        const uint32_t u = __byte_perm(x[0][hh / 2], x[1][hh / 2], sel), v = __byte_perm(x[2][hh / 2], x[3][hh / 2], sel);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t uk = k ? u >> 8 : u, vk = k ? v >> 8 : v;
+          const uint32_t y[4] = {EvenCodes(uk), OddCodes(uk), EvenCodes(vk), OddCodes(vk)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) Mma(o[nt][(g * kW + hh) * 2 + k], y, b0[nt], b1[nt]);
+        }
+      }
+    }
+  };
 
 #pragma unroll
   for (int n = 0; n < kStages - 1; ++n) {
@@ -314,166 +497,13 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
     if (n + kStages - 1 < mine) issue(n + kStages - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
     const int stage = n & (kStages - 1);
-    const uint8_t* st = ring + stage * kStage;
+    const uint32_t st = ring + stage * kStage;
     const int j0 = begin + (warp + n * kWarps) * kTile;
-    const uint32_t ok = s_ok[warp][stage];
+    const uint32_t ok = PAGE16 ? (((there >> n) & 1u) ? 0xffffu : 0u) : s_ok[warp][stage];
 
-    // ---- scores of tokens r, r + 8 and columns 2c, 2c + 1
-    F2 t[NT][2];
-    const __half2* kp = reinterpret_cast<const __half2*>(st + 2 * kCodes);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      uint32_t w0[kW], w1[kW];
-      const int byte = g * (GROUP / 2) + c * (GROUP / 8);
-      const uint8_t* from = st + PieceAt<DIM>(r, byte / 16) + byte % 16;
-      if (kW == 1) { w0[0] = *reinterpret_cast<const uint32_t*>(from); w1[0] = *reinterpret_cast<const uint32_t*>(from + 8 * kRow); }
-      else if (kW == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(from), y = *reinterpret_cast<const uint2*>(from + 8 * kRow);
-        w0[0] = x.x; w0[kW - 1] = x.y; w1[0] = y.x; w1[kW - 1] = y.y;
-      } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(from), y = *reinterpret_cast<const uint4*>(from + 8 * kRow);
-        w0[0] = x.x; w0[1 % kW] = x.y; w0[2 % kW] = x.z; w0[3 % kW] = x.w;
-        w1[0] = y.x; w1[1 % kW] = y.y; w1[2 % kW] = y.z; w1[3 % kW] = y.w;
-      }
-      float acc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kW; ++w) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t u0 = half ? w0[w] >> 8 : w0[w], u1 = half ? w1[w] >> 8 : w1[w];
-          const uint32_t x[4] = {EvenCodes(u0), EvenCodes(u1), OddCodes(u0), OddCodes(u1)};
-          const int ks = (g * kW + w) * 2 + half;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) Mma(acc[nt], x, qf[nt][ks][0], qf[nt][ks][1]);
-        }
-      }
-      const float2 p0 = __half22float2(kp[r * NG + g]), p1 = __half22float2(kp[(r + 8) * NG + g]);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const F2 l0 = Same2(p0.x), l1 = Same2(p1.x);
-        const F2 base0 = g == 0 ? Mul2(l0, qs[nt][g]) : Fma2(l0, qs[nt][g], t[nt][0]);
-        const F2 base1 = g == 0 ? Mul2(l1, qs[nt][g]) : Fma2(l1, qs[nt][g], t[nt][1]);
-        t[nt][0] = Fma2(Same2(p0.y), Add2(Make2(acc[nt][0], acc[nt][1]), qc[nt][g]), base0);
-        t[nt][1] = Fma2(Same2(p1.y), Add2(Make2(acc[nt][2], acc[nt][3]), qc[nt][g]), base1);
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) { t[nt][0] = Mul2(t[nt][0], scale[nt]); t[nt][1] = Mul2(t[nt][1], scale[nt]); }
-
-    // ---- masks: only tiles that not every row sees whole
-    const bool partial = j0 < all_begin || j0 + kTile > all_end || ok != 0xffffu;
-    uint32_t seen = 0xffffffffu;     // bit 4 nt + 2 * (token r + 8) + column
-    if (partial) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int in = r + 8 * k, j = j0 + in;
-          const bool there = ((ok >> in) & 1u) != 0u;
-          float v[2] = {X(t[nt][k]), Y(t[nt][k])};
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!there || j < lo[nt][e] || j >= hi[nt][e]) {
-              seen &= ~(1u << (4 * nt + 2 * k + e));
-              v[e] = kNone;
-            }
-          t[nt][k] = Make2(v[0], v[1]);
-        }
-    }
-    // ---- the running maximum, moved only when a score passes it by more than kRescale
-    bool above = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      above = above || fmaxf(X(t[nt][0]), X(t[nt][1])) > m[nt][0] + kRescale || fmaxf(Y(t[nt][0]), Y(t[nt][1])) > m[nt][1] + kRescale;
-    if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = e ? fmaxf(Y(t[nt][0]), Y(t[nt][1])) : fmaxf(X(t[nt][0]), X(t[nt][1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          top = fmaxf(top, m[nt][e]);
-          f[e] = top == kNone ? 1.f : Exp2(m[nt][e] - top);
-          m[nt][e] = top;
-        }
-        const F2 f2 = Make2(f[0], f[1]);
-        l[nt] = Mul2(l[nt], f2);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) zsum[nt][g] = Mul2(zsum[nt][g], f2);
-#pragma unroll
-        for (int x = 0; x < DIM / 16; ++x) { o[nt][x][0] *= f[0]; o[nt][x][1] *= f[1]; o[nt][x][2] *= f[0]; o[nt][x][3] *= f[1]; }
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const F2 down = Make2(m[nt][0] == kNone ? 0.f : -kShift - m[nt][0], m[nt][1] == kNone ? 0.f : -kShift - m[nt][1]);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const F2 d = Add2(t[nt][k], down);
-        t[nt][k] = Make2(Exp2(X(d)), Exp2(Y(d)));
-        l[nt] = Add2(l[nt], t[nt][k]);
-      }
-    }
-
-    // ---- values: weights times the group's steps as the 8-column operand, codes of 16 channels as rows
-    const uint8_t* sv = st + kCodes;
-    const __half2* vp = reinterpret_cast<const __half2*>(st + 2 * kCodes + kPars);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float2 p0 = __half22float2(vp[r * NG + g]), p1 = __half22float2(vp[(r + 8) * NG + g]);
-      uint32_t b0[NT], b1[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const F2 mid0 = Same2(fmaf(8.f, p0.y, p0.x)), mid1 = Same2(fmaf(8.f, p1.y, p1.x));
-        F2 w0 = Mul2(t[nt][0], Same2(p0.y)), w1 = Mul2(t[nt][1], Same2(p1.y));
-        if (partial) {  // an unseen row's lo and step may be anything
-          const uint32_t b = seen >> (4 * nt);
-          w0 = Make2(b & 1u ? X(w0) : 0.f, b & 2u ? Y(w0) : 0.f);
-          w1 = Make2(b & 4u ? X(w1) : 0.f, b & 8u ? Y(w1) : 0.f);
-          const F2 z0 = Mul2(t[nt][0], mid0), z1 = Mul2(t[nt][1], mid1);
-          zsum[nt][g] = Add2(zsum[nt][g], Add2(Make2(b & 1u ? X(z0) : 0.f, b & 2u ? Y(z0) : 0.f), Make2(b & 4u ? X(z1) : 0.f, b & 8u ? Y(z1) : 0.f)));
-        } else {
-          zsum[nt][g] = Fma2(t[nt][0], mid0, Fma2(t[nt][1], mid1, zsum[nt][g]));
-        }
-        b0[nt] = Transpose8x8(PackHalf(X(w0), Y(w0)));
-        b1[nt] = Transpose8x8(PackHalf(X(w1), Y(w1)));
-      }
-      const int byte = g * (GROUP / 2) + r * (GROUP / 16);
-      const uint8_t* fa = sv + PieceAt<DIM>(2 * c, byte / 16) + byte % 16;
-      const uint8_t* fb = sv + PieceAt<DIM>(2 * c + 1, byte / 16) + byte % 16;
-      uint32_t x[4][kW > 1 ? kW / 2 : 1];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
-      if (kW == 1) {
-        x[0][0] = *reinterpret_cast<const uint16_t*>(fa); x[1][0] = *reinterpret_cast<const uint16_t*>(fb);
-        x[2][0] = *reinterpret_cast<const uint16_t*>(fa + 8 * kRow); x[3][0] = *reinterpret_cast<const uint16_t*>(fb + 8 * kRow);
-      } else if (kW == 2) {
-        x[0][0] = *reinterpret_cast<const uint32_t*>(fa); x[1][0] = *reinterpret_cast<const uint32_t*>(fb);
-        x[2][0] = *reinterpret_cast<const uint32_t*>(fa + 8 * kRow); x[3][0] = *reinterpret_cast<const uint32_t*>(fb + 8 * kRow);
-      } else {
-        const uint2 x0 = *reinterpret_cast<const uint2*>(fa), x1 = *reinterpret_cast<const uint2*>(fb);
-        const uint2 x2 = *reinterpret_cast<const uint2*>(fa + 8 * kRow), x3 = *reinterpret_cast<const uint2*>(fb + 8 * kRow);
-        constexpr int k1 = kW > 2 ? 1 : 0;
-        x[0][0] = x0.x; x[0][k1] = x0.y; x[1][0] = x1.x; x[1][k1] = x1.y;
-        x[2][0] = x2.x; x[2][k1] = x2.y; x[3][0] = x3.x; x[3][k1] = x3.y;
-      }
-#pragma unroll
-      for (int hh = 0; hh < kW; ++hh) {
-        // four codes of each of two tokens, token pairs in the word's halves
-        const uint32_t sel = (hh & 1) ? 0x7632 : 0x5410;
-        const uint32_t u = __byte_perm(x[0][hh / 2], x[1][hh / 2], sel), v = __byte_perm(x[2][hh / 2], x[3][hh / 2], sel);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t uk = k ? u >> 8 : u, vk = k ? v >> 8 : v;
-          const uint32_t y[4] = {EvenCentred(uk), OddCentred(uk), EvenCentred(vk), OddCentred(vk)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) Mma(o[nt][(g * kW + hh) * 2 + k], y, b0[nt], b1[nt]);
-        }
-      }
-    }
+    // two copies of the code: tiles that not every row sees whole carry masks
+    if (j0 < all_begin || j0 + kTile > all_end || ok != 0xffffu) compute(std::true_type{}, st, j0, ok);
+    else compute(std::false_type{}, st, j0, ok);
     __syncwarp();
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -490,7 +520,7 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
       float sum = e ? Y(l[nt]) : X(l[nt]);
       for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       const int row = warp * kRows + nt * 8 + 2 * c + e;
-      if (r == 0) s_ml[row] = make_float2(m[nt][e], sum);
+      if (r == 0) s_ml[row] = make_float2(-kShift - (e ? Y(down[nt]) : X(down[nt])), sum);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float z = e ? Y(zsum[nt][g]) : X(zsum[nt][g]);
@@ -498,7 +528,9 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
 #pragma unroll
         for (int x = 0; x < GROUP / 16; ++x) {
           const int d = g * GROUP + r * (GROUP / 8) + x * 2;
-          *reinterpret_cast<float2*>(s_o + row * DIM + d) = make_float2(o[nt][g * (GROUP / 16) + x][e] + z, o[nt][g * (GROUP / 16) + x][e + 2] + z);
+          const float *v = o[nt][g * (GROUP / 16) + x];
+          *reinterpret_cast<float2*>(s_o + row * DIM + d) =
+              make_float2(fmaf(v[e] - middle[nt][g][e], kUnit, z), fmaf(fmaf(v[e + 2], 0.0625f, -middle[nt][g][e]), kUnit, z));
         }
       }
     }
