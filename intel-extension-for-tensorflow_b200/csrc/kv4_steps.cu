@@ -15,15 +15,18 @@
 // row's largest stay exact and the others are off by 2^-25 of it.  p is kept at most 4 (see kRescale), p * step is then
 // below 2^15.1 for every step a half can hold; small products lose bits only where they are 2^-11 of the largest or less.
 //
-// A warp owns tiles of 16 tokens and keeps its own running maximum, so warps meet only at the end of a block's chunk of
-// tokens.  Both products run on mma.m16n8k16 with the cache as the 16-row operand (16 tokens, 16 channels) and up to
-// 8 query rows of the key/value head as the 8 columns: S^T = K q^T, O^T += V^T P^T; the weights turn from the first one's
-// accumulator layout into the second one's operand by an 8 x 8 transpose each.  Tensor cores of the tcgen05 kind want 64 or
-// more rows, of which a decoding step has 1 to 8, and operands in shared memory; here the tensor work is a small part of
-// the issue slots.  The order of channels inside a product is free, so lanes take them as the codes lie in a word.
+// A warp owns tiles of 16 tokens and keeps its own running maximum, so warps meet only at the end of a block's part.  Both
+// products run on mma.m16n8k16 with the cache as the 16-row operand (16 tokens, 16 channels) and up to 8 query rows of the
+// key/value head as the 8 columns: S^T = K q^T, O^T += V^T P^T; the weights turn from the first one's accumulator layout into
+// the second one's operand by an 8 x 8 transpose each.  Tensor cores of the tcgen05 kind want 64 or more rows, of which a
+// decoding step has 1 to 8, and operands in shared memory; here the tensor work is a small part of the issue slots.  The
+// order of channels inside a product is free, so lanes take them as the codes lie in a word.
 // Tiles come in through per-warp rings of cp.async copies (three tiles in flight per warp, sixteen or more warps per SM); the
 // 16-byte pieces are permuted so that both products read them without bank conflicts.
-// A context is cut into chunks of up to 2048 tokens, one block each; their partial results are joined by a second kernel.
+// The grid is one wave of resident blocks.  The tiles of all sequences and heads form one list, sequence after sequence, of
+// which every block takes an equal, contiguous part; a (sequence, head) that ends inside a block's part is written by it, the
+// others are joined from at most one result per block by a second kernel.  (One block per 2048 tokens instead left a fifth of
+// the machine idle behind the longest contexts, and smaller chunks cost more at their ends than they evened out.)
 #include <algorithm>
 
 #include "kv4_attention.h"
@@ -33,21 +36,28 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;                       // tokens
-constexpr int kStages = 4;
-constexpr int kMaxChunk = kTile * kWarps * 32;  // a lane of each warp holds the page of one of its tiles
+constexpr int kMaxBlocks = 740;                 // five per SM of a 148-SM device
+constexpr int kLeastTiles = 8;                  // of a block's part, where there is little work
 constexpr float kRescale = 4.f;                 // scores may pass the running maximum by 4 before it moves,
 constexpr float kShift = 2.f;                   // so weights are 2^(score - maximum - 2), at most 4
 constexpr float kNone = -3.0e38f;               // the maximum of no scores
 
 struct StepArgs {
   AttnArgs a;
-  int chunk;           // tokens, a multiple of kTile * kWarps
-  int chunks;          // per sequence at most
-  int row_tiles;
-  float* part_o;       // [seqs][kv_heads][max_new * share][chunks][head_dim], null: one chunk, write the output
-  float2* part_ml;     // ... (maximum, sum)
-  int bf16;            // type of q and out, else half
+  int row_tiles, units;      // 8 NT query rows each; units of a sequence: kv_heads * row_tiles
+  int bf16;                  // type of q and out, else half
+  float* part_o;             // [blocks][2][8 NT][head_dim]: a unit begun by an earlier block, a unit left to the next one
+  float2* part_ml;           // [blocks][2][8 NT] (maximum, sum)
+  int64_t* list;             // [2 + seqs]: tiles in all, blocks at work, tiles before each sequence
 };
+
+// Tiles that the new tokens of a sequence see.
+__device__ __forceinline__ int SeqTiles(const AttnArgs& a, const Seq& q) {
+  if (q.nnew == 0) return 0;
+  const int begin = RowBegin(a, q, 0) & ~(kTile - 1), end = RowEnd(a, q, q.nnew - 1);
+  return end > begin ? (end - begin + kTile - 1) / kTile : 0;
+}
+__device__ __forceinline__ int64_t BlockStart(int64_t total, int64_t blocks, int64_t block) { return total * block / blocks; }
 
 template <int DIM> __device__ __forceinline__ uint32_t PieceAt(int row, int piece) {  // byte offset of a 16-byte piece in a tile
   if (DIM == 64) return uint32_t((row >> 2) * 128 + ((((row & 3) * 2 + piece) ^ (((row >> 2) & 1) * 2)) * 16));
@@ -110,7 +120,7 @@ __device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %
 __device__ __forceinline__ F2 Mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 __device__ __forceinline__ F2 Add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 
-// Partial results of four warps (or of several chunks) with maxima m and sums l: what the part's values are weighed with.
+// Partial results of four warps (or of several blocks) with maxima m and sums l: what the part's values are weighed with.
 __device__ __forceinline__ float PartWeight(float m, float l, float top) { return m <= kNone ? (isnan(l) ? l : 0.f) : Exp2(m - top); }
 
 __device__ __forceinline__ void StoreOut(const AttnArgs& a, int bf16, int64_t at, float v) {
@@ -119,41 +129,113 @@ __device__ __forceinline__ void StoreOut(const AttnArgs& a, int bf16, int64_t at
 }
 
 // PAGE16: pages hold a multiple of 16 tokens, so a tile lies in one page.
+// At least so many blocks share an SM (registers): what keeps 16 warps on it for the common shape.
+template <int DIM, int GROUP, int NT> constexpr int kShareSm = DIM == 64 ? (NT == 1 ? 4 : 3) : DIM == 128 ? (NT == 1 ? 3 : 2) : 2;
+// Tiles a warp works on at a time, where registers allow: two give each other something to do and share the bookkeeping.
+template <int DIM, int NT> constexpr int kTogether = DIM < 256 && NT == 1 ? 2 : 1;
+template <int DIM, int NT> constexpr int kStagesOf = kTogether<DIM, NT> == 2 ? 3 : 4;
+
 template <int DIM, int GROUP, int NT, bool PAGE16>
-__global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ StepArgs s) {
+__global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKernel(const __grid_constant__ StepArgs s) {
   constexpr int NG = DIM / GROUP;
   constexpr int kRow = DIM / 2, kPieces = DIM / 32;
   constexpr int kCodes = kTile * kRow, kPars = kTile * NG * 4;
-  constexpr int kStage = 2 * kCodes + 2 * kPars;
+  constexpr int TT = kTogether<DIM, NT>, kStages = kStagesOf<DIM, NT>;
+  constexpr int kTileBytes = 2 * kCodes + 2 * kPars, kStage = TT * kTileBytes;
   constexpr int kW = GROUP / 32;                 // words of codes per lane, group and row (keys); halves (values)
   const AttnArgs& a = s.a;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t s_ok[kWarps][kStages];          // !PAGE16: rows of a tile that are there
-  __shared__ longlong2 s_from[kWarps][32];            // PAGE16: where a tile's codes and params begin, from a page on
+  __shared__ uint32_t s_ok[kWarps][kStages];          // rows of a tile that are there
+  __shared__ longlong2 s_from[kWarps][32];            // PAGE16: where the next tiles' codes and params begin, from a page on
+  __shared__ int64_t s_sum[kWarps];
+  __shared__ int64_t s_pos, s_stop, s_rest;           // place in the list, its end for this block; tiles of sequence s_seq before it
+  __shared__ int s_seq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
-  const int kvh = int(blockIdx.y) / s.row_tiles, rt = int(blockIdx.y) - kvh * s.row_tiles, b = blockIdx.z;
-  const Seq q = SeqOf(a, b, threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0);
-  const int rows = q.nnew * a.share, row0 = rt * 8 * NT;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (row0 >= rows) return;
-  // the tokens that some row of this block sees, and those that all of them see
-  const int i_first = int(QuickDiv(uint32_t(row0), a.div_share)), i_last = int(QuickDiv(uint32_t(min(rows, row0 + 8 * NT) - 1), a.div_share));
-  const int seq_begin = RowBegin(a, q, 0) & ~(kTile - 1);   // of the sequence's first row: chunks are laid out from here
-  const int block_begin = RowBegin(a, q, i_first), all_begin = RowBegin(a, q, i_last), all_end = RowEnd(a, q, i_first);
-  const int begin = seq_begin + int(blockIdx.x) * s.chunk;
-  const int end = min(begin + s.chunk, RowEnd(a, q, i_last));
-  const int ntiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
-  if (ntiles == 0 && (blockIdx.x > 0 || s.part_o != nullptr)) {
-    // the joining kernel reads every chunk of the sequence's rows
-    if (s.part_o != nullptr && begin < RowEnd(a, q, q.nnew - 1)) {
-      const int n = min(8 * NT, rows - row0);
-      const int64_t at = ((int64_t(b) * a.c.kv_heads + kvh) * (int64_t(a.max_new) * a.share) + row0) * s.chunks + blockIdx.x;
-      if (int(threadIdx.x) < n) s.part_ml[at + int64_t(threadIdx.x) * s.chunks] = make_float2(kNone, 0.f);
-      for (int x = threadIdx.x; x < n * DIM; x += kThreads) s.part_o[(at + int64_t(x / DIM) * s.chunks) * DIM + x % DIM] = 0.f;
+
+  // ---- this block's part of the list of tiles
+  {
+    const int per = (a.num_seqs + kThreads - 1) / kThreads;
+    const int b0 = min(a.num_seqs, int(threadIdx.x) * per), b1 = min(a.num_seqs, b0 + per);
+    int64_t sum = 0;
+    for (int x = b0; x < b1; ++x) sum += int64_t(SeqTiles(a, SeqOf(a, x, blockIdx.x == 0))) * s.units;
+    int64_t before = sum;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, before, x);
+      if (lane >= x) before += y;
     }
-    return;
+    if (lane == 31) s_sum[warp] = before;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_sum[w];
+      total += s_sum[w];
+    }
+    before -= sum;
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / kLeastTiles));
+    if (blockIdx.x == 0) {  // for the joining kernel
+      if (threadIdx.x == 0) { s.list[0] = total; s.list[1] = blocks; }
+      int64_t at = before;
+      for (int x = b0; x < b1; ++x) {
+        s.list[2 + x] = at;
+        at += int64_t(SeqTiles(a, SeqOf(a, x, false))) * s.units;
+      }
+    }
+    const int64_t pos = BlockStart(total, blocks, blockIdx.x);
+    const int64_t stop = blockIdx.x < blocks ? BlockStart(total, blocks, blockIdx.x + 1) : pos;
+    if (threadIdx.x == 0) { s_pos = pos; s_stop = stop; }
+    if (pos >= before && pos < before + sum) {
+      int64_t at = before;
+      for (int x = b0; x < b1; ++x) {
+        const int64_t n = int64_t(SeqTiles(a, SeqOf(a, x, false))) * s.units;
+        if (pos < at + n) {
+          s_seq = x;
+          s_rest = pos - at;
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
+  constexpr int kCopies = kPieces * kTile / 32;
+  uint32_t put[kCopies];
+#pragma unroll
+  for (int x = 0; x < kCopies; ++x) put[x] = PieceAt<DIM>((x * 32 + lane) / kPieces, (x * 32 + lane) % kPieces);
+  const uint32_t put_pars = 2 * kCodes + lane * (NG * 4);   // keys' rows, then values'
+  const int64_t lane_step = int64_t(32 / kPieces) * a.c.ct;
+  const uint32_t ring = warp * (kStages * kStage), ring_addr = uint32_t(__cvta_generic_to_shared(smem)) + ring;
+
+  while (s_pos < s_stop) {
+  const int b = s_seq;
+  const Seq q = SeqOf(a, b, false);
+  const int tiles = SeqTiles(a, q);
+  const int64_t rest = s_rest;
+  const int unit = tiles > 0 ? int(rest / tiles) : s.units;
+  const int tile0 = int(rest - int64_t(unit) * tiles), tile1 = int(min(int64_t(tiles), tile0 + (s_stop - s_pos)));
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (unit < s.units) {
+      s_pos += tile1 - tile0;
+      s_rest += tile1 - tile0;
+    } else {               // the next sequence that has any
+      s_rest -= int64_t(tiles) * s.units;
+      s_seq = b + 1;
+    }
+  }
+  __syncthreads();
+  const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
+  const int rows = q.nnew * a.share, row0 = rt * 8 * NT;
+  if (unit >= s.units || row0 >= rows) continue;   // a sequence shorter than the longest has fewer row tiles
+  // the tokens that some row of this unit sees, and those that all of them see
+  const int i_first = int(QuickDiv(uint32_t(row0), a.div_share)), i_last = int(QuickDiv(uint32_t(min(rows, row0 + 8 * NT) - 1), a.div_share));
+  const int some_begin = RowBegin(a, q, i_first), some_end = RowEnd(a, q, i_last);
+  const int all_begin = RowBegin(a, q, i_last), all_end = RowEnd(a, q, i_first);
+  const int begin = (RowBegin(a, q, 0) & ~(kTile - 1)) + tile0 * kTile;
+  const int ntiles = tile1 - tile0;
 
   // ---- query rows as the 8-column operand, and their sums per group times 2^-24
   uint32_t qf[NT][DIM / 16][2];
@@ -227,26 +309,10 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
     }
   }
 
-  // ---- tiles: w, w + 4, ...
-  const uint32_t ring = warp * (kStages * kStage), ring_addr = uint32_t(__cvta_generic_to_shared(smem)) + ring;
-  const int mine = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
+  // ---- steps of TT tiles: w, w + 4, ...
+  const int nsteps = (ntiles + TT - 1) / TT;
+  const int mine = nsteps > warp ? (nsteps - warp + kWarps - 1) / kWarps : 0;
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
-  uint32_t there = 0;   // PAGE16: tiles whose page exists
-  if (PAGE16) {
-    longlong2 from = make_longlong2(0, 0);
-    bool ok = false;
-    if (lane < mine) {
-      const int j0 = begin + (warp + lane * kWarps) * kTile;
-      const int col = int(QuickDiv(uint32_t(j0), a.c.div_page)), off = j0 - col * a.c.page_size;
-      const int page = __ldg(table + col);
-      ok = page >= 0 && page < a.c.num_pages;
-      if (ok) from = make_longlong2(int64_t(page) * a.c.cp + int64_t(off) * a.c.ct, (int64_t(page) * a.c.pp + int64_t(off) * a.c.pt) * 4);
-      else ReportIndex(a.status_word);
-    }
-    s_from[warp][lane] = from;
-    there = __ballot_sync(0xffffffffu, ok);
-    __syncwarp();
-  }
   const uint8_t* kcodes = a.c.k_codes + int64_t(kvh) * a.c.ch;
   const uint8_t* vcodes = a.c.v_codes + int64_t(kvh) * a.c.ch;
   const uint8_t* pars = reinterpret_cast<const uint8_t*>((lane < 16 ? a.c.k_params : a.c.v_params) + int64_t(kvh) * a.c.ph);
@@ -255,61 +321,83 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
     vcodes += int64_t(lane / kPieces) * a.c.ct + (lane % kPieces) * 16;
     pars += int64_t(lane & 15) * a.c.pt * 4;
   }
-  const int64_t lane_step = int64_t(32 / kPieces) * a.c.ct;
-  constexpr int kCopies = kPieces * kTile / 32;
-  uint32_t put[kCopies];
-#pragma unroll
-  for (int x = 0; x < kCopies; ++x) put[x] = PieceAt<DIM>((x * 32 + lane) / kPieces, (x * 32 + lane) % kPieces);
-  const uint32_t put_pars = 2 * kCodes + lane * (NG * 4);   // keys' rows, then values'
+  uint32_t there = 0;   // PAGE16: of the next 32 tiles, those whose page exists and that some row sees
 
-  auto issue = [&](int n) {
-    const int stage = n & (kStages - 1);
-    const int j0 = begin + (warp + n * kWarps) * kTile;
-    const uint32_t dst = ring_addr + stage * kStage;
+  auto issue = [&](int n, int stage) {
+    const uint32_t to = ring_addr + stage * kStage;
+    uint32_t rows_there = 0;
     if (PAGE16) {
-      if ((there >> n) & 1u) {
-        const longlong2 from = s_from[warp][n];
-        const uint8_t *k = kcodes + from.x, *v = vcodes + from.x, *p = pars + from.y;
-#pragma unroll
-        for (int x = 0; x < kCopies; ++x) {
-          CpAsync<16>(dst + put[x], k);
-          CpAsync<16>(dst + kCodes + put[x], v);
-          k += lane_step;
-          v += lane_step;
+      constexpr int kAhead = 32 / TT;
+      if (n % kAhead == 0) {   // a lane looks up the page of one of the next 32 tiles
+        __syncwarp();
+        longlong2 from = make_longlong2(0, 0);
+        bool ok = false;
+        const int tile = (warp + (n + lane / TT) * kWarps) * TT + lane % TT, j0 = begin + tile * kTile;
+        if (tile < ntiles && j0 + kTile > some_begin && j0 < some_end) {
+          const int col = int(QuickDiv(uint32_t(j0), a.c.div_page)), off = j0 - col * a.c.page_size;
+          const int page = __ldg(table + col);
+          ok = page >= 0 && page < a.c.num_pages;
+          if (ok) from = make_longlong2(int64_t(page) * a.c.cp + int64_t(off) * a.c.ct, (int64_t(page) * a.c.pp + int64_t(off) * a.c.pt) * 4);
+          else ReportIndex(a.status_word);
         }
-        if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(dst + put_pars, p);
-        else { CpAsync<16>(dst + put_pars, p); CpAsync<16>(dst + put_pars + 16, p + 16); }
+        s_from[warp][lane] = from;
+        there = __ballot_sync(0xffffffffu, ok);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int h = 0; h < TT; ++h) {
+        const int at = (n % kAhead) * TT + h;
+        if ((there >> at) & 1u) {
+          const uint32_t dst = to + h * kTileBytes;
+          const longlong2 from = s_from[warp][at];
+          const uint8_t *k = kcodes + from.x, *v = vcodes + from.x, *p = pars + from.y;
+#pragma unroll
+          for (int x = 0; x < kCopies; ++x) {
+            CpAsync<16>(dst + put[x], k);
+            CpAsync<16>(dst + kCodes + put[x], v);
+            k += lane_step;
+            v += lane_step;
+          }
+          if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(dst + put_pars, p);
+          else { CpAsync<16>(dst + put_pars, p); CpAsync<16>(dst + put_pars + 16, p + 16); }
+          rows_there |= 0xffffu << (16 * h);
+        }
       }
     } else {
-      int page = -1, off = 0;
-      const int j = j0 + (lane & 15);
-      if (j >= block_begin && j < end) {
-        const int col = int(QuickDiv(uint32_t(j), a.c.div_page));
-        off = j - col * a.c.page_size;
-        page = __ldg(table + col);
-        if (page < 0 || page >= a.c.num_pages) {
-          ReportIndex(a.status_word);
-          page = -1;
-        }
-      }
-      const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
 #pragma unroll
-      for (int x = 0; x < kCopies; ++x) {
-        const int row = (x * 32 + lane) / kPieces, piece = (x * 32 + lane) % kPieces;
-        const int pg = __shfl_sync(0xffffffffu, page, row), of = __shfl_sync(0xffffffffu, off, row);
-        if (pg >= 0) {
-          const int64_t from = int64_t(pg) * a.c.cp + int64_t(of) * a.c.ct + piece * 16;
-          CpAsync<16>(dst + put[x], kcodes + from);
-          CpAsync<16>(dst + kCodes + put[x], vcodes + from);
+      for (int h = 0; h < TT; ++h) {
+        const uint32_t dst = to + h * kTileBytes;
+        const int tile = (warp + n * kWarps) * TT + h;
+        int page = -1, off = 0;
+        const int j = begin + tile * kTile + (lane & 15);
+        if (tile < ntiles && j >= some_begin && j < some_end) {
+          const int col = int(QuickDiv(uint32_t(j), a.c.div_page));
+          off = j - col * a.c.page_size;
+          page = __ldg(table + col);
+          if (page < 0 || page >= a.c.num_pages) {
+            ReportIndex(a.status_word);
+            page = -1;
+          }
+        }
+        rows_there |= (__ballot_sync(0xffffffffu, page >= 0) & 0xffffu) << (16 * h);
+#pragma unroll
+        for (int x = 0; x < kCopies; ++x) {
+          const int row = (x * 32 + lane) / kPieces, piece = (x * 32 + lane) % kPieces;
+          const int pg = __shfl_sync(0xffffffffu, page, row), of = __shfl_sync(0xffffffffu, off, row);
+          if (pg >= 0) {
+            const int64_t from = int64_t(pg) * a.c.cp + int64_t(of) * a.c.ct + piece * 16;
+            CpAsync<16>(dst + put[x], kcodes + from);
+            CpAsync<16>(dst + kCodes + put[x], vcodes + from);
+          }
+        }
+        if (page >= 0) {
+          const uint8_t* p = pars + (int64_t(page) * a.c.pp + int64_t(off) * a.c.pt) * 4;
+          if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(dst + put_pars, p);
+          else { CpAsync<16>(dst + put_pars, p); CpAsync<16>(dst + put_pars + 16, p + 16); }
         }
       }
-      if (page >= 0) {
-        const uint8_t* p = pars + (int64_t(page) * a.c.pp + int64_t(off) * a.c.pt) * 4;
-        if (NG <= 4) CpAsync<(NG > 4 ? 4 : NG) * 4>(dst + put_pars, p);
-        else { CpAsync<16>(dst + put_pars, p); CpAsync<16>(dst + put_pars + 16, p + 16); }
-      }
-      if (lane == 0) s_ok[warp][stage] = ok;
     }
+    if (lane == 0) s_ok[warp][stage] = rows_there;
   };
 
   float o[NT][DIM / 16][4], middle[NT][NG][4];   // sums times 2^-24; the odd channels' (2, 3) are 16 times as large
@@ -334,15 +422,19 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
   const uint32_t value_at1 = kCodes + PieceAt<DIM>(2 * c + 1, r * (GROUP / 16) / 16) + r * (GROUP / 16) % 16;
   const uint32_t pars_at = 2 * kCodes + r * (NG * 4);
   auto compute = [&](auto part, const uint32_t st, const int j0, const uint32_t ok) {
+    float t[TT][NT][4];
+    uint32_t seen = 0xffffffffu;     // bit 16 h + 4 nt + 2 * (token r + 8) + column
+#pragma unroll
+    for (int h = 0; h < TT; ++h) {
+    const uint32_t sh = st + h * kTileBytes;
     // ---- scores of tokens r, r + 8 and columns 2c, 2c + 1
-    float t[NT][4];
     uint32_t kp0[NG], kp1[NG];
-    Lds<NG>(kp0, smem + st + pars_at);
-    Lds<NG>(kp1, smem + st + pars_at + 8 * NG * 4);
+    Lds<NG>(kp0, smem + sh + pars_at);
+    Lds<NG>(kp1, smem + sh + pars_at + 8 * NG * 4);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       uint32_t w0[kW], w1[kW];
-      const uint8_t* from = smem + ((st + key_at) ^ (g * (GROUP / 2)));
+      const uint8_t* from = smem + ((sh + key_at) ^ (g * (GROUP / 2)));
       Lds<kW>(w0, from);
       Lds<kW>(w1, from + 8 * kRow);
       float acc[NT][4];
@@ -367,36 +459,39 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
         for (int e = 0; e < 4; ++e) {
           const float qsum = e & 1 ? Y(qs[nt][g]) : X(qs[nt][g]);
           const float2 p = e < 2 ? p0 : p1;
-          t[nt][e] = fmaf(p.y, acc[nt][e], g == 0 ? p.x * qsum : fmaf(p.x, qsum, t[nt][e]));
+          t[h][nt][e] = fmaf(p.y, acc[nt][e], g == 0 ? p.x * qsum : fmaf(p.x, qsum, t[h][nt][e]));
         }
     }
 
     // ---- masks
-    uint32_t seen = 0xffffffffu;     // bit 4 nt + 2 * (token r + 8) + column
     if constexpr (decltype(part)::value) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int in = r + 8 * k, j = j0 + in;
-          const bool there = ((ok >> in) & 1u) != 0u;
+          const int in = r + 8 * k, j = j0 + h * kTile + in;
+          const bool there = ((ok >> (16 * h + in)) & 1u) != 0u;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (!there || j < lo[nt][e] || j >= hi[nt][e]) {
-              seen &= ~(1u << (4 * nt + 2 * k + e));
-              t[nt][2 * k + e] = -INFINITY;
+              seen &= ~(1u << (16 * h + 4 * nt + 2 * k + e));
+              t[h][nt][2 * k + e] = -INFINITY;
             }
         }
     }
+    }
     // ---- the running maximum, moved only when a score passes it by more than kRescale
-    F2 d[NT][2];
+    F2 d[TT][NT][2];
     float over = -INFINITY;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      d[nt][0] = Fma2(Make2(t[nt][0], t[nt][1]), scale[nt], down[nt]);
-      d[nt][1] = Fma2(Make2(t[nt][2], t[nt][3]), scale[nt], down[nt]);
-      over = fmaxf(over, fmaxf(fmaxf(X(d[nt][0]), Y(d[nt][0])), fmaxf(X(d[nt][1]), Y(d[nt][1]))));
-    }
+    for (int h = 0; h < TT; ++h)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          d[h][nt][k] = Fma2(Make2(t[h][nt][2 * k], t[h][nt][2 * k + 1]), scale[nt], down[nt]);
+          over = fmaxf(over, fmaxf(X(d[h][nt][k]), Y(d[h][nt][k])));
+        }
     if (__any_sync(0xffffffffu, over > kRescale - kShift)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -404,7 +499,10 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float was = e ? Y(down[nt]) : X(down[nt]);
-          float top = fmaxf(t[nt][e], t[nt][e + 2]) * (e ? Y(scale[nt]) : X(scale[nt]));
+          float top = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < TT; ++h) top = fmaxf(top, fmaxf(t[h][nt][e], t[h][nt][e + 2]));
+          top *= e ? Y(scale[nt]) : X(scale[nt]);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -421,21 +519,28 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
         }
 #pragma unroll
         for (int x = 0; x < DIM / 16; ++x) { o[nt][x][0] *= f[0]; o[nt][x][1] *= f[1]; o[nt][x][2] *= f[0]; o[nt][x][3] *= f[1]; }
-        d[nt][0] = Fma2(Make2(t[nt][0], t[nt][1]), scale[nt], down[nt]);
-        d[nt][1] = Fma2(Make2(t[nt][2], t[nt][3]), scale[nt], down[nt]);
+#pragma unroll
+        for (int h = 0; h < TT; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) d[h][nt][k] = Fma2(Make2(t[h][nt][2 * k], t[h][nt][2 * k + 1]), scale[nt], down[nt]);
       }
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      t[nt][0] = Exp2(X(d[nt][0])); t[nt][1] = Exp2(Y(d[nt][0]));
-      t[nt][2] = Exp2(X(d[nt][1])); t[nt][3] = Exp2(Y(d[nt][1]));
-      l[nt] = Add2(l[nt], Add2(Make2(t[nt][0], t[nt][1]), Make2(t[nt][2], t[nt][3])));
-    }
+    for (int h = 0; h < TT; ++h)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[h][nt][e] = Exp2(e & 1 ? Y(d[h][nt][e >> 1]) : X(d[h][nt][e >> 1]));
+        l[nt] = Add2(l[nt], Add2(Make2(t[h][nt][0], t[h][nt][1]), Make2(t[h][nt][2], t[h][nt][3])));
+      }
 
+#pragma unroll
+    for (int h = 0; h < TT; ++h) {
+    const uint32_t sh = st + h * kTileBytes;
     // ---- values: weights times the group's steps as the 8-column operand, codes of 16 channels as rows
     uint32_t vp0[NG], vp1[NG];
-    Lds<NG>(vp0, smem + st + pars_at + kPars);
-    Lds<NG>(vp1, smem + st + pars_at + kPars + 8 * NG * 4);
+    Lds<NG>(vp0, smem + sh + pars_at + kPars);
+    Lds<NG>(vp1, smem + sh + pars_at + kPars + 8 * NG * 4);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float2 p0 = Pair(vp0[g]), p1 = Pair(vp1[g]);
@@ -448,12 +553,12 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
         for (int e = 0; e < 4; ++e) {
           const float step = e < 2 ? p0.y : p1.y;
           if constexpr (decltype(part)::value) {  // an unseen row's lo and step may be anything
-            const bool on = ((seen >> (4 * nt + e)) & 1u) != 0u;
-            w[e] = on ? t[nt][e] * step : 0.f;
-            z[e & 1] = on ? fmaf(t[nt][e], mid[e >> 1], z[e & 1]) : z[e & 1];
+            const bool on = ((seen >> (16 * h + 4 * nt + e)) & 1u) != 0u;
+            w[e] = on ? t[h][nt][e] * step : 0.f;
+            z[e & 1] = on ? fmaf(t[h][nt][e], mid[e >> 1], z[e & 1]) : z[e & 1];
           } else {
-            w[e] = t[nt][e] * step;
-            z[e & 1] = fmaf(t[nt][e], mid[e >> 1], z[e & 1]);
+            w[e] = t[h][nt][e] * step;
+            z[e & 1] = fmaf(t[h][nt][e], mid[e >> 1], z[e & 1]);
           }
         }
         zsum[nt][g] = Make2(z[0], z[1]);
@@ -462,7 +567,7 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
         const uint32_t eights[4] = {kMiddle, kMiddle, kMiddle, kMiddle};
         Mma(middle[nt][g], eights, b0[nt], b1[nt]);
       }
-      const uint8_t *fa = smem + ((st + value_at0) ^ (g * (GROUP / 2))), *fb = smem + ((st + value_at1) ^ (g * (GROUP / 2)));
+      const uint8_t *fa = smem + ((sh + value_at0) ^ (g * (GROUP / 2))), *fb = smem + ((sh + value_at1) ^ (g * (GROUP / 2)));
       uint32_t x[4][kW > 1 ? kW / 2 : 1];   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
       if constexpr (kW == 1) {
         x[0][0] = *reinterpret_cast<const uint16_t*>(fa); x[1][0] = *reinterpret_cast<const uint16_t*>(fb);
@@ -484,27 +589,29 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
         }
       }
     }
+    }
   };
 
 #pragma unroll
   for (int n = 0; n < kStages - 1; ++n) {
-    if (n < mine) issue(n);
+    if (n < mine) issue(n, n);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  for (int n = 0; n < mine; ++n) {
+  for (int n = 0, stage = 0; n < mine; ++n) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();
-    if (n + kStages - 1 < mine) issue(n + kStages - 1);
+    if (n + kStages - 1 < mine) issue(n + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const int stage = n & (kStages - 1);
     const uint32_t st = ring + stage * kStage;
-    const int j0 = begin + (warp + n * kWarps) * kTile;
-    const uint32_t ok = PAGE16 ? (((there >> n) & 1u) ? 0xffffu : 0u) : s_ok[warp][stage];
+    const int j0 = begin + (warp + n * kWarps) * (TT * kTile);
+    const uint32_t ok = s_ok[warp][stage];
+    constexpr uint32_t kAll = TT == 2 ? 0xffffffffu : 0xffffu;
 
     // two copies of the code: tiles that not every row sees whole carry masks
-    if (j0 < all_begin || j0 + kTile > all_end || ok != 0xffffu) compute(std::true_type{}, st, j0, ok);
-    else compute(std::false_type{}, st, j0, ok);
+    if (ok == kAll && j0 >= all_begin && j0 + TT * kTile <= all_end) compute(std::false_type{}, st, j0, ok);
+    else if (ok != 0u) compute(std::true_type{}, st, j0, ok);
     __syncwarp();
+    stage = stage == kStages - 1 ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();   // the rings become the warps' results
@@ -535,7 +642,8 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
       }
     }
   __syncthreads();
-  const int64_t part_row = (int64_t(b) * a.c.kv_heads + kvh) * (int64_t(a.max_new) * a.share) + row0;
+  const bool whole = ntiles == tiles;
+  const int64_t part = (int64_t(blockIdx.x) * 2 + (tile0 == 0)) * kRows;
   for (int x = threadIdx.x; x < min(kRows, rows - row0) * (DIM / 2); x += kThreads) {
     const int row = x / (DIM / 2), d = 2 * (x - row * (DIM / 2));
     float top = kNone;
@@ -551,55 +659,66 @@ __global__ void __launch_bounds__(kThreads) StepsKernel(const __grid_constant__ 
       v0 = fmaf(v.x, f, v0);
       v1 = fmaf(v.y, f, v1);
     }
-    if (s.part_o != nullptr) {
-      const int64_t at = (part_row + row) * s.chunks + blockIdx.x;
-      *reinterpret_cast<float2*>(s.part_o + at * DIM + d) = make_float2(v0, v1);
-      if (d == 0) s.part_ml[at] = make_float2(top, sum);
+    if (!whole) {
+      *reinterpret_cast<float2*>(s.part_o + (part + row) * DIM + d) = make_float2(v0, v1);
+      if (d == 0) s.part_ml[part + row] = make_float2(top, sum);
     } else {
       const int rr = row0 + row, i = int(QuickDiv(uint32_t(rr), a.div_share)), h = kvh * a.share + rr - i * a.share;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      StoreOut(a, s.bf16, (q.row0 + i) * a.ot + int64_t(h) * a.oh + d, v0 * inv);
-      StoreOut(a, s.bf16, (q.row0 + i) * a.ot + int64_t(h) * a.oh + d + 1, v1 * inv);
+      const int64_t at = (q.row0 + i) * a.ot + int64_t(h) * a.oh + d;
+      StoreOut(a, s.bf16, at, v0 * inv);
+      StoreOut(a, s.bf16, at + 1, v1 * inv);
     }
+  }
+  __syncthreads();   // the results become rings again
   }
 }
 
-// Joins the chunks of one query row: WARPS warps take them in turn, the parts are then added in the warps' order.
-template <int DIM, int WARPS>
+// Joins one query row of a unit that several blocks worked on: WARPS warps take the blocks' results in turn, the warps' sums
+// are then added in their order.  Rows that see nothing are set to zero here.
+template <int DIM, int NT, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) JoinKernel(const __grid_constant__ StepArgs s) {
   constexpr int E = DIM / 32;
   constexpr int kBlockRows = WARPS == 1 ? 4 : 1;
   __shared__ float s_o[WARPS == 1 ? 1 : WARPS][WARPS == 1 ? 1 : DIM];
   __shared__ float s_l[WARPS];
   const AttnArgs& a = s.a;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = WARPS == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int max_rows = a.max_new * a.share;
   const int rr = int(blockIdx.x) * kBlockRows + (WARPS == 1 ? int(threadIdx.x >> 5) : 0), kvh = blockIdx.y, b = blockIdx.z;
-  if (rr >= max_rows) return;
   const Seq q = SeqOf(a, b, false);
+  const int tiles = SeqTiles(a, q);
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // every block, so that this kernel does not end before the first one
   if (rr >= q.nnew * a.share) return;
-  const int i = int(QuickDiv(uint32_t(rr), a.div_share)), h = kvh * a.share + rr - i * a.share;
-  const int begin = RowBegin(a, q, 0) & ~(kTile - 1), end = RowEnd(a, q, q.nnew - 1);
-  const int chunks = end > begin ? (end - begin + s.chunk - 1) / s.chunk : 0;
-  const int64_t at = ((int64_t(b) * a.c.kv_heads + kvh) * max_rows + rr) * s.chunks;
+  const int row = rr % (8 * NT);
+  int64_t c0 = 0, c1 = -1;
+  if (tiles > 0) {
+    const int64_t total = s.list[0], blocks = s.list[1];
+    const int64_t x = s.list[2 + b] + (int64_t(kvh) * s.row_tiles + rr / (8 * NT)) * tiles;
+    c0 = ((x + 1) * blocks - 1) / total;              // the block that holds tile x
+    c1 = ((x + tiles) * blocks - 1) / total;
+    if (c0 == c1) return;                             // it wrote the row
+  }
+  const int parts = int(c1 - c0) + 1;
+  // the unit begins in block c0 (its second result) and goes on in the others (their first)
+  auto at = [&](int i) { return ((c0 + i) * 2 + (i == 0)) * (8 * NT) + row; };
   float top = kNone;
-  for (int x = lane; x < chunks; x += 32) top = fmaxf(top, s.part_ml[at + x].x);
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, s.part_ml[at(i)].x);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   float o[E], sum = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-  for (int x = warp; x < chunks; x += WARPS) {
-    const float2 ml = s.part_ml[at + x];
+  for (int i = warp; i < parts; i += WARPS) {
+    const float2 ml = s.part_ml[at(i)];
     float v[E];
-    LoadVec<float, E>(s.part_o + (at + x) * DIM + lane * E, v);
+    LoadVec<float, E>(s.part_o + at(i) * DIM + lane * E, v);
     const float f = PartWeight(ml.x, ml.y, top);
     sum = fmaf(ml.y, f, sum);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], f, o[e]);
   }
+  const int i = int(QuickDiv(uint32_t(rr), a.div_share)), h = kvh * a.share + rr - i * a.share;
   const int64_t out = (q.row0 + i) * a.ot + int64_t(h) * a.oh;
   if (WARPS > 1) {
 #pragma unroll
@@ -621,41 +740,38 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) JoinKernel(cons
   }
 }
 
-struct Plan { int nt, row_tiles, chunk, chunks; };
+struct Plan { int nt, row_tiles; int64_t tiles; };
 
 Plan PlanSteps(const AttnArgs& a) {
   Plan p;
   const int rows = a.max_new * a.share;
   p.nt = rows > 8 && a.c.head_dim < 256 ? 2 : 1;   // 16 columns of 256 channels would not fit a thread's registers
   p.row_tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
-  // tokens that the widest sequence's chunks cover
   int64_t span = std::min<int64_t>(a.max_kept, int64_t(a.table_cols) * a.c.page_size);
   if (a.window > 0) span = std::min<int64_t>(span, int64_t(a.window) + a.max_new + kTile);
-  const int64_t units = int64_t(a.num_seqs) * a.c.kv_heads * p.row_tiles;
-  const int64_t step = kTile * kWarps;
-  const int64_t want = (span * units + 148 * 4 - 1) / (148 * 4);
-  p.chunk = int(std::min<int64_t>(kMaxChunk, std::max<int64_t>(2 * step, (want + step - 1) / step * step)));
-  p.chunks = int(std::max<int64_t>(1, (span + p.chunk - 1) / p.chunk));
+  p.tiles = (span + kTile - 1) / kTile * a.num_seqs * a.c.kv_heads * p.row_tiles;   // at most
   return p;
 }
 
-int64_t PartRows(const AttnArgs& a, const Plan& p) { return int64_t(a.num_seqs) * a.q_heads * a.max_new * p.chunks; }
+size_t PartBytes(const AttnArgs& a, const Plan& p) { return size_t(kMaxBlocks) * 2 * 8 * p.nt * (size_t(a.c.head_dim) * sizeof(float) + sizeof(float2)); }
 
-template <typename K> int Prepare(K kernel, size_t smem) {
-  if (smem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-  return ITEXB_OK;
-}
-
-template <int DIM, int GROUP, int NT, bool PAGE16> int LaunchKernel(const StepArgs& s, cudaStream_t st) {
-  constexpr size_t kStage = 2 * kTile * (DIM / 2) + 2 * kTile * (DIM / GROUP) * 4;
-  constexpr size_t kRing = kWarps * kStages * kStage, kJoin = size_t(kWarps) * 8 * NT * (DIM * 4 + 8);
+template <int DIM, int GROUP, int NT, bool PAGE16> int LaunchKernel(const StepArgs& s, const Plan& p, cudaStream_t st, int* blocks) {
+  constexpr size_t kStage = kTogether<DIM, NT> * (2 * kTile * (DIM / 2) + 2 * kTile * (DIM / GROUP) * 4);
+  constexpr size_t kRing = kWarps * kStagesOf<DIM, NT> * kStage, kJoin = size_t(kWarps) * 8 * NT * (DIM * 4 + 8);
   constexpr size_t kSmem = kRing > kJoin ? kRing : kJoin;
   auto kernel = StepsKernel<DIM, GROUP, NT, PAGE16>;
-  ITEXB_RETURN_IF_ERROR(Prepare(kernel, kSmem));
-  kernel<<<dim3(s.chunks, s.a.c.kv_heads * s.row_tiles, s.a.num_seqs), kThreads, kSmem, st>>>(s);
+  static std::atomic<int> resident{0};   // blocks per SM; the same for every device of this kind
+  int per_sm = resident.load(std::memory_order_relaxed);
+  if (kSmem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
+  if (per_sm == 0) {
+    ITEXB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kSmem));
+    resident.store(per_sm, std::memory_order_relaxed);
+  }
+  *blocks = int(std::min<int64_t>(std::min(kMaxBlocks, per_sm * SmCount()), std::max<int64_t>(1, p.tiles / kLeastTiles)));
+  kernel<<<*blocks, kThreads, kSmem, st>>>(s);
   return CheckLaunch("StepsKernel");
 }
-template <int DIM, int WARPS> int LaunchJoin(const StepArgs& s, cudaStream_t st) {
+template <int DIM, int NT, int WARPS> int LaunchJoin(const StepArgs& s, cudaStream_t st) {
   const int rows = s.a.max_new * s.a.share;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(WARPS == 1 ? (rows + 3) / 4 : rows, s.a.c.kv_heads, s.a.num_seqs);
@@ -667,58 +783,49 @@ template <int DIM, int WARPS> int LaunchJoin(const StepArgs& s, cudaStream_t st)
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  ITEXB_CUDA(cudaLaunchKernelEx(&cfg, JoinKernel<DIM, WARPS>, s));
+  ITEXB_CUDA(cudaLaunchKernelEx(&cfg, JoinKernel<DIM, NT, WARPS>, s));
   return CheckLaunch("JoinKernel");
 }
-template <int DIM, int GROUP, int NT> int LaunchPage(const StepArgs& s, cudaStream_t st) {
-  if (s.a.c.page_size % kTile == 0) return LaunchKernel<DIM, GROUP, NT, true>(s, st);
-  return LaunchKernel<DIM, GROUP, NT, false>(s, st);
+template <int DIM, int GROUP, int NT> int LaunchPage(const StepArgs& s, const Plan& p, cudaStream_t st) {
+  int blocks = 0;
+  if (s.a.c.page_size % kTile == 0) ITEXB_RETURN_IF_ERROR((LaunchKernel<DIM, GROUP, NT, true>(s, p, st, &blocks)));
+  else ITEXB_RETURN_IF_ERROR((LaunchKernel<DIM, GROUP, NT, false>(s, p, st, &blocks)));
+  // more than 8 results per unit: a block of 8 warps adds them up, else a warp
+  if (blocks > 8 * int64_t(s.a.num_seqs) * s.units) return LaunchJoin<DIM, NT, 8>(s, st);
+  return LaunchJoin<DIM, NT, 1>(s, st);
 }
-template <int DIM, int GROUP> int LaunchGroup(const StepArgs& s, int nt, cudaStream_t st) {
-  if constexpr (GROUP <= DIM) {
-    if constexpr (DIM < 256) {
-      ITEXB_RETURN_IF_ERROR((nt == 1 ? LaunchPage<DIM, GROUP, 1>(s, st) : LaunchPage<DIM, GROUP, 2>(s, st)));
-    } else {
-      ITEXB_RETURN_IF_ERROR((LaunchPage<DIM, GROUP, 1>(s, st)));
-    }
-    if (s.part_o == nullptr) return ITEXB_OK;
-    return s.chunks > 8 ? LaunchJoin<DIM, 8>(s, st) : LaunchJoin<DIM, 1>(s, st);
-  } else {
+template <int DIM, int GROUP> int LaunchGroup(const StepArgs& s, const Plan& p, cudaStream_t st) {
+  if constexpr (GROUP > DIM) {
     return SetError(ITEXB_INTERNAL, "kv4_attention: group above head_dim");
+  } else if constexpr (DIM < 256) {
+    return p.nt == 1 ? LaunchPage<DIM, GROUP, 1>(s, p, st) : LaunchPage<DIM, GROUP, 2>(s, p, st);
+  } else {
+    return LaunchPage<DIM, GROUP, 1>(s, p, st);
   }
 }
-template <int DIM> int LaunchDim(const StepArgs& s, int nt, cudaStream_t st) {
-  if (s.a.c.group == 32) return LaunchGroup<DIM, 32>(s, nt, st);
-  if (s.a.c.group == 64) return LaunchGroup<DIM, 64>(s, nt, st);
-  return LaunchGroup<DIM, 128>(s, nt, st);
-}
-int LaunchType(const StepArgs& s, int nt, cudaStream_t st) {
-  if (s.a.c.head_dim == 64) return LaunchDim<64>(s, nt, st);
-  if (s.a.c.head_dim == 128) return LaunchDim<128>(s, nt, st);
-  return LaunchDim<256>(s, nt, st);
+template <int DIM> int LaunchDim(const StepArgs& s, const Plan& p, cudaStream_t st) {
+  if (s.a.c.group == 32) return LaunchGroup<DIM, 32>(s, p, st);
+  if (s.a.c.group == 64) return LaunchGroup<DIM, 64>(s, p, st);
+  return LaunchGroup<DIM, 128>(s, p, st);
 }
 
 }  // namespace
 
-size_t StepsWorkspace(const AttnArgs& a) {
-  const Plan p = PlanSteps(a);
-  return p.chunks == 1 ? 0 : size_t(PartRows(a, p)) * (size_t(a.c.head_dim) * sizeof(float) + sizeof(float2));
-}
+size_t StepsWorkspace(const AttnArgs& a) { return PartBytes(a, PlanSteps(a)) + (size_t(a.num_seqs) + 2) * sizeof(int64_t); }
 
 int LaunchSteps(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st) {
   const Plan p = PlanSteps(a);
-  ITEXB_REQUIRE(int64_t(a.c.kv_heads) * p.row_tiles <= 65535, ITEXB_INVALID_ARGUMENT, "kv4_attention: too many query rows");
   StepArgs s{};
   s.a = a;
-  s.chunk = p.chunk;
-  s.chunks = p.chunks;
   s.row_tiles = p.row_tiles;
-  if (p.chunks > 1) {
-    s.part_o = static_cast<float*>(workspace);
-    s.part_ml = reinterpret_cast<float2*>(s.part_o + PartRows(a, p) * a.c.head_dim);
-  }
+  s.units = a.c.kv_heads * p.row_tiles;
   s.bf16 = dtype == ITEXB_DT_BFLOAT16;
-  return LaunchType(s, p.nt, st);
+  s.part_o = static_cast<float*>(workspace);
+  s.part_ml = reinterpret_cast<float2*>(s.part_o + size_t(kMaxBlocks) * 2 * 8 * p.nt * a.c.head_dim);
+  s.list = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(workspace) + PartBytes(a, p));
+  if (a.c.head_dim == 64) return LaunchDim<64>(s, p, st);
+  if (a.c.head_dim == 128) return LaunchDim<128>(s, p, st);
+  return LaunchDim<256>(s, p, st);
 }
 
 }  // namespace itexb
