@@ -5,6 +5,7 @@ object has not been built the import fails with the build command to run.
 """
 import ctypes as C
 import os
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "lib", "libitexb200.so")
@@ -144,6 +145,22 @@ class Kv4AttentionParams(C.Structure):
         " workspace; size workspace_bytes")
 
 
+def packer(kind):
+    """The pack function of a struct.Struct with the layout of a ctypes Structure, nested ones flattened: filling 30 fields takes a
+    microsecond this way, four as a Structure."""
+    codes = {C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
+
+    def fields(k):
+        return "".join(fields(t) if issubclass(t, C.Structure) else codes[t] for _, t in k._fields_)
+
+    made = struct.Struct("@" + fields(kind))
+    assert made.size == C.sizeof(kind), kind
+    return made.pack
+
+
+pack_rope, pack_qk_norm_rope, pack_qk_norm_rope_grad = packer(RopeParams), packer(QkNormRopeParams), packer(QkNormRopeGradParams)
+pack_kv4_append, pack_kv4_gather, pack_kv4_attention = packer(Kv4AppendParams), packer(Kv4GatherParams), packer(Kv4AttentionParams)
+
 # itexb_status words of the decoder operators
 STATUS_BAD_INDEX, STATUS_WAIT_EXPIRED = 6, 7
 
@@ -187,12 +204,11 @@ def load():
     lib.itexb_peer_signal.argtypes = [C.POINTER(C.c_void_p), C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
     lib.itexb_peer_wait.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.itexb_peer_advance.argtypes = [C.c_void_p, C.c_void_p]
-    for name, params in (("rope", RopeParams), ("qk_norm_rope", QkNormRopeParams), ("qk_norm_rope_grad", QkNormRopeGradParams),
-                         ("kv4_append", Kv4AppendParams), ("kv4_gather", Kv4GatherParams), ("kv4_attention", Kv4AttentionParams)):
-        getattr(lib, "itexb_" + name).argtypes = [C.POINTER(params), C.c_void_p]
+    for name in ("rope", "qk_norm_rope", "qk_norm_rope_grad", "kv4_append", "kv4_gather", "kv4_attention"):
+        getattr(lib, "itexb_" + name).argtypes = [C.c_void_p, C.c_void_p]    # a params struct, or its bytes
     lib.itexb_qk_norm_rope_grad_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
     lib.itexb_qk_norm_rope_grad_workspace_bytes.restype = C.c_size_t
-    lib.itexb_kv4_attention_workspace_bytes.argtypes = [C.POINTER(Kv4AttentionParams)]
+    lib.itexb_kv4_attention_workspace_bytes.argtypes = [C.c_void_p]
     lib.itexb_kv4_attention_workspace_bytes.restype = C.c_size_t
     _lib = lib
     return lib

@@ -150,15 +150,23 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
   __shared__ int64_t s_sum[kWarps];
   __shared__ int64_t s_pos, s_stop, s_rest;           // place in the list, its end for this block; tiles of sequence s_seq before it
   __shared__ int s_seq;
+  __shared__ Seq s_q;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
 
+  // Launched programmatically: what the previous kernel of the stream wrote is visible from here on.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // ---- this block's part of the list of tiles
   {
     const int per = (a.num_seqs + kThreads - 1) / kThreads;
     const int b0 = min(a.num_seqs, int(threadIdx.x) * per), b1 = min(a.num_seqs, b0 + per);
+    Seq one{};              // of sequence b0: the only one of this thread where there are at most 128
     int64_t sum = 0;
-    for (int x = b0; x < b1; ++x) sum += int64_t(SeqTiles(a, SeqOf(a, x, blockIdx.x == 0))) * s.units;
+    for (int x = b0; x < b1; ++x) {
+      const Seq q = SeqOf(a, x, blockIdx.x == 0);
+      if (x == b0) one = q;
+      sum += int64_t(SeqTiles(a, q)) * s.units;
+    }
     int64_t before = sum;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
@@ -175,25 +183,21 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
     }
     before -= sum;
     const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / kLeastTiles));
-    if (blockIdx.x == 0) {  // for the joining kernel
-      if (threadIdx.x == 0) { s.list[0] = total; s.list[1] = blocks; }
-      int64_t at = before;
-      for (int x = b0; x < b1; ++x) {
-        s.list[2 + x] = at;
-        at += int64_t(SeqTiles(a, SeqOf(a, x, false))) * s.units;
-      }
-    }
     const int64_t pos = BlockStart(total, blocks, blockIdx.x);
     const int64_t stop = blockIdx.x < blocks ? BlockStart(total, blocks, blockIdx.x + 1) : pos;
     if (threadIdx.x == 0) { s_pos = pos; s_stop = stop; }
-    if (pos >= before && pos < before + sum) {
+    const bool mine = pos >= before && pos < before + sum;
+    if (mine || blockIdx.x == 0) {
+      if (threadIdx.x == 0 && blockIdx.x == 0) { s.list[0] = total; s.list[1] = blocks; }   // for the joining kernel
       int64_t at = before;
       for (int x = b0; x < b1; ++x) {
-        const int64_t n = int64_t(SeqTiles(a, SeqOf(a, x, false))) * s.units;
-        if (pos < at + n) {
+        const Seq q = x == b0 ? one : SeqOf(a, x, false);
+        const int64_t n = int64_t(SeqTiles(a, q)) * s.units;
+        if (blockIdx.x == 0) s.list[2 + x] = at;
+        if (mine && pos >= at && pos < at + n) {
           s_seq = x;
+          s_q = q;
           s_rest = pos - at;
-          break;
         }
         at += n;
       }
@@ -211,103 +215,36 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
 
   while (s_pos < s_stop) {
   const int b = s_seq;
-  const Seq q = SeqOf(a, b, false);
-  const int tiles = SeqTiles(a, q);
+  const Seq q = s_q;
+  const int tiles = SeqTiles(a, q);      // not 0
   const int64_t rest = s_rest;
-  const int unit = tiles > 0 ? int(rest / tiles) : s.units;
+  const int unit = int(rest / tiles);
   const int tile0 = int(rest - int64_t(unit) * tiles), tile1 = int(min(int64_t(tiles), tile0 + (s_stop - s_pos)));
   __syncthreads();
   if (threadIdx.x == 0) {
-    if (unit < s.units) {
-      s_pos += tile1 - tile0;
-      s_rest += tile1 - tile0;
-    } else {               // the next sequence that has any
-      s_rest -= int64_t(tiles) * s.units;
-      s_seq = b + 1;
+    s_pos += tile1 - tile0;
+    s_rest = rest + (tile1 - tile0);
+    if (s_rest == int64_t(tiles) * s.units && s_pos < s_stop) {   // on to the next sequence that has any
+      int x = b + 1;
+      Seq next = SeqOf(a, x, false);
+      while (SeqTiles(a, next) == 0) next = SeqOf(a, ++x, false);
+      s_seq = x;
+      s_q = next;
+      s_rest = 0;
     }
   }
-  __syncthreads();
   const int kvh = unit / s.row_tiles, rt = unit - kvh * s.row_tiles;
   const int rows = q.nnew * a.share, row0 = rt * 8 * NT;
-  if (unit >= s.units || row0 >= rows) continue;   // a sequence shorter than the longest has fewer row tiles
+  if (row0 >= rows) {   // a sequence shorter than the longest has fewer row tiles
+    __syncthreads();
+    continue;
+  }
   // the tokens that some row of this unit sees, and those that all of them see
   const int i_first = int(QuickDiv(uint32_t(row0), a.div_share)), i_last = int(QuickDiv(uint32_t(min(rows, row0 + 8 * NT) - 1), a.div_share));
   const int some_begin = RowBegin(a, q, i_first), some_end = RowEnd(a, q, i_last);
   const int all_begin = RowBegin(a, q, i_last), all_end = RowEnd(a, q, i_first);
   const int begin = (RowBegin(a, q, 0) & ~(kTile - 1)) + tile0 * kTile;
   const int ntiles = tile1 - tile0;
-
-  // ---- query rows as the 8-column operand, and their sums per group times 2^-24
-  uint32_t qf[NT][DIM / 16][2];
-  F2 qs[NT][NG], scale[NT];              // of columns 2c, 2c + 1
-  int lo[NT][2], hi[NT][2];              // visible tokens of those columns
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int rr = row0 + nt * 8 + r;
-    const bool on = rr < rows;
-    const int i = int(QuickDiv(uint32_t(on ? rr : row0), a.div_share)), h = (on ? rr : row0) - i * a.share;
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (q.row0 + i) * a.qt + int64_t(kvh * a.share + h) * a.qh;
-    union Piece { uint4 v; uint32_t u[4]; uint16_t e[8]; } x[NG][kW];
-    float most = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int w = 0; w < kW; ++w) {
-        const int d = g * GROUP + c * (GROUP / 4) + w * 8;
-        if (!on) x[g][w].v = make_uint4(0, 0, 0, 0);
-        else if (a.q_aligned) x[g][w].v = *reinterpret_cast<const uint4*>(src + d);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[g][w].e[e] = src[d + e];
-        if (s.bf16)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x[g][w].e[e]) << 16)));
-      }
-    // q * down is exact but for underflow; scores are (codes' product) * up, up > 0
-    float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f), up = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-    if (s.bf16) {
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
-      if (most > 0.f && most < INFINITY) {
-        down *= __uint_as_float(uint32_t(254 - e) << 23);
-        up = fmaxf(up * __uint_as_float(uint32_t(e) << 23), 1e-37f);
-      }
-    }
-    up *= kUnit;
-    scale[nt] = Make2(__shfl_sync(0xffffffffu, up, (2 * c) * 4), __shfl_sync(0xffffffffu, up, (2 * c + 1) * 4));
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kW; ++w) {
-        Piece& y = x[g][w];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float raw = s.bf16 ? __uint_as_float(uint32_t(y.e[e]) << 16) : __half2float(__ushort_as_half(y.e[e]));
-          const float f = raw * down;
-          sum += f;
-          y.e[e] = __half_as_ushort(__float2half_rn(e & 1 ? f * 0.0625f : f));
-        }
-        // a word's codes come out in pairs (j, j + 4)
-        const int ks = (g * kW + w) * 2;
-        qf[nt][ks][0] = __byte_perm(y.u[0], y.u[2], 0x5410);
-        qf[nt][ks][1] = __byte_perm(y.u[0], y.u[2], 0x7632);
-        qf[nt][ks + 1][0] = __byte_perm(y.u[1], y.u[3], 0x5410);
-        qf[nt][ks + 1][1] = __byte_perm(y.u[1], y.u[3], 0x7632);
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= 1.f / kUnit;
-      qs[nt][g] = Make2(__shfl_sync(0xffffffffu, sum, (2 * c) * 4), __shfl_sync(0xffffffffu, sum, (2 * c + 1) * 4));
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int ii = int(QuickDiv(uint32_t(min(rows - 1, row0 + nt * 8 + 2 * c + e)), a.div_share));  // a column without a row: any bounds
-      lo[nt][e] = RowBegin(a, q, ii);
-      hi[nt][e] = RowEnd(a, q, ii);
-    }
-  }
 
   // ---- steps of TT tiles: w, w + 4, ...
   const int nsteps = (ntiles + TT - 1) / TT;
@@ -399,6 +336,83 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
     }
     if (lane == 0) s_ok[warp][stage] = rows_there;
   };
+
+#pragma unroll
+  for (int n = 0; n < kStages - 1; ++n) {
+    if (n < mine) issue(n, n);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // ---- query rows as the 8-column operand, and their sums per group times 2^-24
+  uint32_t qf[NT][DIM / 16][2];
+  F2 qs[NT][NG], scale[NT];              // of columns 2c, 2c + 1
+  int lo[NT][2], hi[NT][2];              // visible tokens of those columns
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int rr = row0 + nt * 8 + r;
+    const bool on = rr < rows;
+    const int i = int(QuickDiv(uint32_t(on ? rr : row0), a.div_share)), h = (on ? rr : row0) - i * a.share;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (q.row0 + i) * a.qt + int64_t(kvh * a.share + h) * a.qh;
+    union Piece { uint4 v; uint32_t u[4]; uint16_t e[8]; } x[NG][kW];
+    float most = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        const int d = g * GROUP + c * (GROUP / 4) + w * 8;
+        if (!on) x[g][w].v = make_uint4(0, 0, 0, 0);
+        else if (a.q_aligned) x[g][w].v = *reinterpret_cast<const uint4*>(src + d);
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[g][w].e[e] = src[d + e];
+        if (s.bf16)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x[g][w].e[e]) << 16)));
+      }
+    // q * down is exact but for underflow; scores are (codes' product) * up, up > 0
+    float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f), up = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+    if (s.bf16) {
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
+      if (most > 0.f && most < INFINITY) {
+        down *= __uint_as_float(uint32_t(254 - e) << 23);
+        up = fmaxf(up * __uint_as_float(uint32_t(e) << 23), 1e-37f);
+      }
+    }
+    up *= kUnit;
+    scale[nt] = Make2(__shfl_sync(0xffffffffu, up, (2 * c) * 4), __shfl_sync(0xffffffffu, up, (2 * c + 1) * 4));
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        Piece& y = x[g][w];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float raw = s.bf16 ? __uint_as_float(uint32_t(y.e[e]) << 16) : __half2float(__ushort_as_half(y.e[e]));
+          const float f = raw * down;
+          sum += f;
+          y.e[e] = __half_as_ushort(__float2half_rn(e & 1 ? f * 0.0625f : f));
+        }
+        // a word's codes come out in pairs (j, j + 4)
+        const int ks = (g * kW + w) * 2;
+        qf[nt][ks][0] = __byte_perm(y.u[0], y.u[2], 0x5410);
+        qf[nt][ks][1] = __byte_perm(y.u[0], y.u[2], 0x7632);
+        qf[nt][ks + 1][0] = __byte_perm(y.u[1], y.u[3], 0x5410);
+        qf[nt][ks + 1][1] = __byte_perm(y.u[1], y.u[3], 0x7632);
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= 1.f / kUnit;
+      qs[nt][g] = Make2(__shfl_sync(0xffffffffu, sum, (2 * c) * 4), __shfl_sync(0xffffffffu, sum, (2 * c + 1) * 4));
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int ii = int(QuickDiv(uint32_t(min(rows - 1, row0 + nt * 8 + 2 * c + e)), a.div_share));  // a column without a row: any bounds
+      lo[nt][e] = RowBegin(a, q, ii);
+      hi[nt][e] = RowEnd(a, q, ii);
+    }
+  }
 
   float o[NT][DIM / 16][4], middle[NT][NG][4];   // sums times 2^-24; the odd channels' (2, 3) are 16 times as large
   F2 zsum[NT][NG], l[NT];
@@ -592,11 +606,6 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
     }
   };
 
-#pragma unroll
-  for (int n = 0; n < kStages - 1; ++n) {
-    if (n < mine) issue(n, n);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
   for (int n = 0, stage = 0; n < mine; ++n) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();
@@ -688,6 +697,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) JoinKernel(cons
   const Seq q = SeqOf(a, b, false);
   const int tiles = SeqTiles(a, q);
   asm volatile("griddepcontrol.wait;" ::: "memory");   // every block, so that this kernel does not end before the first one
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (rr >= q.nnew * a.share) return;
   const int row = rr % (8 * NT);
   int64_t c0 = 0, c1 = -1;
@@ -768,7 +778,17 @@ template <int DIM, int GROUP, int NT, bool PAGE16> int LaunchKernel(const StepAr
     resident.store(per_sm, std::memory_order_relaxed);
   }
   *blocks = int(std::min<int64_t>(std::min(kMaxBlocks, per_sm * SmCount()), std::max<int64_t>(1, p.tiles / kLeastTiles)));
-  kernel<<<*blocks, kThreads, kSmem, st>>>(s);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(*blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ITEXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, s));
   return CheckLaunch("StepsKernel");
 }
 template <int DIM, int NT, int WARPS> int LaunchJoin(const StepArgs& s, cudaStream_t st) {

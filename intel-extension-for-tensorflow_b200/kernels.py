@@ -196,67 +196,74 @@ def matmul_scales_dynamic(range3, weight_range, a_dtype, out=None):
 
 
 # ---- decoder operators: rotary positions and per-head norms (the 4-bit cache and its attention: kv4.py) ----
+# A decoding step is short: what these functions do before the launch is kept to about ten microseconds.
 _INDEX_DT = {torch.int32: L.DT_INT32, torch.int64: L.DT_INT64}
 _REAL_DT = {torch.float32: L.DT_FLOAT, torch.bfloat16: L.DT_BFLOAT16, torch.float16: L.DT_HALF}
+_FLOAT64 = {torch.float64: 0}
 
 
 def _rows(t, name, like=None):
     """Checks a [tokens, heads, head_dim] tensor (innermost dimension dense, other strides free); -> (address, token stride,
-    head stride).  `like`: a tensor it must agree with in device, type and shape."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
-        raise ValueError("%s must be [tokens, heads, head_dim] with a dense last dimension, got shape %s, strides %s" % (name, tuple(t.shape), t.stride()))
-    if t.dtype not in _REAL_DT:
-        raise ValueError("%s: unsupported type %s" % (name, t.dtype))
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
-        raise ValueError("%s is %s %s, expected %s %s" % (name, t.dtype, tuple(t.shape), like.dtype, tuple(like.shape)))
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    head stride).  `like`: a tensor it must agree with in type and shape."""
+    st, sh, dt = t.stride(), t.shape, t.dtype
+    if len(st) != 3 or (st[2] != 1 and sh[2] > 1):
+        raise ValueError("%s must be [tokens, heads, head_dim] with a dense last dimension, got shape %s, strides %s" % (name, tuple(sh), st))
+    if dt not in _REAL_DT:
+        raise ValueError("%s: unsupported type %s" % (name, dt))
+    if like is not None and (dt != like.dtype or sh != like.shape):
+        raise ValueError("%s is %s %s, expected %s %s" % (name, dt, tuple(sh), like.dtype, tuple(like.shape)))
+    return t.data_ptr(), st[0], st[1]
 
 
 def _vector(t, name, kinds, n=None):
-    if t.dim() != 1 or t.dtype not in kinds or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+    sh = t.shape
+    if len(sh) != 1 or t.dtype not in kinds or (n is not None and sh[0] != n) or not t.is_contiguous():
         raise ValueError("%s must be a dense vector%s of one of %s, got %s %s" % (
-            name, "" if n is None else " of %d" % n, ", ".join(str(k) for k in kinds), t.dtype, tuple(t.shape)))
+            name, "" if n is None else " of %d" % n, ", ".join(str(k) for k in kinds), t.dtype, tuple(sh)))
     return t.data_ptr()
 
 
-def on_device_of(first, *others):
-    """The device all the tensors (None: left out) live on; raises where they do not share one CUDA device."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError("itex_b200 kernels take CUDA tensors; got a %s tensor" % dev)
-    for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError("tensors on %s and %s" % (dev, t.device))
+def device_of(*tensors):
+    """Ordinal of the device all the tensors (None: left out) live on; raises where they do not share one CUDA device."""
+    dev = tensors[0].get_device()
+    if dev < 0:
+        raise ValueError("itex_b200 kernels take CUDA tensors; got a %s tensor" % tensors[0].device)
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("tensors on %s and %s" % (tensors[0].device, t.device))
     return dev
 
 
 def launch(fn, params, dev):
-    """One C-ABI call on the tensors' device and its current stream, whichever device is current."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        L.check(fn(params, stream))
+    """One C-ABI call on device `dev` and torch's current stream there, whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        status = fn(params, stream)
     else:
         with torch.cuda.device(dev):
-            L.check(fn(params, stream))
+            status = fn(params, stream)
+    if status != L.OK:
+        L.check(status)
 
 
 def _rope_params(q, positions, inv_freq, k, interleaved, mscale, inverse, out_q, out_k):
     qp = _rows(q, "q")
     tokens, q_heads, dim = q.shape
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is None else out_q
-    oqp = _rows(oq, "out_q", q)
-    pairs = inv_freq.shape[0]
+    dt = _REAL_DT[q.dtype]
+    oq = torch.empty_like(q) if out_q is None else out_q
+    oqp = _rows(oq, "out_q", None if out_q is None else q)
     pos = _vector(positions, "positions", _INDEX_DT, tokens)
-    freq = _vector(inv_freq, "inv_freq", (torch.float64,))
+    freq = _vector(inv_freq, "inv_freq", _FLOAT64)
     if k is None:
-        return (tokens, q_heads, 0, dim, 2 * pairs, int(interleaved), int(inverse), _REAL_DT[q.dtype], _INDEX_DT[positions.dtype], mscale, pos, freq,
+        return (tokens, q_heads, 0, dim, 2 * inv_freq.shape[0], int(interleaved), int(inverse), dt, _INDEX_DT[positions.dtype], mscale, pos, freq,
                 *qp, 0, 0, 0, *oqp, 0, 0, 0), oq, None
     kp = _rows(k, "k")
-    if k.shape[0] != tokens or k.shape[2] != dim or k.dtype != q.dtype:
+    k_tokens, k_heads, k_dim = k.shape
+    if k_tokens != tokens or k_dim != dim or k.dtype != q.dtype:
         raise ValueError("k is %s %s beside q %s %s" % (k.dtype, tuple(k.shape), q.dtype, tuple(q.shape)))
-    ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is None else out_k
-    return (tokens, q_heads, k.shape[1], dim, 2 * pairs, int(interleaved), int(inverse), _REAL_DT[q.dtype], _INDEX_DT[positions.dtype], mscale, pos,
-            freq, *qp, *kp, *oqp, *_rows(ok, "out_k", k)), oq, ok
+    ok = torch.empty_like(k) if out_k is None else out_k
+    return (tokens, q_heads, k_heads, dim, 2 * inv_freq.shape[0], int(interleaved), int(inverse), dt, _INDEX_DT[positions.dtype], mscale, pos,
+            freq, *qp, *kp, *oqp, *_rows(ok, "out_k", None if out_k is None else k)), oq, ok
 
 
 def rope(q, positions, inv_freq, k=None, *, interleaved=False, mscale=1.0, inverse=False, out_q=None, out_k=None):
@@ -264,25 +271,24 @@ def rope(q, positions, inv_freq, k=None, *, interleaved=False, mscale=1.0, inver
     be strided views (columns of one projection's output).  The first 2 * len(inv_freq) elements of each head are rotated by
     positions[t] * inv_freq[i]; inv_freq (float64, on the device) and mscale come from kv4.rope_frequencies.  inverse=True is the
     transpose, i.e. the gradient.  out_q / out_k may be q / k (in place).  -> q_out, or (q_out, k_out) with k."""
-    dev = on_device_of(q, k, positions, inv_freq, out_q, out_k)
+    dev = device_of(q, k, positions, inv_freq, out_q, out_k)
     args, oq, ok = _rope_params(q, positions, inv_freq, k, interleaved, mscale, inverse, out_q, out_k)
-    launch(L.load().itexb_rope, L.RopeParams(*args), dev)
+    launch(L.load().itexb_rope, L.pack_rope(*args), dev)
     return oq if k is None else (oq, ok)
 
 
-def _norm_weights(q, k, q_weight, k_weight):
-    wq = _vector(q_weight, "q_weight", _REAL_DT, q.shape[-1])
-    wk = _vector(k_weight, "k_weight", (q_weight.dtype,), q.shape[-1])
+def _norm_weights(q, q_weight, k_weight):
+    wq = _vector(q_weight, "q_weight", _REAL_DT, q.shape[2])
+    wk = _vector(k_weight, "k_weight", (q_weight.dtype,), q.shape[2])
     return wq, wk, _REAL_DT[q_weight.dtype]
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, *, eps=1e-6, interleaved=False, mscale=1.0, out_q=None, out_k=None):
     """Root-mean-square norm of every head of q and k times its weight [head_dim], then rotary positions as by rope(), in one pass
     (itexb_qk_norm_rope).  -> (q_out, k_out)."""
-    dev = on_device_of(q, k, positions, inv_freq, q_weight, k_weight, out_q, out_k)
+    dev = device_of(q, k, positions, inv_freq, q_weight, k_weight, out_q, out_k)
     args, oq, ok = _rope_params(q, positions, inv_freq, k, interleaved, mscale, False, out_q, out_k)
-    wq, wk, wdt = _norm_weights(q, k, q_weight, k_weight)
-    launch(L.load().itexb_qk_norm_rope, L.QkNormRopeParams(L.RopeParams(*args), wq, wk, wdt, eps), dev)
+    launch(L.load().itexb_qk_norm_rope, L.pack_qk_norm_rope(*args, *_norm_weights(q, q_weight, k_weight), eps), dev)
     return oq, ok
 
 
@@ -290,16 +296,15 @@ def qk_norm_rope_backward(grad_q, grad_k, q, k, q_weight, k_weight, positions, i
                           out_q=None, out_k=None):
     """Gradient of qk_norm_rope (itexb_qk_norm_rope_grad): q, k are the forward call's inputs, grad_q, grad_k its outputs' gradients.
     -> (dq, dk, dq_weight, dk_weight); equal calls give equal bits."""
-    dev = on_device_of(q, k, positions, inv_freq, q_weight, k_weight, grad_q, grad_k, out_q, out_k)
+    dev = device_of(q, k, positions, inv_freq, q_weight, k_weight, grad_q, grad_k, out_q, out_k)
     args, oq, ok = _rope_params(q, positions, inv_freq, k, interleaved, mscale, False, out_q, out_k)
-    wq, wk, wdt = _norm_weights(q, k, q_weight, k_weight)
-    dw = torch.empty((2, q.shape[-1]), dtype=q_weight.dtype, device=dev)
+    weights = _norm_weights(q, q_weight, k_weight)
+    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
     lib = L.load()
-    work = torch.empty(lib.itexb_qk_norm_rope_grad_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2]), dtype=torch.uint8, device=dev)
-    n = L.QkNormRopeParams(L.RopeParams(*args), wq, wk, wdt, eps)
-    launch(lib.itexb_qk_norm_rope_grad, L.QkNormRopeGradParams(n, *_rows(grad_q, "grad_q", q), *_rows(grad_k, "grad_k", k), dw[0].data_ptr(),
-                                                               dw[1].data_ptr(), work.data_ptr()), dev)
-    return oq, ok, dw[0], dw[1]
+    work = torch.empty(lib.itexb_qk_norm_rope_grad_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2]), dtype=torch.uint8, device=q.device)
+    launch(lib.itexb_qk_norm_rope_grad, L.pack_qk_norm_rope_grad(*args, *weights, eps, *_rows(grad_q, "grad_q", q), *_rows(grad_k, "grad_k", k),
+                                                                 dwq.data_ptr(), dwk.data_ptr(), work.data_ptr()), dev)
+    return oq, ok, dwq, dwk
 
 
 def launch_count() -> int:

@@ -69,20 +69,22 @@ class Kv4Cache:
     besides the tensors: which page belongs to which sequence is the caller's block table."""
 
     def __init__(self, k_codes, k_params, v_codes, v_params):
-        self.device = K.on_device_of(k_codes, k_params, v_codes, v_params)
-        if k_codes.dim() != 4 or k_params.dim() != 5 or k_codes.dtype != torch.uint8 or k_params.dtype != torch.float16:
-            raise ValueError("codes must be uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16 [.., head_dim / group, 2]")
+        self.dev = K.device_of(k_codes, k_params, v_codes, v_params)
         cs, ps, ct, pt = k_codes.shape, k_params.shape, k_codes.stride(), k_params.stride()
+        if len(cs) != 4 or len(ps) != 5 or k_codes.dtype != torch.uint8 or k_params.dtype != torch.float16:
+            raise ValueError("codes must be uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16 [.., head_dim / group, 2]")
         if v_codes.shape != cs or v_codes.stride() != ct or v_codes.dtype != torch.uint8 or v_params.shape != ps or v_params.stride() != pt \
                 or v_params.dtype != torch.float16:
             raise ValueError("keys and values must agree in shapes, strides and types")
-        if ps[:3] != cs[:3] or ps[4] != 2 or ps[3] < 1 or ct[3] != 1 or pt[4] != 1 or (ps[3] > 1 and pt[3] != 2) or any(s % 2 for s in pt[:3]) \
-                or cs[3] * 2 % ps[3] != 0:
+        pages, heads, page_size, row = cs
+        groups = ps[3]
+        if ps[:3] != cs[:3] or ps[4] != 2 or groups < 1 or ct[3] != 1 or pt[4] != 1 or (groups > 1 and pt[3] != 2) or (pt[0] | pt[1] | pt[2]) & 1 \
+                or 2 * row % groups != 0:
             raise ValueError("codes %s and params %s do not describe one cache with dense rows" % (tuple(cs), tuple(ps)))
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.group = cs[0], cs[1], cs[2], cs[3] * 2, cs[3] * 2 // ps[3]
-        self._c = L.Kv4CacheParams(cs[0], cs[2], cs[1], cs[3] * 2, self.group, 0, k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(),
-                                   v_params.data_ptr(), ct[0], ct[1], ct[2], pt[0] // 2, pt[1] // 2, pt[2] // 2)
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.group = pages, heads, page_size, 2 * row, 2 * row // groups
+        self._c = (pages, page_size, heads, 2 * row, self.group, 0, k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(),
+                   ct[0], ct[1], ct[2], pt[0] // 2, pt[1] // 2, pt[2] // 2)
 
     @classmethod
     def allocate(cls, num_pages, page_size, kv_heads, head_dim, group=64, device="cuda", token_major=False):
@@ -96,38 +98,38 @@ class Kv4Cache:
 
     def _kv(self, k, v, what):
         kp, vp = K._rows(k, "k"), K._rows(v, "v", k)
-        if k.shape[1] != self.kv_heads or k.shape[2] != self.head_dim:
+        n, heads, dim = k.shape
+        if heads != self.kv_heads or dim != self.head_dim:
             raise ValueError("%s: rows %s for a cache of %d heads of %d" % (what, tuple(k.shape), self.kv_heads, self.head_dim))
-        return kp, vp
+        return n, kp, vp
 
     def append(self, k, v, slots, *, positions=None, inv_freq=None, interleaved=False, mscale=1.0, status=None):
         """Writes k, v [tokens, kv_heads, head_dim] (strided views are fine) into rows slots[t] = page * page_size + offset; -1
         skips a token; the other slots of a call must differ.  With positions and inv_freq the keys are rotated on the way."""
-        K.on_device_of(self.k_codes, k, v, slots, positions, inv_freq, status)
+        K.device_of(self.k_codes, k, v, slots, positions, inv_freq, status)
         if (positions is None) != (inv_freq is None):
             raise ValueError("positions and inv_freq go together")
-        kp, vp = self._kv(k, v, "append")
-        n = k.shape[0]
+        n, kp, vp = self._kv(k, v, "append")
         sp = K._vector(slots, "slots", K._INDEX_DT, n)
         pos = freq = pdt = rot = 0
         if positions is not None:
             pos, pdt = K._vector(positions, "positions", K._INDEX_DT, n), K._INDEX_DT[positions.dtype]
-            freq, rot = K._vector(inv_freq, "inv_freq", (torch.float64,)), 2 * inv_freq.shape[0]
-        K.launch(L.load().itexb_kv4_append, L.Kv4AppendParams(self._c, n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
-                                                              int(interleaved), mscale, _status(status)), self.device)
+            freq, rot = K._vector(inv_freq, "inv_freq", K._FLOAT64), 2 * inv_freq.shape[0]
+        K.launch(L.load().itexb_kv4_append, L.pack_kv4_append(*self._c, n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
+                                                              int(interleaved), mscale, _status(status)), self.dev)
 
     def gather(self, slots, dtype=torch.bfloat16, *, out_k=None, out_v=None, status=None):
         """-> (k, v) [len(slots), kv_heads, head_dim]: the values that rows `slots` stand for, zeros for slot -1."""
-        K.on_device_of(self.k_codes, slots, out_k, out_v, status)
+        K.device_of(self.k_codes, slots, out_k, out_v, status)
         sp = K._vector(slots, "slots", K._INDEX_DT)
-        shape = (slots.shape[0], self.kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self.device) if out_k is None else out_k
-        v = torch.empty(shape, dtype=dtype, device=self.device) if out_v is None else out_v
-        kp, vp = self._kv(k, v, "gather")
-        if k.shape[0] != shape[0]:
-            raise ValueError("gather: %d rows for %d slots" % (k.shape[0], shape[0]))
-        K.launch(L.load().itexb_kv4_gather, L.Kv4GatherParams(self._c, shape[0], K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status)),
-                 self.device)
+        tokens = slots.shape[0]
+        k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=slots.device) if out_k is None else out_k
+        v = torch.empty_like(k) if out_v is None else out_v
+        n, kp, vp = self._kv(k, v, "gather")
+        if n != tokens:
+            raise ValueError("gather: %d rows for %d slots" % (n, tokens))
+        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._c, n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status)),
+                 self.dev)
         return k, v
 
     def attention(self, q, block_table, kept, *, q_starts=None, max_new=None, max_kept=None, causal=True, window=0, scale=None, out=None,
@@ -137,39 +139,46 @@ class Kv4Cache:
         q_starts int32 [sequences + 1] gives each sequence's rows of q; without it every sequence has max_new rows.  max_new and
         max_kept are upper bounds of a sequence's new and kept tokens (by default as many as q and the table can hold); a tight
         bound saves work.  -> out, whose rows behind the last sequence stay as they were (uninitialised without `out`).
-        workspace: a uint8 tensor of workspace_bytes(...) to use instead of a fresh one."""
-        K.on_device_of(self.k_codes, q, block_table, kept, q_starts, out, status, workspace)
+        workspace: a dense uint8 tensor to use instead of a fresh one, at least as large as a refusal asks for; calls that may
+        run at the same time need different ones."""
+        K.device_of(self.k_codes, q, block_table, kept, q_starts, out, status, workspace)
         qp = K._rows(q, "q")
+        kp = K._vector(kept, "kept", _INT32)
         seqs = kept.shape[0]
-        kp = K._vector(kept, "kept", (torch.int32,))
-        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != seqs or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-            raise ValueError("block_table must be int32 [sequences, pages] with dense rows, got %s %s" % (block_table.dtype, tuple(block_table.shape)))
         rows, heads, dim = q.shape
         if dim != self.head_dim or heads % self.kv_heads != 0:
             raise ValueError("q %s for a cache of %d heads of %d" % (tuple(q.shape), self.kv_heads, self.head_dim))
+        ts, tst = block_table.shape, block_table.stride()
+        if len(ts) != 2 or block_table.dtype != torch.int32 or ts[0] != seqs or (tst[1] != 1 and ts[1] > 1):
+            raise ValueError("block_table must be int32 [sequences, pages] with dense rows, got %s %s" % (block_table.dtype, tuple(ts)))
+        cols = ts[1]
         sp = 0
         if q_starts is not None:
-            sp = K._vector(q_starts, "q_starts", (torch.int32,), seqs + 1)
+            sp = K._vector(q_starts, "q_starts", _INT32, seqs + 1)
             max_new = rows if max_new is None else max_new
-        elif max_new is None:
-            max_new = rows // max(1, seqs)
-        if q_starts is None and max_new * seqs > rows:
-            raise ValueError("%d sequences of %d new tokens, but q has %d rows" % (seqs, max_new, rows))
-        cols = block_table.shape[1]
+        else:
+            max_new = rows // max(1, seqs) if max_new is None else max_new
+            if max_new * seqs > rows:
+                raise ValueError("%d sequences of %d new tokens, but q has %d rows" % (seqs, max_new, rows))
         max_kept = min(cols * self.page_size, (1 << 31) - 1) if max_kept is None else max_kept
-        o = torch.empty(q.shape, dtype=q.dtype, device=self.device) if out is None else out
-        p = L.Kv4AttentionParams(self._c, K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
-                                 rows, *qp, *K._rows(o, "out", q), block_table.data_ptr(), block_table.stride(0), cols, kp, sp, _status(status), 0, 0)
+        if out is None:
+            out = torch.empty_like(q)
+            op = K._rows(out, "out")
+        else:
+            op = K._rows(out, "out", q)
+        args = (*self._c, K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
+                rows, *qp, *op, block_table.data_ptr(), tst[0], cols, kp, sp, _status(status))
         lib = L.load()
-        need = lib.itexb_kv4_attention_workspace_bytes(p)
-        if need:
-            if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-            elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-                raise ValueError("workspace must be a dense uint8 tensor")
-            p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        K.launch(lib.itexb_kv4_attention, p, self.device)
-        return o
+        if workspace is None:
+            need = lib.itexb_kv4_attention_workspace_bytes(L.pack_kv4_attention(*args, 0, 0))
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise ValueError("workspace must be a dense uint8 tensor")
+        K.launch(lib.itexb_kv4_attention, L.pack_kv4_attention(*args, workspace.data_ptr(), workspace.numel()), self.dev)
+        return out
+
+
+_INT32 = {torch.int32: 0}
 
 
 def _status(t):
