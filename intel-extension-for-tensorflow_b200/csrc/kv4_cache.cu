@@ -4,8 +4,7 @@
 //
 // Both are bound by HBM (append, head_dim 128, groups of 64, bf16: 256 B in, 72 B out per row).  A thread owns 8
 // consecutive elements, which are one 32-bit word of codes; the 4 - 16 threads of a group exchange minimum and maximum
-// by shuffles.  For the rotation of halves a thread loads its partner's 8 elements too (from L1) instead of exchanging
-// them.  Every step is a separately rounded fp32 operation on cosines and sines rounded from 64 bits, so the codes are
+// by shuffles, and the rotation of halves its partners.  Every step is a separately rounded fp32 operation on cosines and sines rounded from 64 bits, so the codes are
 // those of the same formulas written with plain fp32 tensor operations.
 #include <algorithm>
 #include <climits>
@@ -34,9 +33,8 @@ struct RowArgs {
 __device__ __forceinline__ float MinNan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float MaxNan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// The row of a token's slot; false where there is none (-1) or it lies outside the cache (reported).
-__device__ __forceinline__ bool SlotRow(const RowArgs& a, uint32_t token, bool report, uint32_t* page, uint32_t* off) {
-  const int64_t slot = LoadIndex(a.slots, a.slots64, token);
+// The row of a slot; false where there is none (-1) or it lies outside the cache (reported).
+__device__ __forceinline__ bool RowOf(const RowArgs& a, int64_t slot, bool report, uint32_t* page, uint32_t* off) {
   if (slot < 0 || slot >= int64_t(a.c.num_pages) * a.c.page_size) {
     if (slot != -1 && report) ReportIndex(a.status_word);
     return false;
@@ -44,22 +42,6 @@ __device__ __forceinline__ bool SlotRow(const RowArgs& a, uint32_t token, bool r
   *page = QuickDiv(uint32_t(slot), a.c.div_page);
   *off = uint32_t(slot) - *page * uint32_t(a.c.page_size);
   return true;
-}
-
-// Eight elements of a row from element e on; one by one where the row is not aligned.
-template <typename T> __device__ __forceinline__ void Load8(const T* row, int e, bool vec, float (&f)[8]) {
-  if (!vec) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = ToFloat(row[e + i]);
-  } else if constexpr (sizeof(T) == 2) {
-    LoadVec<T, 8>(row + e, f);
-  } else {
-    float lo[4], hi[4];
-    LoadVec<T, 4>(row + e, lo);
-    LoadVec<T, 4>(row + e + 4, hi);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
-  }
 }
 
 // Codes and (lo, step) of the group this thread's eight elements belong to; `lanes` threads share the group.
@@ -87,13 +69,40 @@ __device__ __forceinline__ uint32_t Quantize8(const float (&x)[8], int lanes, __
   return w;
 }
 
-template <typename T, int DIM>
+// A block's rows are taken in P passes whose loads are all issued before the table is formed, as in rope.cu.
+template <typename T, int DIM, int P>
 __global__ void __launch_bounds__(kThreads) Kv4AppendKernel(const __grid_constant__ RowArgs a) {
   extern __shared__ float2 s_table[];
-  constexpr int kTpr = DIM / 8, kRows = kThreads / kTpr;
+  constexpr int kTpr = DIM / 8, kGroups = kThreads / kTpr, kRows = kGroups * P;
   const uint32_t row0 = blockIdx.x * uint32_t(kRows);
   const uint32_t row1 = min(a.rows, row0 + uint32_t(kRows));
   const uint32_t first = QuickDiv(row0, a.div_heads);
+  const int in_row = threadIdx.x % kTpr, e = in_row * 8;
+  union Raw { T v[8]; uint4 w[sizeof(T) / 2]; };   // eight elements as loaded
+  Raw rk[P], rv[P];
+  int64_t slot[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const uint32_t row = row0 + p * kGroups + threadIdx.x / kTpr;
+    slot[p] = -1;
+    if (row < row1) {
+      const uint32_t token = QuickDiv(row, a.div_heads);
+      const int64_t head = row - token * uint32_t(a.c.kv_heads);
+      slot[p] = LoadIndex(a.slots, a.slots64, token);
+      const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + head * a.kh + e;
+      const T* vr = static_cast<const T*>(a.v) + int64_t(token) * a.vt + head * a.vh + e;
+      if (a.vec) {
+#pragma unroll
+        for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+          rk[p].w[i] = reinterpret_cast<const uint4*>(kr)[i];
+          rv[p].w[i] = reinterpret_cast<const uint4*>(vr)[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { rk[p].v[i] = kr[i]; rv[p].v[i] = vr[i]; }
+      }
+    }
+  }
   if (a.positions != nullptr) {
     const int n = int(QuickDiv(row1 - 1, a.div_heads) - first + 1) * a.pairs;
     for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -104,40 +113,46 @@ __global__ void __launch_bounds__(kThreads) Kv4AppendKernel(const __grid_constan
     }
     __syncthreads();
   }
-  const int in_row = threadIdx.x % kTpr, e = in_row * 8;
-  const uint32_t row = row0 + threadIdx.x / kTpr;
-  const bool on = row < row1;
-  const uint32_t token = QuickDiv(on ? row : row0, a.div_heads);
-  const int head = int((on ? row : row0) - token * uint32_t(a.c.kv_heads));
-  uint32_t page = 0, off = 0;
-  const bool keep = on && SlotRow(a, token, in_row == 0 && head == 0, &page, &off);
-  float k[8], v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
-  if (keep) {
-    const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + int64_t(head) * a.kh;
-    Load8<T>(static_cast<const T*>(a.v) + int64_t(token) * a.vt + int64_t(head) * a.vh, e, a.vec, v);
-    Load8<T>(kr, e, a.vec, k);
-    if (a.positions != nullptr && e < 2 * a.pairs) {
+  for (int p = 0; p < P; ++p) {
+    const uint32_t row = row0 + p * kGroups + threadIdx.x / kTpr;
+    if (P > 1 && row0 + p * kGroups >= row1) break;
+    const bool on = row < row1;
+    const uint32_t token = QuickDiv(on ? row : row0, a.div_heads);
+    const int head = int((on ? row : row0) - token * uint32_t(a.c.kv_heads));
+    uint32_t page = 0, off = 0;
+    const bool keep = on && RowOf(a, slot[p], in_row == 0 && head == 0, &page, &off);
+    float k[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { k[i] = on ? ToFloat(rk[p].v[i]) : 0.f; v[i] = on ? ToFloat(rv[p].v[i]) : 0.f; }
+    if (a.positions != nullptr) {
       const float2* cs = s_table + (token - first) * a.pairs;
       if (a.interleaved) {
+        if (e < 2 * a.pairs) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (e / 2 + i < a.pairs) {
-            const float2 p = cs[e / 2 + i];
-            const float x = k[2 * i], y = k[2 * i + 1];
-            k[2 * i] = x * p.x - y * p.y;
-            k[2 * i + 1] = y * p.x + x * p.y;
+          for (int i = 0; i < 4; ++i) {
+            if (e / 2 + i < a.pairs) {
+              const float2 q = cs[e / 2 + i];
+              const float x = k[2 * i], y = k[2 * i + 1];
+              k[2 * i] = x * q.x - y * q.y;
+              k[2 * i + 1] = y * q.x + x * q.y;
+            }
           }
         }
-      } else if (a.pairs % 8 == 0) {  // the eight partners are the eight of another thread
-        const bool upper = e >= a.pairs;
+      } else if (a.pairs % 8 == 0) {  // the eight partners are the eight of another thread of the row
+        const int far = a.pairs / 8;
+        const bool turned = in_row < 2 * far, upper = in_row >= far;
+        const int from = int(threadIdx.x % 32) + (turned ? (upper ? -far : far) : 0);
         float o[8];
-        Load8<T>(kr, upper ? e - a.pairs : e + a.pairs, a.vec, o);
-        const float2* p = cs + (upper ? e - a.pairs : e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = upper ? k[i] * p[i].x + o[i] * p[i].y : k[i] * p[i].x - o[i] * p[i].y;
-      } else {
+        for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, k[i], from);
+        if (turned) {
+          const float2* q = cs + (upper ? e - a.pairs : e);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) k[i] = upper ? k[i] * q[i].x + o[i] * q[i].y : k[i] * q[i].x - o[i] * q[i].y;
+        }
+      } else if (on) {
+        const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + int64_t(head) * a.kh;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (e + i < 2 * a.pairs) {
@@ -149,18 +164,18 @@ __global__ void __launch_bounds__(kThreads) Kv4AppendKernel(const __grid_constan
         }
       }
     }
-  }
-  const int lanes = a.c.group / 8;
-  __half2 kp, vp;
-  const uint32_t kw = Quantize8(k, lanes, &kp), vw = Quantize8(v, lanes, &vp);
-  if (keep) {
-    const int64_t ci = int64_t(page) * a.c.cp + int64_t(head) * a.c.ch + int64_t(off) * a.c.ct + in_row * 4;
-    *reinterpret_cast<uint32_t*>(a.c.k_codes + ci) = kw;
-    *reinterpret_cast<uint32_t*>(a.c.v_codes + ci) = vw;
-    if (in_row % lanes == 0) {
-      const int64_t pi = int64_t(page) * a.c.pp + int64_t(head) * a.c.ph + int64_t(off) * a.c.pt + in_row / lanes;
-      a.c.k_params[pi] = kp;
-      a.c.v_params[pi] = vp;
+    const int lanes = a.c.group / 8;
+    __half2 kp, vp;
+    const uint32_t kw = Quantize8(k, lanes, &kp), vw = Quantize8(v, lanes, &vp);
+    if (keep) {
+      const int64_t ci = int64_t(page) * a.c.cp + int64_t(head) * a.c.ch + int64_t(off) * a.c.ct + in_row * 4;
+      *reinterpret_cast<uint32_t*>(a.c.k_codes + ci) = kw;
+      *reinterpret_cast<uint32_t*>(a.c.v_codes + ci) = vw;
+      if (in_row % lanes == 0) {
+        const int64_t pi = int64_t(page) * a.c.pp + int64_t(head) * a.c.ph + int64_t(off) * a.c.pt + in_row / lanes;
+        a.c.k_params[pi] = kp;
+        a.c.v_params[pi] = vp;
+      }
     }
   }
 }
@@ -178,32 +193,48 @@ template <typename T> __device__ __forceinline__ void Store8(T* row, int e, bool
   }
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int P>
 __global__ void __launch_bounds__(kThreads) Kv4GatherKernel(const __grid_constant__ RowArgs a) {
-  constexpr int kTpr = DIM / 8, kRows = kThreads / kTpr;
-  const uint32_t row = blockIdx.x * uint32_t(kRows) + threadIdx.x / kTpr;
-  if (row >= a.rows) return;
+  constexpr int kTpr = DIM / 8, kGroups = kThreads / kTpr, kRows = kGroups * P;
   const int in_row = threadIdx.x % kTpr, e = in_row * 8;
-  const uint32_t token = QuickDiv(row, a.div_heads);
-  const int head = int(row - token * uint32_t(a.c.kv_heads));
-  uint32_t page = 0, off = 0;
-  float k[8], v[8];
-  if (SlotRow(a, token, in_row == 0 && head == 0, &page, &off)) {
-    const int64_t ci = int64_t(page) * a.c.cp + int64_t(head) * a.c.ch + int64_t(off) * a.c.ct + in_row * 4;
-    const int64_t pi = int64_t(page) * a.c.pp + int64_t(head) * a.c.ph + int64_t(off) * a.c.pt + e / a.c.group;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(a.c.k_codes + ci), vw = *reinterpret_cast<const uint32_t*>(a.c.v_codes + ci);
-    const float2 kp = __half22float2(a.c.k_params[pi]), vp = __half22float2(a.c.v_params[pi]);
+  const uint32_t row0 = blockIdx.x * uint32_t(kRows) + threadIdx.x / kTpr;
+  uint32_t kw[P], vw[P];
+  __half2 kp[P], vp[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const uint32_t row = row0 + p * kGroups;
+    kw[p] = vw[p] = 0u;
+    kp[p] = vp[p] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+    if (row < a.rows) {
+      const uint32_t token = QuickDiv(row, a.div_heads);
+      const int64_t head = row - token * uint32_t(a.c.kv_heads);
+      uint32_t page = 0, off = 0;
+      if (RowOf(a, LoadIndex(a.slots, a.slots64, token), in_row == 0 && head == 0, &page, &off)) {
+        const int64_t ci = int64_t(page) * a.c.cp + head * a.c.ch + int64_t(off) * a.c.ct + in_row * 4;
+        const int64_t pi = int64_t(page) * a.c.pp + head * a.c.ph + int64_t(off) * a.c.pt + e / a.c.group;
+        kw[p] = *reinterpret_cast<const uint32_t*>(a.c.k_codes + ci);
+        vw[p] = *reinterpret_cast<const uint32_t*>(a.c.v_codes + ci);
+        kp[p] = a.c.k_params[pi];
+        vp[p] = a.c.v_params[pi];
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const uint32_t row = row0 + p * kGroups;
+    if (row >= a.rows) break;
+    const uint32_t token = QuickDiv(row, a.div_heads);
+    const int64_t head = row - token * uint32_t(a.c.kv_heads);
+    const float2 fk = __half22float2(kp[p]), fv = __half22float2(vp[p]);
+    float k[8], v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      k[i] = float((kw >> (4 * i)) & 15u) * kp.y + kp.x;
-      v[i] = float((vw >> (4 * i)) & 15u) * vp.y + vp.x;
+      k[i] = float((kw[p] >> (4 * i)) & 15u) * fk.y + fk.x;
+      v[i] = float((vw[p] >> (4 * i)) & 15u) * fv.y + fv.x;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+    Store8<T>(static_cast<T*>(a.k) + int64_t(token) * a.kt + head * a.kh, e, a.vec, k);
+    Store8<T>(static_cast<T*>(a.v) + int64_t(token) * a.vt + head * a.vh, e, a.vec, v);
   }
-  Store8<T>(static_cast<T*>(a.k) + int64_t(token) * a.kt + int64_t(head) * a.kh, e, a.vec, k);
-  Store8<T>(static_cast<T*>(a.v) + int64_t(token) * a.vt + int64_t(head) * a.vh, e, a.vec, v);
 }
 
 int CheckRows(const char* what, int64_t tokens, int dtype, int slots_dtype, const Kv4View& c) {
@@ -218,26 +249,33 @@ bool RowsAligned(const void* p, int64_t t, int64_t h, int esz) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (t * esz) % 16 == 0 && (h * esz) % 16 == 0;
 }
 
-template <typename T, bool APPEND> int LaunchDim(const RowArgs& a, cudaStream_t st) {
-  const int rows = kThreads / (a.c.head_dim / 8);
-  const unsigned blocks = (a.rows + rows - 1) / rows;
-  size_t smem = 0;
-  if (APPEND && a.positions != nullptr) smem = size_t(std::min(rows, rows / a.c.kv_heads + 2)) * a.pairs * sizeof(float2);
-#define ITEXB_KV4_DIM(D)                                                                     \
-  do {                                                                                       \
-    if (APPEND) Kv4AppendKernel<T, D><<<blocks, kThreads, smem, st>>>(a);                    \
-    else Kv4GatherKernel<T, D><<<blocks, kThreads, 0, st>>>(a);                              \
-  } while (0)
-  if (a.c.head_dim == 64) ITEXB_KV4_DIM(64);
-  else if (a.c.head_dim == 128) ITEXB_KV4_DIM(128);
-  else ITEXB_KV4_DIM(256);
-#undef ITEXB_KV4_DIM
-  return CheckLaunch(APPEND ? "Kv4AppendKernel" : "Kv4GatherKernel");
+template <typename T, int DIM, int P, bool APPEND> int LaunchPasses(const RowArgs& a, cudaStream_t st) {
+  constexpr int kRows = kThreads / (DIM / 8) * P;
+  const unsigned blocks = (a.rows + kRows - 1) / kRows;
+  if (APPEND) {
+    size_t smem = 0;
+    if (a.positions != nullptr) smem = size_t(std::min(kRows, kRows / a.c.kv_heads + 2)) * a.pairs * sizeof(float2);
+    Kv4AppendKernel<T, DIM, P><<<blocks, kThreads, smem, st>>>(a);
+    return CheckLaunch("Kv4AppendKernel");
+  }
+  Kv4GatherKernel<T, DIM, P><<<blocks, kThreads, 0, st>>>(a);
+  return CheckLaunch("Kv4GatherKernel");
+}
+template <typename T, int DIM, bool APPEND> int LaunchDim(const RowArgs& a, cudaStream_t st) {
+  // four passes where that still gives every SM four blocks
+  constexpr int kPasses = APPEND ? 1 : 4;
+  if (kPasses > 1 && a.rows >= uint32_t(kThreads / (DIM / 8)) * kPasses * 148 * 4) return LaunchPasses<T, DIM, kPasses, APPEND>(a, st);
+  return LaunchPasses<T, DIM, 1, APPEND>(a, st);
+}
+template <typename T, bool APPEND> int LaunchType(const RowArgs& a, cudaStream_t st) {
+  if (a.c.head_dim == 64) return LaunchDim<T, 64, APPEND>(a, st);
+  if (a.c.head_dim == 128) return LaunchDim<T, 128, APPEND>(a, st);
+  return LaunchDim<T, 256, APPEND>(a, st);
 }
 template <bool APPEND> int Launch(const RowArgs& a, int dtype, cudaStream_t st) {
-  if (dtype == ITEXB_DT_FLOAT) return LaunchDim<float, APPEND>(a, st);
-  if (dtype == ITEXB_DT_BFLOAT16) return LaunchDim<__nv_bfloat16, APPEND>(a, st);
-  return LaunchDim<__half, APPEND>(a, st);
+  if (dtype == ITEXB_DT_FLOAT) return LaunchType<float, APPEND>(a, st);
+  if (dtype == ITEXB_DT_BFLOAT16) return LaunchType<__nv_bfloat16, APPEND>(a, st);
+  return LaunchType<__half, APPEND>(a, st);
 }
 
 }  // namespace

@@ -17,7 +17,7 @@ namespace itexb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxGradBlocks = 592;  // partial weight gradients: four blocks per SM of a 148-SM device
+constexpr int kMaxGradBlocks = 296;  // per side; partial weight gradients: four blocks per SM of a 148-SM device for both
 enum { kRope = 0, kNorm = 1, kGrad = 2 };
 
 struct Side {  // queries or keys
@@ -87,154 +87,215 @@ template <int VEC> __device__ __forceinline__ Item ItemOf(int j, const RopeArgs&
   return {2 * VEC * j, 2 * VEC * j + VEC, j < nt};   // interleaved pairs, or the elements behind the rotated ones
 }
 
-template <typename T, int VEC, int NI, int MODE>
+// The weights as fp32 in shared memory: [queries, keys][head_dim].
+__device__ __forceinline__ void FillWeights(float* w, const RopeArgs& a) {
+  for (int i = threadIdx.x; i < 2 * a.head_dim; i += kThreads) {
+    const int side = i >= a.head_dim;
+    if (a.side[side].w != nullptr) w[i] = LoadW(a.side[side].w, a.w_dtype, i - side * a.head_dim);
+  }
+}
+template <int VEC> __device__ __forceinline__ void TimesWeights(float (&u)[VEC], float (&v)[VEC], const float* w, const Item& it) {
+  float p[VEC], q[VEC];
+  LoadVec<float, VEC>(w + it.o0, p);
+  LoadVec<float, VEC>(w + it.o1, q);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) { u[i] *= p[i]; v[i] *= q[i]; }
+}
+
+// A thread's pieces of one row, as loaded.
+template <typename T, int VEC, int NI> struct Pieces {
+  Vec<T, VEC> u[NI], v[NI];
+  __device__ __forceinline__ void Load(const T* x, int in_row, bool on, const RopeArgs& a) {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int j = in_row + n * a.tpr;
+      if (on && j < a.items) {
+        const Item it = ItemOf<VEC>(j, a);
+        u[n] = *reinterpret_cast<const Vec<T, VEC>*>(x + it.o0);
+        v[n] = *reinterpret_cast<const Vec<T, VEC>*>(x + it.o1);
+      }
+    }
+  }
+  __device__ __forceinline__ void Floats(int n, float (&fu)[VEC], float (&fv)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { fu[i] = ToFloat(u[n].v[i]); fv[i] = ToFloat(v[n].v[i]); }
+  }
+};
+
+// A block's rows are taken in P passes whose loads are all issued before the table is formed: long calls keep 4 x 32 bytes
+// per thread in flight (norms and rotation of 8192 tokens, 168 MB: 55 us with one pass per block).  Short ones take one pass
+// per block and so reach more SMs.
+template <typename T, int VEC, int NI, int MODE, int P>
 __global__ void __launch_bounds__(kThreads) RopeKernel(const __grid_constant__ RopeArgs a) {
-  extern __shared__ float2 s_table[];
+  extern __shared__ float4 s_mem[];
+  float* s_w = reinterpret_cast<float*>(s_mem);                              // kNorm
+  float2* s_table = reinterpret_cast<float2*>(s_w + (MODE == kNorm ? 2 * a.head_dim : 0));
   const int group = threadIdx.x / a.tpr, in_row = threadIdx.x - group * a.tpr;
   const int groups = kThreads / a.tpr;
   const uint32_t row0 = blockIdx.x * uint32_t(a.rows_per_block);
   const uint32_t row1 = min(a.rows, row0 + uint32_t(a.rows_per_block));
   const uint32_t first = QuickDiv(row0, a.div_heads);
   const uint32_t heads = uint32_t(a.heads[0] + a.heads[1]);
+  Pieces<T, VEC, NI> x[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const uint32_t row = row0 + p * groups + group;
+    if (row < row1) {
+      const uint32_t token = QuickDiv(row, a.div_heads);
+      const int head = int(row - token * heads);
+      const int is_k = head >= a.heads[0];
+      const Side& s = a.side[is_k];
+      x[p].Load(static_cast<const T*>(s.x) + int64_t(token) * s.xt + int64_t(head - (is_k ? a.heads[0] : 0)) * s.xh, in_row, true, a);
+    }
+  }
   FillTable(s_table, a, first, QuickDiv(row1 - 1, a.div_heads) - first + 1);
+  if (MODE == kNorm) FillWeights(s_w, a);
   __syncthreads();
-  for (uint32_t base = row0; base < row1; base += groups) {
-    const uint32_t row = base + group;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const uint32_t row = row0 + p * groups + group;
     const bool on = row < row1;
+    if (P > 1 && row0 + p * groups >= row1) break;
     const uint32_t token = QuickDiv(on ? row : row0, a.div_heads);
     const int head = int((on ? row : row0) - token * heads);
-    const bool is_k = head >= a.heads[0];
+    const int is_k = head >= a.heads[0];
     const Side& s = a.side[is_k];
-    const int64_t h = is_k ? head - a.heads[0] : head;
-    const T* x = static_cast<const T*>(s.x) + token * s.xt + h * s.xh;
-    T* y = static_cast<T*>(s.y) + token * s.yt + h * s.yh;
-    float u[NI][VEC], v[NI][VEC];
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      const int j = in_row + n * a.tpr;
-      if (on && j < a.items) {
-        const Item it = ItemOf<VEC>(j, a);
-        LoadVec<T, VEC>(x + it.o0, u[n]);
-        LoadVec<T, VEC>(x + it.o1, v[n]);
-        if (MODE == kNorm) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) sum = fmaf(u[n][i], u[n][i], fmaf(v[n][i], v[n][i], sum));
-        }
-      }
-    }
     float r = 1.f;
     if (MODE == kNorm) {
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        if (on && in_row + n * a.tpr < a.items) {
+          float u[VEC], v[VEC];
+          x[p].Floats(n, u, v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum = fmaf(u[i], u[i], fmaf(v[i], v[i], sum));
+        }
+      }
       for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       r = rsqrtf(sum / float(a.head_dim) + a.eps);
     }
+    T* y = static_cast<T*>(s.y) + int64_t(token) * s.yt + int64_t(head - (is_k ? a.heads[0] : 0)) * s.yh;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
       const int j = in_row + n * a.tpr;
       if (on && j < a.items) {
         const Item it = ItemOf<VEC>(j, a);
+        float u[VEC], v[VEC];
+        x[p].Floats(n, u, v);
         if (MODE == kNorm) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            u[n][i] = u[n][i] * r * LoadW(s.w, a.w_dtype, it.o0 + i);
-            v[n][i] = v[n][i] * r * LoadW(s.w, a.w_dtype, it.o1 + i);
-          }
+          for (int i = 0; i < VEC; ++i) { u[i] *= r; v[i] *= r; }
+          TimesWeights<VEC>(u, v, s_w + is_k * a.head_dim, it);
         }
-        if (it.turned) Turn<VEC>(u[n], v[n], s_table + (token - first) * a.pairs + j * VEC, a.interleaved);
-        StoreVec<T, VEC>(y + it.o0, u[n]);
-        StoreVec<T, VEC>(y + it.o1, v[n]);
+        if (it.turned) Turn<VEC>(u, v, s_table + (token - first) * a.pairs + j * VEC, a.interleaved);
+        StoreVec<T, VEC>(y + it.o0, u);
+        StoreVec<T, VEC>(y + it.o1, v);
       }
     }
   }
 }
 
 // blockIdx.y chooses queries or keys; blocks walk the row tiles with a fixed stride, so the partial sums of the weight
-// gradient, and with them its bits, depend on the shape alone.
+// gradient, and with them its bits, depend on the shape alone.  The next tile's loads are issued before this one's work.
 template <typename T, int VEC, int NI>
 __global__ void __launch_bounds__(kThreads) NormRopeGradKernel(const __grid_constant__ RopeArgs a) {
-  extern __shared__ float2 s_table[];
+  extern __shared__ float4 s_mem[];
+  float* s_w = reinterpret_cast<float*>(s_mem);
+  float2* s_table = reinterpret_cast<float2*>(s_w + 2 * a.head_dim);
   const int which = blockIdx.y;
   const Side& s = a.side[which];
   const uint32_t heads = uint32_t(a.heads[which]);
   const uint32_t rows = uint32_t(a.tokens) * heads;
   const int group = threadIdx.x / a.tpr, in_row = threadIdx.x - group * a.tpr;
   const int groups = kThreads / a.tpr;
+  const uint32_t stride = gridDim.x * uint32_t(groups);
   float du[NI][VEC], dv[NI][VEC];
 #pragma unroll
   for (int n = 0; n < NI; ++n)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) du[n][i] = dv[n][i] = 0.f;
-  for (uint32_t row0 = blockIdx.x * uint32_t(a.rows_per_block); row0 < rows; row0 += gridDim.x * uint32_t(a.rows_per_block)) {
-    const uint32_t row1 = min(rows, row0 + uint32_t(a.rows_per_block));
+  FillWeights(s_w, a);
+  Pieces<T, VEC, NI> x, g;
+  auto load = [&](uint32_t row) {
+    if (row < rows) {
+      const uint32_t token = QuickDiv(row, a.div_side[which]);
+      const int64_t h = row - token * heads;
+      x.Load(static_cast<const T*>(s.x) + int64_t(token) * s.xt + h * s.xh, in_row, true, a);
+      g.Load(static_cast<const T*>(s.g) + int64_t(token) * s.gt + h * s.gh, in_row, true, a);
+    }
+  };
+  load(blockIdx.x * uint32_t(groups) + group);
+  for (uint32_t row0 = blockIdx.x * uint32_t(groups); row0 < rows; row0 += stride) {
+    const uint32_t row1 = min(rows, row0 + uint32_t(groups));
     const uint32_t first = QuickDiv(row0, a.div_side[which]);
     __syncthreads();
     FillTable(s_table, a, first, QuickDiv(row1 - 1, a.div_side[which]) - first + 1);
     __syncthreads();
-    for (uint32_t base = row0; base < row1; base += groups) {
-      const uint32_t row = base + group;
-      const bool on = row < row1;
-      const uint32_t token = QuickDiv(on ? row : row0, a.div_side[which]);
-      const int64_t h = (on ? row : row0) - token * heads;
-      const T* x = static_cast<const T*>(s.x) + token * s.xt + h * s.xh;
-      const T* g = static_cast<const T*>(s.g) + token * s.gt + h * s.gh;
-      T* y = static_cast<T*>(s.y) + token * s.yt + h * s.yh;
-      float xu[NI][VEC], xv[NI][VEC], gu[NI][VEC], gv[NI][VEC];
-      float sum = 0.f;
+    const uint32_t row = row0 + group;
+    const bool on = row < row1;
+    const uint32_t token = QuickDiv(on ? row : row0, a.div_side[which]);
+    const int64_t h = (on ? row : row0) - token * heads;
+    T* y = static_cast<T*>(s.y) + int64_t(token) * s.yt + h * s.yh;
+    const Pieces<T, VEC, NI> cx = x, cg = g;
+    load(row + stride);
+    float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int j = in_row + n * a.tpr;
-        if (on && j < a.items) {
-          const Item it = ItemOf<VEC>(j, a);
-          LoadVec<T, VEC>(x + it.o0, xu[n]);
-          LoadVec<T, VEC>(x + it.o1, xv[n]);
-          LoadVec<T, VEC>(g + it.o0, gu[n]);
-          LoadVec<T, VEC>(g + it.o1, gv[n]);
+    for (int n = 0; n < NI; ++n) {
+      if (on && in_row + n * a.tpr < a.items) {
+        float u[VEC], v[VEC];
+        cx.Floats(n, u, v);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) sum = fmaf(xu[n][i], xu[n][i], fmaf(xv[n][i], xv[n][i], sum));
-        }
+        for (int i = 0; i < VEC; ++i) sum = fmaf(u[i], u[i], fmaf(v[i], v[i], sum));
       }
-      for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = rsqrtf(sum / float(a.head_dim) + a.eps);
-      float dot = 0.f;
+    }
+    for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float r = rsqrtf(sum / float(a.head_dim) + a.eps);
+    float gu[NI][VEC], gv[NI][VEC];
+    float dot = 0.f;
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int j = in_row + n * a.tpr;
-        if (on && j < a.items) {
-          const Item it = ItemOf<VEC>(j, a);
-          if (it.turned) Turn<VEC>(gu[n], gv[n], s_table + (token - first) * a.pairs + j * VEC, a.interleaved);
+    for (int n = 0; n < NI; ++n) {
+      const int j = in_row + n * a.tpr;
+      if (on && j < a.items) {
+        const Item it = ItemOf<VEC>(j, a);
+        float u[VEC], v[VEC];
+        cx.Floats(n, u, v);
+        cg.Floats(n, gu[n], gv[n]);
+        if (it.turned) Turn<VEC>(gu[n], gv[n], s_table + (token - first) * a.pairs + j * VEC, a.interleaved);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            xu[n][i] *= r;
-            xv[n][i] *= r;
-            du[n][i] = fmaf(gu[n][i], xu[n][i], du[n][i]);
-            dv[n][i] = fmaf(gv[n][i], xv[n][i], dv[n][i]);
-            gu[n][i] *= LoadW(s.w, a.w_dtype, it.o0 + i);
-            gv[n][i] *= LoadW(s.w, a.w_dtype, it.o1 + i);
-            dot = fmaf(gu[n][i], xu[n][i], fmaf(gv[n][i], xv[n][i], dot));
-          }
+        for (int i = 0; i < VEC; ++i) {
+          u[i] *= r;
+          v[i] *= r;
+          du[n][i] = fmaf(gu[n][i], u[i], du[n][i]);
+          dv[n][i] = fmaf(gv[n][i], v[i], dv[n][i]);
         }
+        TimesWeights<VEC>(gu[n], gv[n], s_w + which * a.head_dim, it);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) dot = fmaf(gu[n][i], u[i], fmaf(gv[n][i], v[i], dot));
       }
-      for (int o = a.tpr >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      dot /= float(a.head_dim);
+    }
+    for (int o = a.tpr >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    dot /= float(a.head_dim);
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int j = in_row + n * a.tpr;
-        if (on && j < a.items) {
-          const Item it = ItemOf<VEC>(j, a);
+    for (int n = 0; n < NI; ++n) {
+      const int j = in_row + n * a.tpr;
+      if (on && j < a.items) {
+        const Item it = ItemOf<VEC>(j, a);
+        float u[VEC], v[VEC];
+        cx.Floats(n, u, v);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            gu[n][i] = r * (gu[n][i] - xu[n][i] * dot);
-            gv[n][i] = r * (gv[n][i] - xv[n][i] * dot);
-          }
-          StoreVec<T, VEC>(y + it.o0, gu[n]);
-          StoreVec<T, VEC>(y + it.o1, gv[n]);
+        for (int i = 0; i < VEC; ++i) {
+          gu[n][i] = r * (gu[n][i] - u[i] * r * dot);
+          gv[n][i] = r * (gv[n][i] - v[i] * r * dot);
         }
+        StoreVec<T, VEC>(y + it.o0, gu[n]);
+        StoreVec<T, VEC>(y + it.o1, gv[n]);
       }
     }
   }
   // the block's partial sums: rows of one position in the row tile are added in the order of their thread groups
   __syncthreads();
-  float* acc = reinterpret_cast<float*>(s_table);  // [groups][head_dim]
+  float* acc = reinterpret_cast<float*>(s_mem);  // [groups][head_dim]
 #pragma unroll
   for (int n = 0; n < NI; ++n) {
     const int j = in_row + n * a.tpr;
@@ -255,18 +316,20 @@ __global__ void __launch_bounds__(kThreads) NormRopeGradKernel(const __grid_cons
   }
 }
 
-// Column sums of the partial weight gradients, in 64 bits (up to 592 terms, a few microseconds either way).
-__global__ void __launch_bounds__(kThreads) WeightGradKernel(const __grid_constant__ RopeArgs a, int blocks) {
-  __shared__ double s_sum[kThreads / 32][33];
+// Column sums of the partial weight gradients, in 64 bits: 32 columns a block, 32 warps that take up to 10 terms each.
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) WeightGradKernel(const __grid_constant__ RopeArgs a, int blocks) {
+  __shared__ double s_sum[kSumThreads / 32][33];
   const int which = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   double sum = 0.0;
   if (c < a.head_dim)
-    for (int b = warp; b < blocks; b += kThreads / 32) sum += double(a.partial[(size_t(which) * blocks + b) * a.head_dim + c]);
+#pragma unroll 10
+    for (int b = warp; b < blocks; b += kSumThreads / 32) sum += double(a.partial[(size_t(which) * blocks + b) * a.head_dim + c]);
   s_sum[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && c < a.head_dim) {
-    for (int w = 1; w < kThreads / 32; ++w) sum += s_sum[w][lane];
+    for (int w = 1; w < kSumThreads / 32; ++w) sum += s_sum[w][lane];
     void* dw = a.side[which].dw;
     if (a.w_dtype == ITEXB_DT_FLOAT) static_cast<float*>(dw)[c] = float(sum);
     else if (a.w_dtype == ITEXB_DT_BFLOAT16) static_cast<__nv_bfloat16*>(dw)[c] = __double2bfloat16(sum);
@@ -335,29 +398,38 @@ int GradBlocks(int64_t tokens, int q_heads, int k_heads, int rows_per_block) {
   return int(std::max<int64_t>(1, std::min<int64_t>(kMaxGradBlocks, (most + rows_per_block - 1) / rows_per_block)));
 }
 
+template <typename T, int VEC, int NI, int MODE, int P> int RunPasses(RopeArgs& a, size_t weights, cudaStream_t st) {
+  const int heads = a.heads[0] + a.heads[1];
+  a.rows_per_block = kThreads / a.tpr * P;
+  const size_t smem = weights + size_t(std::min(a.rows_per_block, a.rows_per_block / heads + 2)) * a.pairs * sizeof(float2);
+  auto kernel = RopeKernel<T, VEC, NI, MODE, P>;
+  if (smem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  kernel<<<(a.rows + a.rows_per_block - 1) / a.rows_per_block, kThreads, smem, st>>>(a);
+  return CheckLaunch("RopeKernel");
+}
+
 template <typename T, int VEC, int NI, int MODE> int Run(RopeArgs& a, cudaStream_t st) {
   a.items = a.head_dim / (2 * VEC);
   a.tpr = 1;
   while (a.tpr < 32 && a.tpr < a.items) a.tpr *= 2;
-  a.rows_per_block = kThreads / a.tpr;
-  const int least = MODE == kGrad ? std::min(a.heads[0], a.heads[1] > 0 ? a.heads[1] : a.heads[0]) : a.heads[0] + a.heads[1];
-  const size_t tokens = size_t(std::min(a.rows_per_block, a.rows_per_block / least + 2));
-  size_t smem = tokens * a.pairs * sizeof(float2);
+  const int groups = kThreads / a.tpr;
+  const size_t weights = size_t(2) * a.head_dim * sizeof(float);
   if constexpr (MODE == kGrad) {
-    smem = std::max(smem, size_t(kThreads / a.tpr) * a.head_dim * sizeof(float));
+    const int least = std::min(a.heads[0], a.heads[1] > 0 ? a.heads[1] : a.heads[0]);
+    const size_t smem = std::max(weights + size_t(std::min(groups, groups / least + 2)) * a.pairs * sizeof(float2), size_t(groups) * a.head_dim * sizeof(float));
     auto kernel = NormRopeGradKernel<T, VEC, NI>;
     if (smem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
     const int sides = a.heads[1] > 0 ? 2 : 1;
-    const int blocks = GradBlocks(a.tokens, a.heads[0], a.heads[1], a.rows_per_block);
+    const int blocks = GradBlocks(a.tokens, a.heads[0], a.heads[1], groups);
     kernel<<<dim3(blocks, sides), kThreads, smem, st>>>(a);
     ITEXB_RETURN_IF_ERROR(CheckLaunch("NormRopeGradKernel"));
-    WeightGradKernel<<<dim3((a.head_dim + 31) / 32, sides), kThreads, 0, st>>>(a, blocks);
+    WeightGradKernel<<<dim3((a.head_dim + 31) / 32, sides), kSumThreads, 0, st>>>(a, blocks);
     return CheckLaunch("WeightGradKernel");
   } else {
-    auto kernel = RopeKernel<T, VEC, NI, MODE>;
-    if (smem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    kernel<<<(a.rows + a.rows_per_block - 1) / a.rows_per_block, kThreads, smem, st>>>(a);
-    return CheckLaunch("RopeKernel");
+    // four passes where that still gives every SM four blocks, and where the pieces fit the registers
+    constexpr int kPasses = NI == 1 && MODE == kRope ? 4 : 1;
+    if (kPasses > 1 && a.rows >= uint32_t(groups) * kPasses * 148 * 4) return RunPasses<T, VEC, NI, MODE, kPasses>(a, MODE == kNorm ? weights : 0, st);
+    return RunPasses<T, VEC, NI, MODE, 1>(a, MODE == kNorm ? weights : 0, st);
   }
 }
 
