@@ -37,7 +37,7 @@ int CheckAttention(const itexb_kv4_attention_params_t* p, AttnArgs* a) {
 extern "C" size_t itexb_kv4_attention_workspace_bytes(const itexb_kv4_attention_params_t* p) {
   AttnArgs a{};
   if (CheckAttention(p, &a) != ITEXB_OK || p->num_seqs == 0 || p->max_new == 0 || p->total_rows == 0) return 0;
-  return IsPrefill(a) ? 0 : StepsWorkspace(a);
+  return IsPrefill(a) ? PrefillWorkspace(a) : StepsWorkspace(a);
 }
 
 extern "C" int itexb_kv4_attention(const itexb_kv4_attention_params_t* p, itexb_stream_t stream) {
@@ -45,9 +45,9 @@ extern "C" int itexb_kv4_attention(const itexb_kv4_attention_params_t* p, itexb_
   ITEXB_RETURN_IF_ERROR(CheckAttention(p, &a));
   if (p->num_seqs == 0 || p->max_new == 0 || p->total_rows == 0) return ITEXB_OK;
   ITEXB_REQUIRE(p->q && p->out && p->kept && (p->block_table || p->table_cols == 0), ITEXB_INVALID_ARGUMENT, "kv4_attention: NULL tensor");
-  if (IsPrefill(a)) return LaunchPrefill(a, p->dtype, AsCuda(stream));
-  const size_t need = StepsWorkspace(a);
-  ITEXB_REQUIRE(need == 0 || (p->workspace && p->workspace_bytes >= need && reinterpret_cast<uintptr_t>(p->workspace) % 16 == 0), ITEXB_INVALID_ARGUMENT,
+  const size_t need = IsPrefill(a) ? PrefillWorkspace(a) : StepsWorkspace(a);
+  ITEXB_REQUIRE(p->workspace && p->workspace_bytes >= need && reinterpret_cast<uintptr_t>(p->workspace) % 16 == 0, ITEXB_INVALID_ARGUMENT,
                 "kv4_attention: a 16-byte aligned workspace of %zu bytes is needed, got %zu", need, p->workspace_bytes);
+  if (IsPrefill(a)) return LaunchPrefill(a, p->dtype, p->workspace, AsCuda(stream));
   return LaunchSteps(a, p->dtype, p->workspace, AsCuda(stream));
 }

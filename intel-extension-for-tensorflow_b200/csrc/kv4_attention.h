@@ -58,7 +58,8 @@ __device__ __forceinline__ float Exp2(float x) { float r; asm("ex2.approx.ftz.f3
 
 size_t StepsWorkspace(const AttnArgs& a);
 int LaunchSteps(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st);
-int LaunchPrefill(const AttnArgs& a, int dtype, cudaStream_t st);
+size_t PrefillWorkspace(const AttnArgs& a);
+int LaunchPrefill(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st);
 
 }  // namespace itexb
 

@@ -3,14 +3,15 @@
 // Bound: the tensor cores' 4 head_dim operations per (row, token) pair, and beside them the exponentials: 16 per clock and SM
 // against the 32 pairs per clock that the two products of head_dim 128 allow.
 //
-// One block of 512 threads owns 256 query rows of one key/value head (new tokens times the query heads that share it; 128
-// rows for head_dim 256) and walks the visible tokens in tiles of 128:
+// A unit of work is 256 query rows of one key/value head (new tokens times the query heads that share it; 128 rows for
+// head_dim 256) against the tokens they see, in tiles of 128.  One block of 512 threads per SM takes an equal, contiguous part
+// of the list of all units' tiles; units that several blocks share are joined by a second kernel:
 //   warp 0       issues tcgen05.mma (f16 operands, fp32 accumulators in tensor memory): S = q K^T and O += P V for the two
 //                halves of 128 rows in turn, so that one half's products run under the other half's softmax
 //   warp 1       allocates tensor memory: S of each half (128 columns; P overwrites it as halves), O of each half
-//   warps 4-11   softmax, a thread per row: weights 2^(s - m + 7) straight from S with the maximum m of earlier tiles; only when
-//                a row's weights of a tile add up to more than 2^15 is the maximum looked for, the accumulator rescaled and the
-//                tile done again.  Weights go back to tensor memory as the second product's A operand
+//   warps 4-11   softmax, a thread per row: weights 2^(s - m + 7) straight from S with the maximum m of earlier tokens; only
+//                when a row's weights of 32 tokens add up to more than 2^15 is the maximum looked for, and what was made with
+//                the old one rescaled.  Weights go back to tensor memory as the second product's A operand
 //   warps 12-15  a thread per token: page lookup, codes and params into registers one tile ahead, values lo + step * code as
 //                halves into shared memory in the layout the tensor cores read (128-byte swizzle; keys K-major, values
 //                MN-major: both are rows of channels)
@@ -29,7 +30,7 @@ constexpr int kThreads = 512;
 constexpr int kTokens = 128;                 // per tile
 constexpr int kRows = 128;                   // per half: lanes of tensor memory
 constexpr float kUp = 7.f;                   // weights are 2^(score - maximum + 7),
-constexpr float kLimit = 32768.f;            // and their sum over a tile at most 2^15, so that none overflows a half
+constexpr float kLimit = 32768.f;            // and their sum over 32 tokens at most 2^15, so that none overflows a half
 constexpr float kNone = 3.0e38f;             // -maximum + 7 of no scores
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 
@@ -101,23 +102,56 @@ __device__ __forceinline__ void TmemLoad32(uint32_t at, uint32_t (&v)[32]) {
                  "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
                  "+r"(v[31])::"memory");
 }
-__device__ __forceinline__ void TmemStore32(uint32_t at, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
-      "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-      "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+__device__ __forceinline__ void TmemStore16(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+__device__ __forceinline__ void TmemLoad16(uint32_t at, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                 "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
 }
 __device__ __forceinline__ void TmemStoreDone() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A row's accumulator (o_at 0: there is none yet) and the first `chunks` blocks of 16 columns of its weights times f.
+template <int DIM> __device__ __noinline__ void Rescale(uint32_t o_at, uint32_t p_at, int chunks, float f) {
+  uint32_t v[16];
+  if (o_at != 0u) {
+#pragma unroll 1
+    for (int c = 0; c < DIM / 16; ++c) {
+      TmemLoad16(o_at + c * 16, v);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+      TmemStore16(o_at + c * 16, v);
+    }
+  }
+  TmemStoreDone();
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    TmemLoad16(p_at + c * 16, v);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v[e]) : "f"(x.y * f), "f"(x.x * f));
+    }
+    TmemStore16(p_at + c * 16, v);
+  }
+  TmemStoreDone();
+}
+
 struct Shared {   // behind the operand tiles
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drained;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drained;
   uint32_t tmem;
   volatile int quit;
   int nan_values;          // some value group is stored as NaN
   uint32_t there[4][4];    // of the last four tiles: tokens that exist, 32 per word
+  int64_t sums[kThreads / 32], left;
+  int b, rt, kvh, tile;    // where this block's part begins
 };
 
 // Byte offset of 16-byte piece `piece` of row `row` in a tile of rows of DIM halves: blocks of 64 channels, 128-byte swizzle.
@@ -141,6 +175,21 @@ __device__ __forceinline__ uint4 Values8(uint32_t w, uint32_t step2, uint32_t lo
   const uint32_t u = w >> 8;
   return make_uint4(Value2(AndOr(w, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2(AndOr(w, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2),
                     Value2(AndOr(u, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2(AndOr(u, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2));
+}
+
+// Eight outputs, from the codes' order (0 4 1 5 2 6 3 7) back to the channels'.
+__device__ __forceinline__ void StoreOut8(const AttnArgs& a, int bf16, int64_t at, const float (&f)[8]) {
+  union { uint4 x; uint16_t e[8]; } out;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = f[e < 4 ? 2 * e : 2 * (e - 4) + 1];
+    out.e[e] = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+  }
+  uint16_t* to = static_cast<uint16_t*>(a.out) + at;
+  if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) *reinterpret_cast<uint4*>(to) = out.x;
+  else
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to[e] = out.e[e];
 }
 
 // A token's row of codes and params.
@@ -185,15 +234,44 @@ template <int DIM, int GROUP> struct Row {
 };
 __device__ __forceinline__ bool NotFinite(uint32_t half2) { return (half2 & 0x7c00u) == 0x7c00u || (half2 & 0x7c000000u) == 0x7c000000u; }
 
+struct Head {              // the unit that a block goes on with at its start, for the joining kernel
+  int b, kvh, row0;        // b < 0: it starts with a unit of its own
+  int first, last;         // blocks that share the unit
+};
 struct PrefillArgs {
   AttnArgs a;
-  int bf16;
+  int bf16, row_tiles;     // row tiles of a sequence at most
+  float* part_o;           // [blocks][2][head_dim / 4][rows][4]: of a unit begun by an earlier block, of one left to the next
+  float2* part_l;          // [blocks][2][rows] (shift, sum of weights)
+  Head* heads;             // [blocks]
 };
+constexpr int kMaxBlocks = 148;
+constexpr int kLeastTiles = 2;    // of a block's part, where there is little work
+
+// A unit of work: M * 128 query rows of a sequence and key/value head.  The list of units runs over sequences, their row tiles
+// and the heads, in this order.
+struct Unit { int row0, row1, begin, some_begin, end, tiles; };
+template <int ROWS> __device__ __forceinline__ Unit UnitOf(const AttnArgs& a, const Seq& q, int rt) {
+  Unit u;
+  const int rows = q.nnew * a.share;
+  u.row0 = rt * ROWS;
+  u.row1 = min(rows, u.row0 + ROWS);
+  u.begin = u.some_begin = u.end = u.tiles = 0;
+  if (u.row0 >= rows) return u;
+  u.some_begin = RowBegin(a, q, int(QuickDiv(uint32_t(u.row0), a.div_share)));
+  u.end = RowEnd(a, q, int(QuickDiv(uint32_t(u.row1 - 1), a.div_share)));
+  u.begin = u.some_begin & ~15;
+  u.tiles = max(1, (u.end - u.begin + kTokens - 1) / kTokens);   // rows that see nothing are one empty tile
+  return u;
+}
+
+// What a block works on next; every role walks the same segments.
+struct Segment { Seq q; Unit u; int b, kvh, tile0, tile1, halves; };
 
 template <int DIM, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_constant__ PrefillArgs s) {
   using H = Shape<DIM>;
-  constexpr int M = H::kHalves, ST = H::kStages, NG = DIM / GROUP;
+  constexpr int M = H::kHalves, ST = H::kStages, NG = DIM / GROUP, ROWS = M * kRows;
   const AttnArgs& a = s.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* const s_q = smem;
@@ -201,26 +279,72 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
   uint8_t* const s_v = s_k + ST * H::kTileBytes;
   Shared& sh = *reinterpret_cast<Shared*>(s_v + ST * H::kTileBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y, b = blockIdx.z;
   if ((SmemAt(smem) & 1023u) != 0) {   // the swizzle needs it; refuse rather than compute garbage
     if (threadIdx.x == 0 && a.status_word != nullptr) atomicCAS(a.status_word, 0, ITEXB_STATUS_WAIT_EXPIRED);
     return;
   }
-  const Seq q = SeqOf(a, b, threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0);
-  const int rows = q.nnew * a.share;
-  const int blocks = (rows + M * kRows - 1) / (M * kRows);
-  // the last rows see the most tokens: their blocks come first
-  const int row0 = (blocks - 1 - int(blockIdx.x)) * (M * kRows);
-  if (int(blockIdx.x) >= blocks) return;
-  const int row1 = min(rows, row0 + M * kRows);
-  const int halves = row1 - row0 > kRows ? 2 : 1;
-  const int i_first = int(QuickDiv(uint32_t(row0), a.div_share)), i_last = int(QuickDiv(uint32_t(row1 - 1), a.div_share));
-  const int some_begin = RowBegin(a, q, i_first), end = RowEnd(a, q, i_last), begin = some_begin & ~15;
-  const int tiles = end > begin ? (end - begin + kTokens - 1) / kTokens : 0;
+  // Launched programmatically: what the previous kernel of the stream wrote is visible from here on.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
+  // ---- this block's part of the list: threads add up contiguous shares of the (sequence, row tile) pairs
+  {
+    const int64_t pairs = int64_t(a.num_seqs) * s.row_tiles, per = (pairs + kThreads - 1) / kThreads;
+    const int64_t p0 = min(pairs, int64_t(threadIdx.x) * per), p1 = min(pairs, p0 + per);
+    auto walk = [&](auto visit) {   // visit(b, rt, q, unit) -> go on
+      int b = int(p0 / s.row_tiles), rt = int(p0 - int64_t(b) * s.row_tiles);
+      Seq q{};
+      for (int64_t p = p0; p < p1; ++p) {
+        if (p == p0 || rt == 0) q = SeqOf(a, b, blockIdx.x == 0 && rt == 0);
+        if (!visit(b, rt, q, UnitOf<ROWS>(a, q, rt))) return;
+        if (++rt == s.row_tiles) { rt = 0; ++b; }
+      }
+    };
+    int64_t sum = 0;
+    walk([&](int, int, const Seq&, const Unit& u) { sum += int64_t(u.tiles) * a.c.kv_heads; return true; });
+    int64_t before = sum;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, before, x);
+      if (lane >= x) before += y;
+    }
+    if (lane == 31) sh.sums[warp] = before;
+    if (threadIdx.x == 0) s.heads[blockIdx.x].b = -1;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll 1
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += sh.sums[w];
+      total += sh.sums[w];
+    }
+    before -= sum;
+    const int64_t blocks = max(int64_t(1), min(int64_t(gridDim.x), total / kLeastTiles));
+    const int64_t pos = total * blockIdx.x / blocks;
+    const int64_t stop = int64_t(blockIdx.x) < blocks ? total * (blockIdx.x + 1) / blocks : pos;
+    if (threadIdx.x == 0) sh.left = stop - pos;
+    if (stop > pos && pos >= before && pos < before + sum) {
+      int64_t at = before;
+      walk([&](int b, int rt, const Seq&, const Unit& u) {
+        const int64_t n = int64_t(u.tiles) * a.c.kv_heads;
+        if (pos >= at + n) { at += n; return true; }
+        sh.b = b;
+        sh.rt = rt;
+        sh.kvh = int((pos - at) / u.tiles);
+        sh.tile = int((pos - at) - int64_t(sh.kvh) * u.tiles);
+        if (sh.tile > 0) {
+          const int64_t x = at + int64_t(sh.kvh) * u.tiles;     // the unit's first tile in the list
+          Head h;
+          h.b = b; h.kvh = sh.kvh; h.row0 = u.row0;
+          h.first = int(((x + 1) * blocks - 1) / total);
+          h.last = int(((x + u.tiles) * blocks - 1) / total);
+          s.heads[blockIdx.x] = h;
+        }
+        return false;
+      });
+    }
+  }
   if (threadIdx.x == 0) {
-    BarInit(&sh.q_full, uint32_t(halves * kRows));
     for (int i = 0; i < 2; ++i) {
+      BarInit(&sh.q_full[i], kRows);
       BarInit(&sh.k_full[i], 128);
       BarInit(&sh.k_empty[i], 1);
       BarInit(&sh.v_full[i], 128);
@@ -235,6 +359,10 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t part = sh.left;       // tiles of this block
+  if (part == 0) return;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAt(&sh.tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -245,13 +373,51 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
   const uint32_t tmem = sh.tmem;
   volatile int* const quit = &sh.quit;
 
+  // The segments of this block's part, one after the other.
+  struct Walker {
+    int b, rt, kvh, tile;
+    int64_t left;
+    Seq q;
+    Unit u;
+    bool fresh;
+  };
+  Walker wk{sh.b, sh.rt, sh.kvh, sh.tile, part, {}, {}, true};
+  auto next_segment = [&](Segment& g) {
+    if (wk.left <= 0) return false;
+    if (wk.fresh) {
+      wk.q = SeqOf(a, wk.b, false);
+      wk.u = UnitOf<ROWS>(a, wk.q, wk.rt);
+      while (wk.u.tiles == 0) {   // a sequence has fewer row tiles than the longest
+        if (++wk.rt == s.row_tiles) { wk.rt = 0; wk.q = SeqOf(a, ++wk.b, false); }
+        wk.u = UnitOf<ROWS>(a, wk.q, wk.rt);
+      }
+      wk.fresh = false;
+    }
+    g.q = wk.q;
+    g.u = wk.u;
+    g.b = wk.b;
+    g.kvh = wk.kvh;
+    g.tile0 = wk.tile;
+    g.tile1 = int(min(int64_t(wk.u.tiles), wk.tile + wk.left));
+    g.halves = wk.u.row1 - wk.u.row0 > kRows ? 2 : 1;
+    wk.left -= g.tile1 - g.tile0;
+    wk.tile = 0;
+    if (++wk.kvh == a.c.kv_heads) {
+      wk.kvh = 0;
+      wk.fresh = true;
+      if (++wk.rt == s.row_tiles) { wk.rt = 0; ++wk.b; }
+    }
+    return true;
+  };
+  Segment g;
+
   if (warp == 0) {
     // ---------------- products ----------------
-    if (lane == 0 && tiles > 0) {
+    if (lane == 0) {
       constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(kTokens >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (uint32_t(DIM >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
-      auto scores = [&](int m, int j) {
-        const uint32_t qa = SmemAt(s_q) + m * (kRows * DIM * 2), ka = SmemAt(s_k) + (j % ST) * H::kTileBytes;
+      auto scores = [&](int m, uint32_t t, bool last) {
+        const uint32_t qa = SmemAt(s_q) + m * (kRows * DIM * 2), ka = SmemAt(s_k) + (t % ST) * H::kTileBytes;
 #pragma unroll
         for (int k = 0; k < DIM / 16; ++k) {
           const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
@@ -259,30 +425,42 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
         }
         Commit(&sh.s_full[m]);
         BarArrive(&sh.s_full[m]);
-        if (m == halves - 1) Commit(&sh.k_empty[j % ST]);
+        if (last) Commit(&sh.k_empty[t % ST]);
       };
-      bool ok = BarWait(&sh.q_full, 0, quit, a.status_word) && BarWait(&sh.k_full[0], 0, quit, a.status_word);
-      FenceAfter();
-      for (int m = 0; m < halves && ok; ++m) scores(m, 0);
-      for (int j = 0; j < tiles && ok; ++j) {
-        for (int m = 0; m < halves && ok; ++m) {
-          ok = BarWait(&sh.p_full[m], j & 1, quit, a.status_word) && (m > 0 || BarWait(&sh.v_full[j % ST], (j / ST) & 1, quit, a.status_word));
+      bool ok = true;
+      uint32_t t = 0, done[2] = {0, 0}, segs[2] = {0, 0};   // tiles; tiles of each half; segments of each half
+      while (ok && next_segment(g)) {
+        const int n = g.tile1 - g.tile0;
+        ok = BarWait(&sh.k_full[t % ST], (t / ST) & 1, quit, a.status_word);
+        for (int m = 0; m < g.halves && ok; ++m) {
+          // the half's last weights of the segment before have been read, its next rows of q are there
+          ok = (done[m] == 0 || BarWait(&sh.o_done[m], (done[m] - 1) & 1, quit, a.status_word)) && BarWait(&sh.q_full[m], segs[m] & 1, quit, a.status_word);
           if (!ok) break;
+          ++segs[m];
           FenceAfter();
-          const uint32_t va = SmemAt(s_v) + (j % ST) * H::kTileBytes;
-#pragma unroll
-          for (int k = 0; k < kTokens / 16; ++k)
-            MmaTmem(tmem + H::kOColumn + m * DIM, tmem + m * 128 + k * 8, Desc(va + k * 2048, 128 * 128), kIdescO, j > 0 || k > 0);
-          Commit(&sh.o_done[m]);
-          BarArrive(&sh.o_done[m]);
-          if (m == halves - 1) Commit(&sh.v_empty[j % ST]);
-          if (j + 1 < tiles) {
-            ok = m > 0 || BarWait(&sh.k_full[(j + 1) % ST], ((j + 1) / ST) & 1, quit, a.status_word);
-            // P is read from where the next S goes
-            ok = ok && BarWait(&sh.o_done[m], j & 1, quit, a.status_word);
+          scores(m, t, m == g.halves - 1);
+        }
+        for (int j = 0; j < n && ok; ++j, ++t) {
+          for (int m = 0; m < g.halves && ok; ++m) {
+            ok = BarWait(&sh.p_full[m], done[m] & 1, quit, a.status_word) && (m > 0 || BarWait(&sh.v_full[t % ST], (t / ST) & 1, quit, a.status_word));
             if (!ok) break;
             FenceAfter();
-            scores(m, j + 1);
+            const uint32_t va = SmemAt(s_v) + (t % ST) * H::kTileBytes;
+#pragma unroll
+            for (int k = 0; k < kTokens / 16; ++k)
+              MmaTmem(tmem + H::kOColumn + m * DIM, tmem + m * 128 + k * 8, Desc(va + k * 2048, 128 * 128), kIdescO, j > 0 || k > 0);
+            Commit(&sh.o_done[m]);
+            BarArrive(&sh.o_done[m]);
+            if (m == g.halves - 1) Commit(&sh.v_empty[t % ST]);
+            if (j + 1 < n) {
+              ok = m > 0 || BarWait(&sh.k_full[(t + 1) % ST], ((t + 1) / ST) & 1, quit, a.status_word);
+              // P is read from where the next S goes
+              ok = ok && BarWait(&sh.o_done[m], done[m] & 1, quit, a.status_word);
+              if (!ok) break;
+              FenceAfter();
+              scores(m, t + 1, m == g.halves - 1);
+            }
+            ++done[m];
           }
         }
       }
@@ -290,235 +468,229 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       Commit(&sh.drained);
       BarWait(&sh.drained, 0, nullptr, a.status_word);
     }
-  } else if (warp >= 4 && warp < 4 + 4 * halves) {
+  } else if (warp >= 4 && warp < 4 + 4 * M) {
     // ---------------- softmax ----------------
     const int m = (warp - 4) >> 2, in_half = (warp & 3) * 32 + lane;
-    const int rr = row0 + m * kRows + in_half;
-    const bool on = rr < row1;
-    const int i = int(QuickDiv(uint32_t(on ? rr : row0), a.div_share)), h = (on ? rr : row0) - i * a.share;
-    const int lo = on ? RowBegin(a, q, i) : 0, hi = on ? RowEnd(a, q, i) : 0;
-    // tokens that all rows of this warp see
-    const int w_first = int(QuickDiv(uint32_t(min(row1 - 1, row0 + m * kRows + (warp & 3) * 32)), a.div_share));
-    const int w_last = int(QuickDiv(uint32_t(min(row1, row0 + m * kRows + (warp & 3) * 32 + 32) - 1), a.div_share));
-    const int all_begin = RowBegin(a, q, max(w_first, w_last)), all_end = RowEnd(a, q, min(w_first, w_last));
-    float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-    {
-      // ---- the row of q: half, scaled, in the codes' order
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (q.row0 + i) * a.qt + int64_t(kvh * a.share + h) * a.qh;
-      union Piece { uint4 v; uint32_t u[4]; uint16_t e[8]; };
-      auto piece = [&](int p) {
-        Piece x;
-        if (!on) x.v = make_uint4(0, 0, 0, 0);
-        else if (a.q_aligned) x.v = __ldg(reinterpret_cast<const uint4*>(src) + p);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x.e[e] = src[p * 8 + e];
-        return x;
-      };
-      float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
-      if (s.bf16) {
-        float most = 0.f;
-#pragma unroll 4
-        for (int p = 0; p < DIM / 8; ++p) {
-          const Piece x = piece(p);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x.e[e]) << 16)));
-        }
-        const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
-        if (most > 0.f && most < INFINITY) {
-          down *= __uint_as_float(uint32_t(254 - e) << 23);
-          scale = fmaxf(scale * __uint_as_float(uint32_t(e) << 23), 1e-37f);
-        }
-      }
-      uint8_t* const to = s_q + m * (kRows * DIM * 2);
-#pragma unroll 4
-      for (int p = 0; p < DIM / 8; ++p) {
-        Piece x = piece(p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float raw = s.bf16 ? __uint_as_float(uint32_t(x.e[e]) << 16) : __half2float(__ushort_as_half(x.e[e]));
-          x.e[e] = __half_as_ushort(__float2half_rn(raw * down));
-        }
-        *reinterpret_cast<uint4*>(to + PieceAt(in_half, p)) =
-            make_uint4(__byte_perm(x.u[0], x.u[2], 0x5410), __byte_perm(x.u[0], x.u[2], 0x7632), __byte_perm(x.u[1], x.u[3], 0x5410), __byte_perm(x.u[1], x.u[3], 0x7632));
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      BarArrive(&sh.q_full);
-    }
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + H::kOColumn + m * DIM;
-    float shift = kNone, total = 0.f;       // weights are 2^(score * scale + shift)
+    uint32_t tile = 0, t4 = 0;   // tiles of this half; all tiles of the block
     bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      ok = BarWait(&sh.s_full[m], j & 1, quit, a.status_word);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      FenceAfter();
-      const int j0 = begin + j * kTokens;
-      const uint32_t* there = sh.there[j & 3];
-      const bool partial = j0 < all_begin || j0 + kTokens > all_end || (there[0] & there[1] & there[2] & there[3]) != 0xffffffffu;
-      uint32_t p[kTokens / 2];
-      float sum = 0.f;
-      auto weights = [&]() {
-        float part[2] = {0.f, 0.f};
+    while (ok && next_segment(g)) {
+      const int n = g.tile1 - g.tile0;
+      if (m >= g.halves) { t4 += n; continue; }
+      const int rr = g.u.row0 + m * kRows + in_half;
+      const bool on = rr < g.u.row1;
+      const int i = int(QuickDiv(uint32_t(on ? rr : g.u.row0), a.div_share)), h = g.kvh * a.share + (on ? rr : g.u.row0) - i * a.share;
+      const int lo = on ? RowBegin(a, g.q, i) : 0, hi = on ? RowEnd(a, g.q, i) : 0;
+      // tokens that all rows of this warp see
+      const int w_row = g.u.row0 + m * kRows + (warp & 3) * 32;
+      const int w_first = int(QuickDiv(uint32_t(min(g.u.row1 - 1, w_row)), a.div_share)), w_last = int(QuickDiv(uint32_t(min(g.u.row1, w_row + 32) - 1), a.div_share));
+      const int all_begin = RowBegin(a, g.q, max(w_first, w_last)), all_end = RowEnd(a, g.q, min(w_first, w_last));
+      float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+      {
+        // ---- the row of q: half, scaled, in the codes' order
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (g.q.row0 + i) * a.qt + int64_t(h) * a.qh;
+        union Piece { uint4 v; uint32_t u[4]; uint16_t e[8]; };
+        auto piece = [&](int p) {
+          Piece x;
+          if (!on) x.v = make_uint4(0, 0, 0, 0);
+          else if (a.q_aligned) x.v = __ldg(reinterpret_cast<const uint4*>(src) + p);
+          else
 #pragma unroll
+            for (int e = 0; e < 8; ++e) x.e[e] = src[p * 8 + e];
+          return x;
+        };
+        float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
+        if (s.bf16) {
+          float most = 0.f;
+#pragma unroll 4
+          for (int p = 0; p < DIM / 8; ++p) {
+            const Piece x = piece(p);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x.e[e]) << 16)));
+          }
+          const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
+          if (most > 0.f && most < INFINITY) {
+            down *= __uint_as_float(uint32_t(254 - e) << 23);
+            scale = fmaxf(scale * __uint_as_float(uint32_t(e) << 23), 1e-37f);
+          }
+        }
+        uint8_t* const to = s_q + m * (kRows * DIM * 2);
+#pragma unroll 4
+        for (int p = 0; p < DIM / 8; ++p) {
+          Piece x = piece(p);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float raw = s.bf16 ? __uint_as_float(uint32_t(x.e[e]) << 16) : __half2float(__ushort_as_half(x.e[e]));
+            x.e[e] = __half_as_ushort(__float2half_rn(raw * down));
+          }
+          *reinterpret_cast<uint4*>(to + PieceAt(in_half, p)) =
+              make_uint4(__byte_perm(x.u[0], x.u[2], 0x5410), __byte_perm(x.u[0], x.u[2], 0x7632), __byte_perm(x.u[1], x.u[3], 0x5410), __byte_perm(x.u[1], x.u[3], 0x7632));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        BarArrive(&sh.q_full[m]);
+      }
+      float shift = kNone, total = 0.f;       // weights are 2^(score * scale + shift)
+      for (int j = 0; j < n && ok; ++j, ++tile, ++t4) {
+        ok = BarWait(&sh.s_full[m], tile & 1, quit, a.status_word);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        FenceAfter();
+        const int j0 = g.u.begin + (g.tile0 + j) * kTokens;
+        const uint32_t* there = sh.there[t4 & 3];
+        const bool partial = j0 < all_begin || j0 + kTokens > all_end || (there[0] & there[1] & there[2] & there[3]) != 0xffffffffu;
+        // 32 tokens at a time, a short loop that stays in the instruction cache; P's columns 16 c .. are S's columns of
+        // tokens that have been read already
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
+          uint32_t v[32], p[16];
           TmemLoad32(s_at + c * 32, v);
           if (partial) {
             const uint32_t word = there[c];
+            const int from = lo - (j0 + c * 32), to = hi - (j0 + c * 32);   // visible: from <= e < to
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int t = j0 + c * 32 + e;
-              if (t < lo || t >= hi || ((word >> e) & 1u) == 0u) v[e] = 0xff800000u;
+            for (int e = 0; e < 32; ++e)
+              if (e < from || e >= to || ((word >> e) & 1u) == 0u) v[e] = 0xff800000u;
+          }
+          float part[2];
+          auto weights = [&]() {
+            part[0] = part[1] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float x = Exp2(fmaf(__uint_as_float(v[e]), scale, shift)), y = Exp2(fmaf(__uint_as_float(v[e + 1]), scale, shift));
+              part[0] += x;
+              part[1] += y;
+              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[e / 2]) : "f"(y), "f"(x));
             }
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float x = Exp2(fmaf(__uint_as_float(v[e]), scale, shift)), y = Exp2(fmaf(__uint_as_float(v[e + 1]), scale, shift));
-            part[0] += x;
-            part[1] += y;
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[c * 16 + e / 2]) : "f"(y), "f"(x));
-          }
-        }
-        sum = part[0] + part[1];
-      };
-      weights();
-      if (__any_sync(0xffffffffu, sum > kLimit)) {
-        // a new maximum for the rows that passed it
-        float top = -INFINITY;
+          };
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          TmemLoad32(s_at + c * 32, v);
-          const uint32_t word = there[c];
+          for (;;) {
+            weights();
+            if (!__any_sync(0xffffffffu, part[0] + part[1] > kLimit)) break;
+            // a new maximum for the rows that passed it; what was made with the old one is scaled
+            float top = __uint_as_float(v[0]);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int t = j0 + c * 32 + e;
-            if (!partial || (t >= lo && t < hi && ((word >> e) & 1u) != 0u)) top = fmaxf(top, __uint_as_float(v[e]));
+            for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+            const float to = fminf(shift, kUp - top * scale);
+            const float f = Exp2(to - shift);
+            shift = to;
+            total *= f;
+            Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
           }
+          total += part[0] + part[1];
+          TmemStore16(s_at + c * 16, p);
         }
-        const float to = fminf(shift, kUp - top * scale);
-        const float f = Exp2(to - shift);
-        shift = to;
-        total *= f;
-        if (j > 0) {
-#pragma unroll 1
-          for (int c = 0; c < DIM / 32; ++c) {
-            uint32_t v[32];
-            TmemLoad32(o_at + c * 32, v);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-            TmemStore32(o_at + c * 32, v);
-          }
-        }
-        weights();
+        TmemStoreDone();
+        FenceBefore();
+        BarArrive(&sh.p_full[m]);
       }
-      total += sum;
-      TmemStore32(s_at, p);
-      TmemStore32(s_at + 32, p + 32);
-      TmemStoreDone();
-      FenceBefore();
-      BarArrive(&sh.p_full[m]);
-    }
-    if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, BarWait(&sh.o_done[m], (tiles - 1) & 1, quit, a.status_word));
-    if (ok) {
+      if (ok) ok = __all_sync(0xffffffffu, BarWait(&sh.o_done[m], (tile - 1) & 1, quit, a.status_word));
+      if (!ok) break;
       FenceAfter();
       uint32_t nan_groups = 0;
-      if (tiles > 0 && sh.nan_values != 0) {   // rare: find the value groups that are NaN among the tokens this row sees
+      if (sh.nan_values != 0) {   // rare: find the value groups that are NaN among the tokens this row sees
         for (int t = lo; t < hi; ++t) {
-          const int col = int(QuickDiv(uint32_t(t), a.c.div_page)), page = __ldg(a.table + int64_t(b) * a.table_stride + col);
+          const int col = int(QuickDiv(uint32_t(t), a.c.div_page)), page = __ldg(a.table + int64_t(g.b) * a.table_stride + col);
           if (page < 0 || page >= a.c.num_pages) continue;
-          const __half2* at = a.c.v_params + int64_t(page) * a.c.pp + int64_t(kvh) * a.c.ph + int64_t(t - col * a.c.page_size) * a.c.pt;
-          for (int g = 0; g < NG; ++g) nan_groups |= uint32_t(NotFinite(__ldg(reinterpret_cast<const uint32_t*>(at + g)))) << g;
+          const __half2* at = a.c.v_params + int64_t(page) * a.c.pp + int64_t(g.kvh) * a.c.ph + int64_t(t - col * a.c.page_size) * a.c.pt;
+          for (int x = 0; x < NG; ++x) nan_groups |= uint32_t(NotFinite(__ldg(reinterpret_cast<const uint32_t*>(at + x)))) << x;
         }
       }
       __syncwarp();
+      const bool whole = g.tile1 - g.tile0 == g.u.tiles;
+      const int64_t slot = int64_t(blockIdx.x) * 2 + (g.tile0 == 0);
+      const int in_unit = m * kRows + in_half;
+      if (!whole) s.part_l[slot * ROWS + in_unit] = make_float2(shift, total);
+      float4* const part_to = reinterpret_cast<float4*>(s.part_o) + slot * (DIM / 4) * ROWS + in_unit;
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int64_t at = (q.row0 + i) * a.ot + int64_t(kvh * a.share + h) * a.oh;
-      const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ot & 7) == 0 && (a.oh & 7) == 0;
+      const int64_t at = (g.q.row0 + i) * a.ot + int64_t(h) * a.oh;
 #pragma unroll 1
       for (int c = 0; c < DIM / 32; ++c) {
         uint32_t v[32];
         __syncwarp();
-        if (tiles > 0) TmemLoad32(o_at + c * 32, v);
-        else
+        TmemLoad32(o_at + c * 32, v);
+        if ((nan_groups >> (c * 32 / GROUP)) & 1u) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
-        const bool is_nan = (nan_groups >> (c * 32 / GROUP)) & 1u;
+          for (int e = 0; e < 32; ++e) v[e] = 0x7fffffffu;
+        }
+        if (!whole) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          union { uint4 x; uint16_t e[8]; } out;
+          for (int w = 0; w < 8; ++w)
+            part_to[(c * 8 + w) * ROWS] = make_float4(__uint_as_float(v[4 * w]), __uint_as_float(v[4 * w + 1]), __uint_as_float(v[4 * w + 2]), __uint_as_float(v[4 * w + 3]));
+        } else if (on) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int from = e < 4 ? 2 * e : 2 * (e - 4) + 1;   // back from the codes' order
-            const float f = is_nan ? __uint_as_float(0x7fffffffu) : (total == 0.f ? 0.f : __uint_as_float(v[w * 8 + from]) * inv);
-            out.e[e] = s.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
-          }
-          if (on) {
-            uint16_t* to = static_cast<uint16_t*>(a.out) + at + c * 32 + w * 8;
-            if (wide) *reinterpret_cast<uint4*>(to) = out.x;
-            else
+          for (int w = 0; w < 4; ++w) {
+            float f[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) to[e] = out.e[e];
+            for (int e = 0; e < 8; ++e) f[e] = total == 0.f ? 0.f : __uint_as_float(v[w * 8 + e]) * inv;
+            StoreOut8(a, s.bf16, at + c * 32 + w * 8, f);
           }
         }
       }
+      FenceBefore();
     }
-    FenceBefore();
   } else if (warp >= 12) {
     // ---------------- codes to operands ----------------
     const int t = threadIdx.x - 12 * 32, w = warp - 12;
-    const int32_t* table = a.table + int64_t(b) * a.table_stride;
-    const uint8_t* kc = a.c.k_codes + int64_t(kvh) * a.c.ch;
-    const uint8_t* vc = a.c.v_codes + int64_t(kvh) * a.c.ch;
-    const __half2* kp = a.c.k_params + int64_t(kvh) * a.c.ph;
-    const __half2* vp = a.c.v_params + int64_t(kvh) * a.c.ph;
     Row<DIM, GROUP> k, v;
-    // the page of this thread's token of a tile, -1 where there is none
-    auto page_of = [&](int j) {
-      const int tok = begin + j * kTokens + t;
-      if (j >= tiles || tok < some_begin || tok >= end) return -1;
-      const int page = __ldg(table + QuickDiv(uint32_t(tok), a.c.div_page));
-      if (page >= 0 && page < a.c.num_pages) return page;
-      ReportIndex(a.status_word);
-      return -1;
-    };
-    auto offset_of = [&](int j) {
-      const int tok = begin + j * kTokens + t;
-      return tok - int(QuickDiv(uint32_t(tok), a.c.div_page)) * a.c.page_size;
-    };
-    auto load = [&](Row<DIM, GROUP>& r, const uint8_t* codes, const __half2* params, int page, int j) {
-      if (page < 0) { r.Clear(); return; }
-      const int64_t off = offset_of(j);
-      r.Load(codes + int64_t(page) * a.c.cp + off * a.c.ct, params + int64_t(page) * a.c.pp + off * a.c.pt);
-    };
-    int page = page_of(0), next = page_of(1);
-    load(k, kc, kp, page, 0);
-    load(v, vc, vp, page, 0);
+    uint32_t n = 0;      // tiles so far
     bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int after = page_of(j + 2);
-      if (j >= ST) ok = BarWait(&sh.k_empty[j % ST], ((j / ST) - 1) & 1, quit, a.status_word);
+    // a tile: where this thread's token lies, -1 where there is none
+    struct Place { int page, off, kvh; };
+    Segment ahead{};
+    int ahead_tile = 0;
+    bool more = next_segment(ahead);
+    ahead_tile = ahead.tile0;
+    auto place = [&]() {   // of the tile `ahead` stands at, and one on
+      Place x{-1, 0, 0};
+      if (!more) return x;
+      const int tok = ahead.u.begin + ahead_tile * kTokens + t;
+      x.kvh = ahead.kvh;
+      if (tok >= ahead.u.some_begin && tok < ahead.u.end) {
+        const int col = int(QuickDiv(uint32_t(tok), a.c.div_page));
+        x.off = tok - col * a.c.page_size;
+        x.page = __ldg(a.table + int64_t(ahead.b) * a.table_stride + col);
+        if (x.page < 0 || x.page >= a.c.num_pages) {
+          ReportIndex(a.status_word);
+          x.page = -1;
+        }
+      }
+      if (++ahead_tile == ahead.tile1) {
+        more = next_segment(ahead);
+        ahead_tile = ahead.tile0;
+      }
+      return x;
+    };
+    auto load = [&](Row<DIM, GROUP>& r, const uint8_t* codes, const __half2* params, const Place& x) {
+      if (x.page < 0) { r.Clear(); return; }
+      r.Load(codes + int64_t(x.page) * a.c.cp + int64_t(x.kvh) * a.c.ch + int64_t(x.off) * a.c.ct,
+             params + int64_t(x.page) * a.c.pp + int64_t(x.kvh) * a.c.ph + int64_t(x.off) * a.c.pt);
+    };
+    Place now = place(), next = place();
+    load(k, a.c.k_codes, a.c.k_params, now);
+    load(v, a.c.v_codes, a.c.v_params, now);
+    for (int64_t j = 0; j < part && ok; ++j, ++n) {
+      const Place after = place();
+      if (n >= uint32_t(ST)) ok = BarWait(&sh.k_empty[n % ST], (n / ST - 1) & 1, quit, a.status_word);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      k.Store(s_k + (j % ST) * H::kTileBytes, t);
-      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0) sh.there[j & 3][w] = there;
+      k.Store(s_k + (n % ST) * H::kTileBytes, t);
+      const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
+      if (lane == 0) sh.there[n & 3][w] = there;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      BarArrive(&sh.k_full[j % ST]);
-      load(k, kc, kp, next, j + 1);
-      if (j >= ST) ok = BarWait(&sh.v_empty[j % ST], ((j / ST) - 1) & 1, quit, a.status_word);
+      BarArrive(&sh.k_full[n % ST]);
+      load(k, a.c.k_codes, a.c.k_params, next);
+      if (n >= uint32_t(ST)) ok = BarWait(&sh.v_empty[n % ST], (n / ST - 1) & 1, quit, a.status_word);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       bool bad = false;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        if (NotFinite(v.params[g])) { v.params[g] = 0; bad = true; }
+      for (int x = 0; x < NG; ++x)
+        if (NotFinite(v.params[x])) { v.params[x] = 0; bad = true; }
       if (bad) sh.nan_values = 1;
-      v.Store(s_v + (j % ST) * H::kTileBytes, t);
+      v.Store(s_v + (n % ST) * H::kTileBytes, t);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      BarArrive(&sh.v_full[j % ST]);
-      load(v, vc, vp, next, j + 1);
-      page = next;
+      BarArrive(&sh.v_full[n % ST]);
+      load(v, a.c.v_codes, a.c.v_params, next);
+      now = next;
       next = after;
     }
   }
@@ -530,17 +702,79 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
   }
 }
 
-template <int DIM, int GROUP> int LaunchGroup(const PrefillArgs& s, cudaStream_t st) {
+// Joins the parts of a unit that several blocks worked on.  blockIdx.x: the block that went on with it first; a thread adds 8
+// channels of one row.
+template <int DIM>
+__global__ void __launch_bounds__(256) PrefillJoinKernel(const __grid_constant__ PrefillArgs s) {
+  constexpr int ROWS = Shape<DIM>::kHalves * kRows;
+  const AttnArgs& a = s.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Head h = s.heads[blockIdx.x];
+  if (h.b < 0 || h.first + 1 != int(blockIdx.x)) return;
+  const Seq q = SeqOf(a, h.b, false);
+  const int x = blockIdx.y * 256 + threadIdx.x, row = x % ROWS, piece = x / ROWS;   // threads along rows: the parts lie so
+  const int rr = h.row0 + row;
+  if (rr >= q.nnew * a.share) return;
+  float least = kNone;
+  for (int c = h.first; c <= h.last; ++c) least = fminf(least, s.part_l[(int64_t(c) * 2 + (c == h.first)) * ROWS + row].x);
+  float sum = 0.f, f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = 0.f;
+#pragma unroll 4
+  for (int c = h.first; c <= h.last; ++c) {
+    const int64_t slot = int64_t(c) * 2 + (c == h.first);
+    const float2 l = s.part_l[slot * ROWS + row];
+    const float w = l.x >= kNone ? (isnan(l.y) ? l.y : 0.f) : Exp2(least - l.x);
+    const float4* from = reinterpret_cast<const float4*>(s.part_o) + (slot * (DIM / 4) + piece * 2) * ROWS + row;
+    const float4 u = from[0], v = from[ROWS];
+    const float o[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    sum = fmaf(l.y, w, sum);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fmaf(o[e], w, f[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = sum == 0.f ? 0.f : f[e] / sum;
+  const int i = int(QuickDiv(uint32_t(rr), a.div_share));
+  StoreOut8(a, s.bf16, (q.row0 + i) * a.ot + int64_t(h.kvh * a.share + rr - i * a.share) * a.oh + piece * 8, f);
+}
+
+size_t PartBytes(const AttnArgs& a) {
+  const size_t rows = (a.c.head_dim == 256 ? 1 : 2) * kRows;
+  return size_t(kMaxBlocks) * 2 * rows * (size_t(a.c.head_dim) * sizeof(float) + sizeof(float2));
+}
+
+template <int DIM, int GROUP> int LaunchGroup(PrefillArgs& s, cudaStream_t st) {
   using H = Shape<DIM>;
-  constexpr int kSmem = H::kSmem + int(sizeof(Shared));
+  constexpr int kSmem = H::kSmem + int(sizeof(Shared)), ROWS = H::kHalves * kRows;
   auto kernel = PrefillKernel<DIM, GROUP>;
   ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const int64_t rows = int64_t(s.a.max_new) * s.a.share;
-  const dim3 grid(unsigned((rows + H::kHalves * kRows - 1) / (H::kHalves * kRows)), s.a.c.kv_heads, s.a.num_seqs);
-  kernel<<<grid, kThreads, kSmem, st>>>(s);
-  return CheckLaunch("PrefillKernel");
+  s.row_tiles = int((rows + ROWS - 1) / ROWS);
+  int64_t span = std::min<int64_t>(s.a.max_kept, int64_t(s.a.table_cols) * s.a.c.page_size);
+  if (s.a.window > 0) span = std::min<int64_t>(span, int64_t(s.a.window) + s.a.max_new);
+  const int64_t most = (span / kTokens + 2) * s.a.num_seqs * s.row_tiles * s.a.c.kv_heads;   // tiles
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(std::min(kMaxBlocks, SmCount()), std::max<int64_t>(1, most / kLeastTiles))));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const unsigned blocks = cfg.gridDim.x;
+  ITEXB_CUDA(cudaLaunchKernelEx(&cfg, kernel, s));
+  ITEXB_RETURN_IF_ERROR(CheckLaunch("PrefillKernel"));
+  if (blocks == 1) return ITEXB_OK;
+  cfg.gridDim = dim3(blocks, ROWS * (DIM / 8) / 256);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  ITEXB_CUDA(cudaLaunchKernelEx(&cfg, PrefillJoinKernel<DIM>, s));
+  return CheckLaunch("PrefillJoinKernel");
 }
-template <int DIM> int LaunchDim(const PrefillArgs& s, cudaStream_t st) {
+template <int DIM> int LaunchDim(PrefillArgs& s, cudaStream_t st) {
   if (s.a.c.group == 32) return LaunchGroup<DIM, 32>(s, st);
   if (s.a.c.group == 64) return LaunchGroup<DIM, 64>(s, st);
   if constexpr (DIM >= 128) return LaunchGroup<DIM, 128>(s, st);
@@ -549,8 +783,15 @@ template <int DIM> int LaunchDim(const PrefillArgs& s, cudaStream_t st) {
 
 }  // namespace
 
-int LaunchPrefill(const AttnArgs& a, int dtype, cudaStream_t st) {
-  PrefillArgs s{a, dtype == ITEXB_DT_BFLOAT16};
+size_t PrefillWorkspace(const AttnArgs& a) { return PartBytes(a) + kMaxBlocks * sizeof(Head); }
+
+int LaunchPrefill(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st) {
+  PrefillArgs s{};
+  s.a = a;
+  s.bf16 = dtype == ITEXB_DT_BFLOAT16;
+  s.part_o = static_cast<float*>(workspace);
+  s.part_l = reinterpret_cast<float2*>(s.part_o + size_t(kMaxBlocks) * 2 * (a.c.head_dim == 256 ? 1 : 2) * kRows * a.c.head_dim);
+  s.heads = reinterpret_cast<Head*>(static_cast<uint8_t*>(workspace) + PartBytes(a));
   if (a.c.head_dim == 64) return LaunchDim<64>(s, st);
   if (a.c.head_dim == 128) return LaunchDim<128>(s, st);
   return LaunchDim<256>(s, st);
