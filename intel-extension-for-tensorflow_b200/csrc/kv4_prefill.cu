@@ -88,7 +88,8 @@ __device__ __forceinline__ void MmaTmem(uint32_t d, uint32_t a, uint64_t b, uint
 __device__ __forceinline__ uint64_t Desc(uint32_t at, uint32_t lead) {
   return uint64_t((at & 0x3ffffu) >> 4) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
-__device__ __forceinline__ void TmemLoad32(uint32_t at, uint32_t (&v)[32]) {
+// A load of 32 columns in two steps; the registers are in the second's operands so that no use moves above it.
+__device__ __forceinline__ void TmemLoadStart(uint32_t at, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -96,11 +97,17 @@ __device__ __forceinline__ void TmemLoad32(uint32_t at, uint32_t (&v)[32]) {
         "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
         "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(at));
+}
+__device__ __forceinline__ void TmemLoadDone(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
                  "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
                  "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
                  "+r"(v[31])::"memory");
+}
+__device__ __forceinline__ void TmemLoad32(uint32_t at, uint32_t (&v)[32]) {
+  TmemLoadStart(at, v);
+  TmemLoadDone(v);
 }
 __device__ __forceinline__ void TmemStore16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -118,8 +125,11 @@ __device__ __forceinline__ void TmemLoad16(uint32_t at, uint32_t (&v)[16]) {
 }
 __device__ __forceinline__ void TmemStoreDone() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+template <int N> __device__ __forceinline__ void RegistersDown() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void RegistersUp() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // A row's accumulator (o_at 0: there is none yet) and the first `chunks` blocks of 16 columns of its weights times f.
-template <int DIM> __device__ __noinline__ void Rescale(uint32_t o_at, uint32_t p_at, int chunks, float f) {
+template <int DIM> __device__ __forceinline__ void Rescale(uint32_t o_at, uint32_t p_at, int chunks, float f) {
   uint32_t v[16];
   if (o_at != 0u) {
 #pragma unroll 1
@@ -143,16 +153,6 @@ template <int DIM> __device__ __noinline__ void Rescale(uint32_t o_at, uint32_t 
   }
   TmemStoreDone();
 }
-
-struct Shared {   // behind the operand tiles
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drained;
-  uint32_t tmem;
-  volatile int quit;
-  int nan_values;          // some value group is stored as NaN
-  uint32_t there[4][4];    // of the last four tiles: tokens that exist, 32 per word
-  int64_t sums[kThreads / 32], left;
-  int b, rt, kvh, tile;    // where this block's part begins
-};
 
 // Byte offset of 16-byte piece `piece` of row `row` in a tile of rows of DIM halves: blocks of 64 channels, 128-byte swizzle.
 __device__ __forceinline__ uint32_t PieceAt(int row, int piece) {
@@ -246,6 +246,7 @@ struct PrefillArgs {
   Head* heads;             // [blocks]
 };
 constexpr int kMaxBlocks = 148;
+constexpr int kIssueRegs = 56, kSoftmaxRegs = 176, kConvertRegs = 104, kIssueRegsAlone = 80;
 constexpr int kLeastTiles = 2;    // of a block's part, where there is little work
 
 // A unit of work: M * 128 query rows of a sequence and key/value head.  The list of units runs over sequences, their row tiles
@@ -267,6 +268,19 @@ template <int ROWS> __device__ __forceinline__ Unit UnitOf(const AttnArgs& a, co
 
 // What a block works on next; every role walks the same segments.
 struct Segment { Seq q; Unit u; int b, kvh, tile0, tile1, halves; };
+struct Walker { int64_t left; int b, rt, kvh, tile; bool fresh; };   // what lies behind it
+
+struct Shared {   // behind the operand tiles
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drained;
+  uint32_t tmem;
+  volatile int quit;
+  int nan_values;          // some value group is stored as NaN
+  uint32_t there[4][4];    // of the last four tiles: tokens that exist, 32 per word
+  int64_t sums[kThreads / 32], left;
+  int b, rt, kvh, tile;    // where this block's part begins
+  Walker walk[kThreads / 32];
+  Segment seg[kThreads / 32];
+};
 
 template <int DIM, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_constant__ PrefillArgs s) {
@@ -373,33 +387,31 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
   const uint32_t tmem = sh.tmem;
   volatile int* const quit = &sh.quit;
 
-  // The segments of this block's part, one after the other.
-  struct Walker {
-    int b, rt, kvh, tile;
-    int64_t left;
-    Seq q;
-    Unit u;
-    bool fresh;
-  };
-  Walker wk{sh.b, sh.rt, sh.kvh, sh.tile, part, {}, {}, true};
-  auto next_segment = [&](Segment& g) {
-    if (wk.left <= 0) return false;
+  // The segments of this block's part, one after the other: each warp walks them by itself, its place in shared memory (in
+  // registers it would cost every role twenty).
+  Walker& wk = sh.walk[warp];
+  Segment& g = sh.seg[warp];
+  if (lane == 0) {
+    wk.b = sh.b; wk.rt = sh.rt; wk.kvh = sh.kvh; wk.tile = sh.tile;
+    wk.left = part;
+    wk.fresh = true;
+  }
+  auto advance = [&]() {   // one thread
+    if (wk.left <= 0) { g.tile0 = g.tile1 = 0; return; }
     if (wk.fresh) {
-      wk.q = SeqOf(a, wk.b, false);
-      wk.u = UnitOf<ROWS>(a, wk.q, wk.rt);
-      while (wk.u.tiles == 0) {   // a sequence has fewer row tiles than the longest
-        if (++wk.rt == s.row_tiles) { wk.rt = 0; wk.q = SeqOf(a, ++wk.b, false); }
-        wk.u = UnitOf<ROWS>(a, wk.q, wk.rt);
+      g.q = SeqOf(a, wk.b, false);
+      g.u = UnitOf<ROWS>(a, g.q, wk.rt);
+      while (g.u.tiles == 0) {   // a sequence has fewer row tiles than the longest
+        if (++wk.rt == s.row_tiles) { wk.rt = 0; g.q = SeqOf(a, ++wk.b, false); }
+        g.u = UnitOf<ROWS>(a, g.q, wk.rt);
       }
       wk.fresh = false;
     }
-    g.q = wk.q;
-    g.u = wk.u;
     g.b = wk.b;
     g.kvh = wk.kvh;
     g.tile0 = wk.tile;
-    g.tile1 = int(min(int64_t(wk.u.tiles), wk.tile + wk.left));
-    g.halves = wk.u.row1 - wk.u.row0 > kRows ? 2 : 1;
+    g.tile1 = int(min(int64_t(g.u.tiles), wk.tile + wk.left));
+    g.halves = g.u.row1 - g.u.row0 > kRows ? 2 : 1;
     wk.left -= g.tile1 - g.tile0;
     wk.tile = 0;
     if (++wk.kvh == a.c.kv_heads) {
@@ -407,13 +419,21 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       wk.fresh = true;
       if (++wk.rt == s.row_tiles) { wk.rt = 0; ++wk.b; }
     }
-    return true;
   };
-  Segment g;
+  auto next_segment = [&]() {   // the whole warp
+    __syncwarp();
+    if (lane == 0) advance();
+    __syncwarp();
+    return g.tile1 > g.tile0;
+  };
 
-  if (warp == 0) {
+  // Registers go from the warps that issue and convert to the softmax warps.  Per thread, by groups of four warps, of the
+  // launch's 4 x 128: 56, 176, 176, 104 (head_dim 256, where the third group has no work: 80, 176, 80, 128).
+  // Each role's branch states its own, so that its code is compiled for it.
+  if (warp < 4) {
+    RegistersDown<M == 2 ? kIssueRegs : kIssueRegsAlone>();
     // ---------------- products ----------------
-    if (lane == 0) {
+    if (warp == 0 && lane == 0) {
       constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(kTokens >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (uint32_t(DIM >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       auto scores = [&](int m, uint32_t t, bool last) {
@@ -429,19 +449,19 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       };
       bool ok = true;
       uint32_t t = 0, done[2] = {0, 0}, segs[2] = {0, 0};   // tiles; tiles of each half; segments of each half
-      while (ok && next_segment(g)) {
-        const int n = g.tile1 - g.tile0;
+      for (advance(); ok && g.tile1 > g.tile0; advance()) {
+        const int n = g.tile1 - g.tile0, halves = g.halves;
         ok = BarWait(&sh.k_full[t % ST], (t / ST) & 1, quit, a.status_word);
-        for (int m = 0; m < g.halves && ok; ++m) {
+        for (int m = 0; m < halves && ok; ++m) {
           // the half's last weights of the segment before have been read, its next rows of q are there
           ok = (done[m] == 0 || BarWait(&sh.o_done[m], (done[m] - 1) & 1, quit, a.status_word)) && BarWait(&sh.q_full[m], segs[m] & 1, quit, a.status_word);
           if (!ok) break;
           ++segs[m];
           FenceAfter();
-          scores(m, t, m == g.halves - 1);
+          scores(m, t, m == halves - 1);
         }
         for (int j = 0; j < n && ok; ++j, ++t) {
-          for (int m = 0; m < g.halves && ok; ++m) {
+          for (int m = 0; m < halves && ok; ++m) {
             ok = BarWait(&sh.p_full[m], done[m] & 1, quit, a.status_word) && (m > 0 || BarWait(&sh.v_full[t % ST], (t / ST) & 1, quit, a.status_word));
             if (!ok) break;
             FenceAfter();
@@ -451,14 +471,14 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
               MmaTmem(tmem + H::kOColumn + m * DIM, tmem + m * 128 + k * 8, Desc(va + k * 2048, 128 * 128), kIdescO, j > 0 || k > 0);
             Commit(&sh.o_done[m]);
             BarArrive(&sh.o_done[m]);
-            if (m == g.halves - 1) Commit(&sh.v_empty[t % ST]);
+            if (m == halves - 1) Commit(&sh.v_empty[t % ST]);
             if (j + 1 < n) {
               ok = m > 0 || BarWait(&sh.k_full[(t + 1) % ST], ((t + 1) / ST) & 1, quit, a.status_word);
               // P is read from where the next S goes
               ok = ok && BarWait(&sh.o_done[m], done[m] & 1, quit, a.status_word);
               if (!ok) break;
               FenceAfter();
-              scores(m, t + 1, m == g.halves - 1);
+              scores(m, t + 1, m == halves - 1);
             }
             ++done[m];
           }
@@ -468,14 +488,15 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       Commit(&sh.drained);
       BarWait(&sh.drained, 0, nullptr, a.status_word);
     }
-  } else if (warp >= 4 && warp < 4 + 4 * M) {
+  } else if (warp < 4 + 4 * M) {
     // ---------------- softmax ----------------
+    RegistersUp<kSoftmaxRegs>();
     const int m = (warp - 4) >> 2, in_half = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + H::kOColumn + m * DIM;
     uint32_t tile = 0, t4 = 0;   // tiles of this half; all tiles of the block
     bool ok = true;
-    while (ok && next_segment(g)) {
+    while (ok && next_segment()) {
       const int n = g.tile1 - g.tile0;
       if (m >= g.halves) { t4 += n; continue; }
       const int rr = g.u.row0 + m * kRows + in_half;
@@ -486,46 +507,59 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       const int w_row = g.u.row0 + m * kRows + (warp & 3) * 32;
       const int w_first = int(QuickDiv(uint32_t(min(g.u.row1 - 1, w_row)), a.div_share)), w_last = int(QuickDiv(uint32_t(min(g.u.row1, w_row + 32) - 1), a.div_share));
       const int all_begin = RowBegin(a, g.q, max(w_first, w_last)), all_end = RowEnd(a, g.q, min(w_first, w_last));
+      const int some_begin = RowBegin(a, g.q, min(w_first, w_last)), some_end = RowEnd(a, g.q, max(w_first, w_last));   // that one of them sees
       float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
       {
         // ---- the row of q: half, scaled, in the codes' order
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + (g.q.row0 + i) * a.qt + int64_t(h) * a.qh;
         union Piece { uint4 v; uint32_t u[4]; uint16_t e[8]; };
-        auto piece = [&](int p) {
-          Piece x;
-          if (!on) x.v = make_uint4(0, 0, 0, 0);
-          else if (a.q_aligned) x.v = __ldg(reinterpret_cast<const uint4*>(src) + p);
-          else
+        // up to 128 channels at a time in registers, all their loads in flight
+        constexpr int kPieces = DIM / 8, kHeld = kPieces < 16 ? kPieces : 16;
+        Piece x[kHeld];
+        auto fetch = [&](int p0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x.e[e] = src[p * 8 + e];
-          return x;
+          for (int p = 0; p < kHeld; ++p) {
+            if (!on) x[p].v = make_uint4(0, 0, 0, 0);
+            else if (a.q_aligned) x[p].v = __ldg(reinterpret_cast<const uint4*>(src) + p0 + p);
+            else
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[p].e[e] = src[(p0 + p) * 8 + e];
+          }
         };
         float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
         if (s.bf16) {
           float most = 0.f;
-#pragma unroll 4
-          for (int p = 0; p < DIM / 8; ++p) {
-            const Piece x = piece(p);
+#pragma unroll 1
+          for (int p0 = kPieces - kHeld; p0 >= 0; p0 -= kHeld) {   // the first ones last: they stay
+            fetch(p0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x.e[e]) << 16)));
+            for (int p = 0; p < kHeld; ++p)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x[p].e[e]) << 16)));
           }
           const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
           if (most > 0.f && most < INFINITY) {
             down *= __uint_as_float(uint32_t(254 - e) << 23);
             scale = fmaxf(scale * __uint_as_float(uint32_t(e) << 23), 1e-37f);
           }
+        } else {
+          fetch(0);
         }
         uint8_t* const to = s_q + m * (kRows * DIM * 2);
-#pragma unroll 4
-        for (int p = 0; p < DIM / 8; ++p) {
-          Piece x = piece(p);
+#pragma unroll 1
+        for (int p0 = 0; p0 < kPieces; p0 += kHeld) {
+          if (p0 > 0) fetch(p0);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float raw = s.bf16 ? __uint_as_float(uint32_t(x.e[e]) << 16) : __half2float(__ushort_as_half(x.e[e]));
-            x.e[e] = __half_as_ushort(__float2half_rn(raw * down));
+          for (int p = 0; p < kHeld; ++p) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float raw = s.bf16 ? __uint_as_float(uint32_t(x[p].e[e]) << 16) : __half2float(__ushort_as_half(x[p].e[e]));
+              x[p].e[e] = __half_as_ushort(__float2half_rn(raw * down));
+            }
+            const uint32_t* u = x[p].u;
+            *reinterpret_cast<uint4*>(to + PieceAt(in_half, p0 + p)) =
+                make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[1], u[3], 0x7632));
           }
-          *reinterpret_cast<uint4*>(to + PieceAt(in_half, p)) =
-              make_uint4(__byte_perm(x.u[0], x.u[2], 0x5410), __byte_perm(x.u[0], x.u[2], 0x7632), __byte_perm(x.u[1], x.u[3], 0x5410), __byte_perm(x.u[1], x.u[3], 0x7632));
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         BarArrive(&sh.q_full[m]);
@@ -538,47 +572,63 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
         FenceAfter();
         const int j0 = g.u.begin + (g.tile0 + j) * kTokens;
         const uint32_t* there = sh.there[t4 & 3];
-        const bool partial = j0 < all_begin || j0 + kTokens > all_end || (there[0] & there[1] & there[2] & there[3]) != 0xffffffffu;
         // 32 tokens at a time, a short loop that stays in the instruction cache; P's columns 16 c .. are S's columns of
-        // tokens that have been read already
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], p[16];
-          TmemLoad32(s_at + c * 32, v);
-          if (partial) {
+        // tokens that have been read already, the next 32 among them
+        uint32_t buf[2][32];
+        TmemLoadStart(s_at, buf[0]);
+        auto chunk = [&](uint32_t (&v)[32], uint32_t (&ahead)[32], int c) {
+          TmemLoadDone(v);
+          if (c < 3) TmemLoadStart(s_at + c * 32 + 32, ahead);
+          const int t0 = j0 + c * 32;
+          uint32_t p[16];
+          if (t0 >= some_end || t0 + 32 <= some_begin) {   // nothing that a row of this warp sees
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = 0u;
+          } else {
             const uint32_t word = there[c];
-            const int from = lo - (j0 + c * 32), to = hi - (j0 + c * 32);   // visible: from <= e < to
+            if (t0 < all_begin || t0 + 32 > all_end || word != 0xffffffffu) {
+              // bits lo - t0 .. hi - t0 - 1 of the tokens that exist
+              const int from = min(max(lo - t0, 0), 32), to = min(max(hi - t0, 0), 32);
+              const uint32_t seen = word & uint32_t((uint64_t(1) << to) - 1) & ~uint32_t((uint64_t(1) << from) - 1);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (e < from || e >= to || ((word >> e) & 1u) == 0u) v[e] = 0xff800000u;
-          }
-          float part[2];
-          auto weights = [&]() {
-            part[0] = part[1] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float x = Exp2(fmaf(__uint_as_float(v[e]), scale, shift)), y = Exp2(fmaf(__uint_as_float(v[e + 1]), scale, shift));
-              part[0] += x;
-              part[1] += y;
-              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[e / 2]) : "f"(y), "f"(x));
+              for (int e = 0; e < 32; ++e)
+                if ((seen & (1u << e)) == 0u) v[e] = 0xff800000u;
             }
-          };
+            const F2 scale2 = Make2(scale, scale);
 #pragma unroll 1
-          for (;;) {
-            weights();
-            if (!__any_sync(0xffffffffu, part[0] + part[1] > kLimit)) break;
-            // a new maximum for the rows that passed it; what was made with the old one is scaled
-            float top = __uint_as_float(v[0]);
+            for (;;) {
+              const F2 shift2 = Make2(shift, shift);
+              F2 part = Make2(0.f, 0.f);
 #pragma unroll
-            for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
-            const float to = fminf(shift, kUp - top * scale);
-            const float f = Exp2(to - shift);
-            shift = to;
-            total *= f;
-            Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
+              for (int e = 0; e < 32; e += 2) {
+                const F2 d = Fma2(Make2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, shift2);
+                const float x = Exp2(X(d)), y = Exp2(Y(d));
+                part = Add2(part, Make2(x, y));
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[e / 2]) : "f"(y), "f"(x));
+              }
+              const float sum = X(part) + Y(part);
+              if (!__any_sync(0xffffffffu, sum > kLimit)) {
+                total += sum;
+                break;
+              }
+              // a new maximum for the rows that passed it; what was made with the old one is scaled
+              float top = __uint_as_float(v[0]);
+#pragma unroll
+              for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+              const float to = fminf(shift, kUp - top * scale);
+              const float f = Exp2(to - shift);
+              shift = to;
+              total *= f;
+              if (c < 3) TmemLoadDone(ahead);
+              Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
+            }
           }
-          total += part[0] + part[1];
           TmemStore16(s_at + c * 16, p);
+        };
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          chunk(buf[0], buf[1], c);
+          chunk(buf[1], buf[0], c + 1);
         }
         TmemStoreDone();
         FenceBefore();
@@ -629,35 +679,36 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       }
       FenceBefore();
     }
-  } else if (warp >= 12) {
+  } else if (warp < 12) {
+    RegistersDown<M == 2 ? kIssueRegs : kIssueRegsAlone>();
+  } else {
     // ---------------- codes to operands ----------------
+    if (M == 2) RegistersDown<kConvertRegs>();
     const int t = threadIdx.x - 12 * 32, w = warp - 12;
     Row<DIM, GROUP> k, v;
     uint32_t n = 0;      // tiles so far
     bool ok = true;
     // a tile: where this thread's token lies, -1 where there is none
     struct Place { int page, off, kvh; };
-    Segment ahead{};
-    int ahead_tile = 0;
-    bool more = next_segment(ahead);
-    ahead_tile = ahead.tile0;
-    auto place = [&]() {   // of the tile `ahead` stands at, and one on
+    bool more = next_segment();
+    int ahead = g.tile0;
+    auto place = [&]() {   // of the tile that `ahead` stands at, and one on
       Place x{-1, 0, 0};
       if (!more) return x;
-      const int tok = ahead.u.begin + ahead_tile * kTokens + t;
-      x.kvh = ahead.kvh;
-      if (tok >= ahead.u.some_begin && tok < ahead.u.end) {
+      const int tok = g.u.begin + ahead * kTokens + t;
+      x.kvh = g.kvh;
+      if (tok >= g.u.some_begin && tok < g.u.end) {
         const int col = int(QuickDiv(uint32_t(tok), a.c.div_page));
         x.off = tok - col * a.c.page_size;
-        x.page = __ldg(a.table + int64_t(ahead.b) * a.table_stride + col);
+        x.page = __ldg(a.table + int64_t(g.b) * a.table_stride + col);
         if (x.page < 0 || x.page >= a.c.num_pages) {
           ReportIndex(a.status_word);
           x.page = -1;
         }
       }
-      if (++ahead_tile == ahead.tile1) {
-        more = next_segment(ahead);
-        ahead_tile = ahead.tile0;
+      if (++ahead == g.tile1) {
+        more = next_segment();
+        ahead = g.tile0;
       }
       return x;
     };
