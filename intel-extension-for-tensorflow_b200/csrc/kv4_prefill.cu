@@ -4,17 +4,19 @@
 // against the 32 pairs per clock that the two products of head_dim 128 allow.
 //
 // A unit of work is 256 query rows of one key/value head (new tokens times the query heads that share it; 128 rows for
-// head_dim 256) against the tokens they see, in tiles of 128.  One block of 512 threads per SM takes an equal, contiguous part
+// head_dim 256) against the tokens they see, in tiles of 128.  One block of 640 (512) threads per SM takes an equal, contiguous part
 // of the list of all units' tiles; units that several blocks share are joined by a second kernel:
-//   warp 0       issues tcgen05.mma (f16 operands, fp32 accumulators in tensor memory): S = q K^T and O += P V for the two
-//                halves of 128 rows in turn, so that one half's products run under the other half's softmax
-//   warp 1       allocates tensor memory: S of each half (128 columns; P overwrites it as halves), O of each half
+//   warps 0, 1   issue tcgen05.mma (f16 operands, fp32 accumulators in tensor memory) for a half of 128 rows each: S = q K^T
+//                and O += P V, 64 tokens at a time.  A half has two S, so that the next one is there before its softmax asks
+//                for it.  (One warp for both halves spent more time on its waits and instructions than the tensor cores on
+//                the products: 1760 clocks per half and 64 tokens against 640.)
+//                Tensor memory: two S of each half (64 columns; P overwrites it as halves), O of each half
 //   warps 4-11   softmax, a thread per row: weights 2^(s - m + 7) straight from S with the maximum m of earlier tokens; only
 //                when a row's weights of 32 tokens add up to more than 2^15 is the maximum looked for, and what was made with
 //                the old one rescaled.  Weights go back to tensor memory as the second product's A operand
-//   warps 12-15  a thread per token: page lookup, codes and params into registers one tile ahead, values lo + step * code as
-//                halves into shared memory in the layout the tensor cores read (128-byte swizzle; keys K-major, values
-//                MN-major: both are rows of channels)
+//   warps 12-15, 16-19  keys and values, a thread per token: page lookup, codes and params into registers one tile ahead, values
+//                lo + step * code as halves into shared memory in the layout the tensor cores read (128-byte swizzle; keys
+//                K-major, values MN-major: both are rows of channels).
 // Halves hold a value to 2^-12 of itself; q enters scaled by a power of two per row (see kv4_steps.cu).  The order of
 // channels is the codes' in a word, for q, keys and the output alike.
 // Rows of the cache that no query may see are zeros here; a value group stored as NaN is zeros too and makes the rows that see
@@ -26,8 +28,8 @@
 namespace itexb {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kTokens = 128;                 // per tile
+constexpr int kTokens = 128;                 // per tile,
+constexpr int kPart = 64;                    // and per product: half a tile
 constexpr int kRows = 128;                   // per half: lanes of tensor memory
 constexpr float kUp = 7.f;                   // weights are 2^(score - maximum + 7),
 constexpr float kLimit = 32768.f;            // and their sum over 32 tokens at most 2^15, so that none overflows a half
@@ -37,9 +39,13 @@ constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 template <int DIM> struct Shape {
   static constexpr int kHalves = DIM == 256 ? 1 : 2;       // of 128 rows
   static constexpr int kStages = DIM == 256 ? 1 : 2;       // tiles of keys, and of values
+  // groups of four warps: issue, softmax of each half, keys, values
+  static constexpr int kThreads = (3 + kHalves) * 128;
+  // registers per thread of these groups; their sum is at most what the launch gives (a multiple of 8 up to 65536 / kThreads)
+  static constexpr int kIssueRegs = DIM == 256 ? 80 : 56, kSoftmaxRegs = DIM == 256 ? 176 : 152, kConvertRegs = DIM == 256 ? 128 : 56;
   static constexpr int kQBytes = kHalves * kRows * DIM * 2, kTileBytes = kTokens * DIM * 2;
   static constexpr int kSmem = kQBytes + 2 * kStages * kTileBytes;
-  static constexpr int kOColumn = kHalves * 128;           // of the first half's O; S of half m starts at column 128 m
+  static constexpr int kOColumn = kHalves * 128;           // of the first half's O; S `u` of half m starts at column 128 m + 64 u
 };
 
 __device__ __forceinline__ uint32_t SmemAt(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -71,22 +77,28 @@ __device__ __forceinline__ void FenceAfter() { asm volatile("tcgen05.fence::afte
 __device__ __forceinline__ void Commit(uint64_t* b) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(SmemAt(b)) : "memory");
 }
-__device__ __forceinline__ void MmaSmem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// Operand descriptors: rows of 128 bytes in groups of eight, 1024 bytes apart, 128-byte swizzle.  The low word holds the
+// address and `lead`, the bytes between blocks of 64 channels where channels are the operand's outer dimension (values); the high
+// word is a constant.  `off`: bytes from `low`'s address on.
+__device__ __forceinline__ uint32_t DescLow(uint32_t at, uint32_t lead) { return ((at & 0x3ffffu) >> 4) | ((lead >> 4) << 16); }
+constexpr uint32_t kDescHigh = uint32_t(1024 >> 4) | (1u << 14) | (2u << 29);
+template <bool ADD> __device__ __forceinline__ void MmaSmem(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)), "r"(0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "n"(kDescHigh), "n"(int(ADD))
       : "memory");
 }
-__device__ __forceinline__ void MmaTmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+template <bool ADD> __device__ __forceinline__ void MmaTmem(uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)), "r"(0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b_low), "r"(idesc), "n"(kDescHigh), "n"(int(ADD))
       : "memory");
 }
-// Rows of 128 bytes in groups of eight, 1024 bytes apart, 128-byte swizzle.  `lead`: bytes between blocks of 64 channels where
-// channels are the operand's outer dimension (values).
-__device__ __forceinline__ uint64_t Desc(uint32_t at, uint32_t lead) {
-  return uint64_t((at & 0x3ffffu) >> 4) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// One lane of a converged warp; the code around it stays uniform, so that operands live in uniform registers.
+__device__ __forceinline__ bool ElectOne() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 // A load of 32 columns in two steps; the registers are in the second's operands so that no use moves above it.
 __device__ __forceinline__ void TmemLoadStart(uint32_t at, uint32_t (&v)[32]) {
@@ -246,7 +258,6 @@ struct PrefillArgs {
   Head* heads;             // [blocks]
 };
 constexpr int kMaxBlocks = 148;
-constexpr int kIssueRegs = 56, kSoftmaxRegs = 176, kConvertRegs = 104, kIssueRegsAlone = 80;
 constexpr int kLeastTiles = 2;    // of a block's part, where there is little work
 
 // A unit of work: M * 128 query rows of a sequence and key/value head.  The list of units runs over sequences, their row tiles
@@ -271,21 +282,21 @@ struct Segment { Seq q; Unit u; int b, kvh, tile0, tile1, halves; };
 struct Walker { int64_t left; int b, rt, kvh, tile; bool fresh; };   // what lies behind it
 
 struct Shared {   // behind the operand tiles
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], drained;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], drained[2];
   uint32_t tmem;
   volatile int quit;
   int nan_values;          // some value group is stored as NaN
   uint32_t there[4][4];    // of the last four tiles: tokens that exist, 32 per word
-  int64_t sums[kThreads / 32], left;
+  int64_t sums[20], left;
   int b, rt, kvh, tile;    // where this block's part begins
-  Walker walk[kThreads / 32];
-  Segment seg[kThreads / 32];
+  Walker walk[20];
+  Segment seg[20];
 };
 
 template <int DIM, int GROUP>
-__global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_constant__ PrefillArgs s) {
+__global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const __grid_constant__ PrefillArgs s) {
   using H = Shape<DIM>;
-  constexpr int M = H::kHalves, ST = H::kStages, NG = DIM / GROUP, ROWS = M * kRows;
+  constexpr int M = H::kHalves, ST = H::kStages, NG = DIM / GROUP, ROWS = M * kRows, kThreads = H::kThreads;
   const AttnArgs& a = s.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* const s_q = smem;
@@ -360,14 +371,16 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
     for (int i = 0; i < 2; ++i) {
       BarInit(&sh.q_full[i], kRows);
       BarInit(&sh.k_full[i], 128);
-      BarInit(&sh.k_empty[i], 1);
+      BarInit(&sh.k_empty[i], M);
       BarInit(&sh.v_full[i], 128);
-      BarInit(&sh.v_empty[i], 1);
-      BarInit(&sh.s_full[i], 2);      // the products' completion, and the issuer itself (for what it has seen others write)
-      BarInit(&sh.p_full[i], kRows);
-      BarInit(&sh.o_done[i], 2);
+      BarInit(&sh.v_empty[i], M);
+      BarInit(&sh.drained[i], 1);
+      for (int u = 0; u < 2; ++u) {
+        BarInit(&sh.s_full[i][u], 2);      // the products' completion, and the issuer itself (for what it has seen others write)
+        BarInit(&sh.p_full[i][u], kRows);
+        BarInit(&sh.o_done[i][u], 2);
+      }
     }
-    BarInit(&sh.drained, 1);
     sh.quit = 0;
     sh.nan_values = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -427,74 +440,96 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
     return g.tile1 > g.tile0;
   };
 
-  // Registers go from the warps that issue and convert to the softmax warps.  Per thread, by groups of four warps, of the
-  // launch's 4 x 128: 56, 176, 176, 104 (head_dim 256, where the third group has no work: 80, 176, 80, 128).
-  // Each role's branch states its own, so that its code is compiled for it.
+  // Registers go from the warps that issue and convert to the softmax warps; each role's branch states its own, so that its
+  // code is compiled for it.
   if (warp < 4) {
-    RegistersDown<M == 2 ? kIssueRegs : kIssueRegsAlone>();
-    // ---------------- products ----------------
-    if (warp == 0 && lane == 0) {
-      constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(kTokens >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+    RegistersDown<H::kIssueRegs>();
+    // ---------------- products: a warp for each half ----------------
+    // The whole warp walks the loop, one lane issues.
+    if (warp < M) {
+      constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(kPart >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (uint32_t(DIM >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
-      auto scores = [&](int m, uint32_t t, bool last) {
-        const uint32_t qa = SmemAt(s_q) + m * (kRows * DIM * 2), ka = SmemAt(s_k) + (t % ST) * H::kTileBytes;
-#pragma unroll
-        for (int k = 0; k < DIM / 16; ++k) {
-          const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-          MmaSmem(tmem + m * 128, Desc(qa + off, 16), Desc(ka + off, 16), kIdescS, k > 0);
-        }
-        Commit(&sh.s_full[m]);
-        BarArrive(&sh.s_full[m]);
-        if (last) Commit(&sh.k_empty[t % ST]);
-      };
+      const int m = __shfl_sync(0xffffffffu, warp, 0);
+      const uint32_t s_d = __shfl_sync(0xffffffffu, tmem, 0) + m * 128, o_d = s_d + H::kOColumn + m * (DIM - 128);
+      const uint32_t q_low = DescLow(SmemAt(s_q), 16) + m * (kRows * DIM * 2 / 16), k_low = DescLow(SmemAt(s_k), 16), v_low = DescLow(SmemAt(s_v), 128 * 128);
+      uint32_t t = 0;            // tiles of the block
+      uint32_t parts = 0;        // half tiles of this half whose weights have been multiplied; even between tiles
+      uint32_t segs = 0;
       bool ok = true;
-      uint32_t t = 0, done[2] = {0, 0}, segs[2] = {0, 0};   // tiles; tiles of each half; segments of each half
-      for (advance(); ok && g.tile1 > g.tile0; advance()) {
-        const int n = g.tile1 - g.tile0, halves = g.halves;
-        ok = BarWait(&sh.k_full[t % ST], (t / ST) & 1, quit, a.status_word);
-        for (int m = 0; m < halves && ok; ++m) {
-          // the half's last weights of the segment before have been read, its next rows of q are there
-          ok = (done[m] == 0 || BarWait(&sh.o_done[m], (done[m] - 1) & 1, quit, a.status_word)) && BarWait(&sh.q_full[m], segs[m] & 1, quit, a.status_word);
-          if (!ok) break;
-          ++segs[m];
-          FenceAfter();
-          scores(m, t, m == halves - 1);
-        }
-        for (int j = 0; j < n && ok; ++j, ++t) {
-          for (int m = 0; m < halves && ok; ++m) {
-            ok = BarWait(&sh.p_full[m], done[m] & 1, quit, a.status_word) && (m > 0 || BarWait(&sh.v_full[t % ST], (t / ST) & 1, quit, a.status_word));
-            if (!ok) break;
-            FenceAfter();
-            const uint32_t va = SmemAt(s_v) + (t % ST) * H::kTileBytes;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = __all_sync(0xffffffffu, ok && BarWait(bar, parity & 1, quit, a.status_word)); };
+      // S of half tile u of tile `tile`
+      auto scores = [&](uint32_t tile, int u) {
+        FenceAfter();
+        if (ElectOne()) {
+          const uint32_t ka = k_low + (tile % ST) * (H::kTileBytes / 16) + u * (kPart * 128 / 16), d = s_d + u * kPart;
+          MmaSmem<false>(d, q_low, ka, kIdescS);
 #pragma unroll
-            for (int k = 0; k < kTokens / 16; ++k)
-              MmaTmem(tmem + H::kOColumn + m * DIM, tmem + m * 128 + k * 8, Desc(va + k * 2048, 128 * 128), kIdescO, j > 0 || k > 0);
-            Commit(&sh.o_done[m]);
-            BarArrive(&sh.o_done[m]);
-            if (m == halves - 1) Commit(&sh.v_empty[t % ST]);
-            if (j + 1 < n) {
-              ok = m > 0 || BarWait(&sh.k_full[(t + 1) % ST], ((t + 1) / ST) & 1, quit, a.status_word);
-              // P is read from where the next S goes
-              ok = ok && BarWait(&sh.o_done[m], done[m] & 1, quit, a.status_word);
-              if (!ok) break;
-              FenceAfter();
-              scores(m, t + 1, m == halves - 1);
-            }
-            ++done[m];
+          for (int k = 1; k < DIM / 16; ++k) {
+            constexpr int kBlock = 128 * 128 / 16;
+            MmaSmem<true>(d, q_low + (k / 4) * kBlock + (k % 4) * 2, ka + (k / 4) * kBlock + (k % 4) * 2, kIdescS);
           }
+          Commit(&sh.s_full[m][u]);
+          BarArrive(&sh.s_full[m][u]);
+          if (u == 1) Commit(&sh.k_empty[tile % ST]);
+        }
+        __syncwarp();
+      };
+      while (ok && next_segment()) {
+        const int n = __shfl_sync(0xffffffffu, 2 * (g.tile1 - g.tile0), 0), halves = __shfl_sync(0xffffffffu, g.halves, 0);
+        if (m >= halves) {
+          // no rows here: the tiles are let through one by one, since a barrier's parity tells only neighbouring phases apart
+          for (int j = 0; j < n / 2 && ok; ++j, ++t) {
+            if (!wait(&sh.k_full[t % ST], t / ST)) break;
+            if (ElectOne()) BarArrive(&sh.k_empty[t % ST]);
+            if (!wait(&sh.v_full[t % ST], t / ST)) break;
+            if (ElectOne()) BarArrive(&sh.v_empty[t % ST]);
+            __syncwarp();
+          }
+          continue;
+        }
+        // the half's last weights of the segment before have been multiplied, its next rows of q are there
+        if (parts > 0) wait(&sh.o_done[m][1], (parts - 1) >> 1);
+        wait(&sh.q_full[m], segs++);
+        if (!wait(&sh.k_full[t % ST], t / ST)) break;
+        scores(t, 0);
+        for (int j = 0; j < n; ++j, ++parts) {
+          const int u = j & 1;
+          if (j + 1 < n) {
+            // S of the half tile after this one goes where the weights of the one before it were
+            if (u == 1) wait(&sh.k_full[(t + 1) % ST], (t + 1) / ST);
+            if (j > 0) wait(&sh.o_done[m][u ^ 1], (parts - 1) >> 1);
+            if (!ok) break;
+            scores(t + u, u ^ 1);
+          }
+          if (u == 0) wait(&sh.v_full[t % ST], t / ST);
+          if (!wait(&sh.p_full[m][u], parts >> 1)) break;
+          FenceAfter();
+          if (ElectOne()) {
+            const uint32_t va = v_low + (t % ST) * (H::kTileBytes / 16) + u * (kPart * 128 / 16), p = s_d + u * kPart;
+            if (j > 0) MmaTmem<true>(o_d, p, va, kIdescO);
+            else MmaTmem<false>(o_d, p, va, kIdescO);
+#pragma unroll
+            for (int k = 1; k < kPart / 16; ++k) MmaTmem<true>(o_d, p + k * 8, va + k * 128, kIdescO);
+            Commit(&sh.o_done[m][u]);
+            BarArrive(&sh.o_done[m][u]);
+            if (u == 1) Commit(&sh.v_empty[t % ST]);
+          }
+          __syncwarp();
+          t += u;
         }
       }
       // nothing in flight when tensor memory is given back
-      Commit(&sh.drained);
-      BarWait(&sh.drained, 0, nullptr, a.status_word);
+      if (ElectOne()) Commit(&sh.drained[m]);
+      __syncwarp();
+      BarWait(&sh.drained[m], 0, nullptr, a.status_word);
     }
   } else if (warp < 4 + 4 * M) {
     // ---------------- softmax ----------------
-    RegistersUp<kSoftmaxRegs>();
+    RegistersUp<H::kSoftmaxRegs>();
     const int m = (warp - 4) >> 2, in_half = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + H::kOColumn + m * DIM;
-    uint32_t tile = 0, t4 = 0;   // tiles of this half; all tiles of the block
+    const uint32_t s_m = tmem + lanes + m * 128, o_at = tmem + lanes + H::kOColumn + m * DIM;
+    uint32_t parts = 0, t4 = 0;   // half tiles of this half; all tiles of the block
     bool ok = true;
     while (ok && next_segment()) {
       const int n = g.tile1 - g.tile0;
@@ -565,20 +600,22 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
         BarArrive(&sh.q_full[m]);
       }
       float shift = kNone, total = 0.f;       // weights are 2^(score * scale + shift)
-      for (int j = 0; j < n && ok; ++j, ++tile, ++t4) {
-        ok = BarWait(&sh.s_full[m], tile & 1, quit, a.status_word);
+      for (int j = 0; j < 2 * n && ok; ++j, ++parts) {
+        const int u = j & 1;
+        ok = BarWait(&sh.s_full[m][u], (parts >> 1) & 1, quit, a.status_word);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         FenceAfter();
-        const int j0 = g.u.begin + (g.tile0 + j) * kTokens;
-        const uint32_t* there = sh.there[t4 & 3];
+        const int j0 = g.u.begin + g.tile0 * kTokens + j * kPart;
+        const uint32_t* there = sh.there[t4 & 3] + 2 * u;
+        const uint32_t s_at = s_m + u * kPart;
         // 32 tokens at a time, a short loop that stays in the instruction cache; P's columns 16 c .. are S's columns of
         // tokens that have been read already, the next 32 among them
         uint32_t buf[2][32];
         TmemLoadStart(s_at, buf[0]);
         auto chunk = [&](uint32_t (&v)[32], uint32_t (&ahead)[32], int c) {
           TmemLoadDone(v);
-          if (c < 3) TmemLoadStart(s_at + c * 32 + 32, ahead);
+          if (c == 0) TmemLoadStart(s_at + 32, ahead);
           const int t0 = j0 + c * 32;
           uint32_t p[16];
           if (t0 >= some_end || t0 + 32 <= some_begin) {   // nothing that a row of this warp sees
@@ -619,22 +656,26 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
               const float f = Exp2(to - shift);
               shift = to;
               total *= f;
-              if (c < 3) TmemLoadDone(ahead);
+              if (c == 0) TmemLoadDone(ahead);
+              // the accumulator is free to be changed once the half tile before has been added to it
+              if (j > 0) {
+                ok = ok && BarWait(&sh.o_done[m][u ^ 1], ((parts - 1) >> 1) & 1, quit, a.status_word);
+                __syncwarp();
+                FenceAfter();
+              }
               Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
             }
           }
           TmemStore16(s_at + c * 16, p);
         };
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          chunk(buf[0], buf[1], c);
-          chunk(buf[1], buf[0], c + 1);
-        }
+        chunk(buf[0], buf[1], 0);
+        chunk(buf[1], buf[0], 1);
         TmemStoreDone();
         FenceBefore();
-        BarArrive(&sh.p_full[m]);
+        BarArrive(&sh.p_full[m][u]);
+        t4 += u;
       }
-      if (ok) ok = __all_sync(0xffffffffu, BarWait(&sh.o_done[m], (tile - 1) & 1, quit, a.status_word));
+      ok = __all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, BarWait(&sh.o_done[m][1], ((parts - 1) >> 1) & 1, quit, a.status_word));
       if (!ok) break;
       FenceAfter();
       uint32_t nan_groups = 0;
@@ -679,14 +720,17 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       }
       FenceBefore();
     }
-  } else if (warp < 12) {
-    RegistersDown<M == 2 ? kIssueRegs : kIssueRegsAlone>();
   } else {
-    // ---------------- codes to operands ----------------
-    if (M == 2) RegistersDown<kConvertRegs>();
-    const int t = threadIdx.x - 12 * 32, w = warp - 12;
-    Row<DIM, GROUP> k, v;
-    uint32_t n = 0;      // tiles so far
+    // ---------------- codes to operands: one group of warps for the keys, one for the values ----------------
+    if (H::kConvertRegs < 128) RegistersDown<H::kConvertRegs>();
+    const bool values = warp >= 8 + 4 * M;
+    const int t = threadIdx.x & 127, w = warp & 3;
+    const uint8_t* const codes = values ? a.c.v_codes : a.c.k_codes;
+    const __half2* const params = values ? a.c.v_params : a.c.k_params;
+    uint8_t* const tiles = values ? s_v : s_k;
+    uint64_t* const full = values ? sh.v_full : sh.k_full;
+    uint64_t* const empty = values ? sh.v_empty : sh.k_empty;
+    Row<DIM, GROUP> row;
     bool ok = true;
     // a tile: where this thread's token lies, -1 where there is none
     struct Place { int page, off, kvh; };
@@ -712,35 +756,32 @@ __global__ void __launch_bounds__(kThreads, 1) PrefillKernel(const __grid_consta
       }
       return x;
     };
-    auto load = [&](Row<DIM, GROUP>& r, const uint8_t* codes, const __half2* params, const Place& x) {
-      if (x.page < 0) { r.Clear(); return; }
-      r.Load(codes + int64_t(x.page) * a.c.cp + int64_t(x.kvh) * a.c.ch + int64_t(x.off) * a.c.ct,
-             params + int64_t(x.page) * a.c.pp + int64_t(x.kvh) * a.c.ph + int64_t(x.off) * a.c.pt);
+    auto load = [&](const Place& x) {
+      if (x.page < 0) { row.Clear(); return; }
+      row.Load(codes + int64_t(x.page) * a.c.cp + int64_t(x.kvh) * a.c.ch + int64_t(x.off) * a.c.ct,
+               params + int64_t(x.page) * a.c.pp + int64_t(x.kvh) * a.c.ph + int64_t(x.off) * a.c.pt);
     };
     Place now = place(), next = place();
-    load(k, a.c.k_codes, a.c.k_params, now);
-    load(v, a.c.v_codes, a.c.v_params, now);
-    for (int64_t j = 0; j < part && ok; ++j, ++n) {
+    load(now);
+    uint32_t n = 0;      // tiles so far
+    for (int64_t j = 0; j < part; ++j, ++n) {
       const Place after = place();
-      if (n >= uint32_t(ST)) ok = BarWait(&sh.k_empty[n % ST], (n / ST - 1) & 1, quit, a.status_word);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      k.Store(s_k + (n % ST) * H::kTileBytes, t);
-      const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
-      if (lane == 0) sh.there[n & 3][w] = there;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      BarArrive(&sh.k_full[n % ST]);
-      load(k, a.c.k_codes, a.c.k_params, next);
-      if (n >= uint32_t(ST)) ok = BarWait(&sh.v_empty[n % ST], (n / ST - 1) & 1, quit, a.status_word);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      bool bad = false;
+      if (n >= uint32_t(ST)) ok = BarWait(&empty[n % ST], (n / ST - 1) & 1, quit, a.status_word);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (values) {
+        bool bad = false;
 #pragma unroll
-      for (int x = 0; x < NG; ++x)
-        if (NotFinite(v.params[x])) { v.params[x] = 0; bad = true; }
-      if (bad) sh.nan_values = 1;
-      v.Store(s_v + (n % ST) * H::kTileBytes, t);
+        for (int x = 0; x < NG; ++x)
+          if (NotFinite(row.params[x])) { row.params[x] = 0; bad = true; }
+        if (bad) sh.nan_values = 1;
+      } else {
+        const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
+        if (lane == 0) sh.there[n & 3][w] = there;
+      }
+      row.Store(tiles + (n % ST) * H::kTileBytes, t);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      BarArrive(&sh.v_full[n % ST]);
-      load(v, a.c.v_codes, a.c.v_params, next);
+      BarArrive(&full[n % ST]);
+      load(next);
       now = next;
       next = after;
     }
@@ -807,7 +848,7 @@ template <int DIM, int GROUP> int LaunchGroup(PrefillArgs& s, cudaStream_t st) {
   const int64_t most = (span / kTokens + 2) * s.a.num_seqs * s.row_tiles * s.a.c.kv_heads;   // tiles
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(std::min<int64_t>(std::min(kMaxBlocks, SmCount()), std::max<int64_t>(1, most / kLeastTiles))));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(H::kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
