@@ -542,7 +542,6 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
       const int w_row = g.u.row0 + m * kRows + (warp & 3) * 32;
       const int w_first = int(QuickDiv(uint32_t(min(g.u.row1 - 1, w_row)), a.div_share)), w_last = int(QuickDiv(uint32_t(min(g.u.row1, w_row + 32) - 1), a.div_share));
       const int all_begin = RowBegin(a, g.q, max(w_first, w_last)), all_end = RowEnd(a, g.q, min(w_first, w_last));
-      const int some_begin = RowBegin(a, g.q, min(w_first, w_last)), some_end = RowEnd(a, g.q, max(w_first, w_last));   // that one of them sees
       float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
       {
         // ---- the row of q: half, scaled, in the codes' order
@@ -610,66 +609,61 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         const uint32_t* there = sh.there[t4 & 3] + 2 * u;
         const uint32_t s_at = s_m + u * kPart;
         // 32 tokens at a time, a short loop that stays in the instruction cache; P's columns 16 c .. are S's columns of
-        // tokens that have been read already, the next 32 among them
-        uint32_t buf[2][32];
-        TmemLoadStart(s_at, buf[0]);
-        auto chunk = [&](uint32_t (&v)[32], uint32_t (&ahead)[32], int c) {
-          TmemLoadDone(v);
-          if (c == 0) TmemLoadStart(s_at + 32, ahead);
-          const int t0 = j0 + c * 32;
-          uint32_t p[16];
-          if (t0 >= some_end || t0 + 32 <= some_begin) {   // nothing that a row of this warp sees
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = 0u;
-          } else {
-            const uint32_t word = there[c];
-            if (t0 < all_begin || t0 + 32 > all_end || word != 0xffffffffu) {
-              // bits lo - t0 .. hi - t0 - 1 of the tokens that exist
-              const int from = min(max(lo - t0, 0), 32), to = min(max(hi - t0, 0), 32);
-              const uint32_t seen = word & uint32_t((uint64_t(1) << to) - 1) & ~uint32_t((uint64_t(1) << from) - 1);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if ((seen & (1u << e)) == 0u) v[e] = 0xff800000u;
-            }
-            const F2 scale2 = Make2(scale, scale);
+        // tokens that have been read already
+        const F2 scale2 = Make2(scale, scale);
+        uint32_t v[32], p[16];
 #pragma unroll 1
-            for (;;) {
-              const F2 shift2 = Make2(shift, shift);
-              F2 part = Make2(0.f, 0.f);
+        for (int c = 0; c < 2;) {
+          TmemLoad32(s_at + c * 32, v);
+          const int t0 = j0 + c * 32;
+          const uint32_t word = there[c];
+          if (t0 < all_begin || t0 + 32 > all_end || word != 0xffffffffu) {
+            // bits lo - t0 .. hi - t0 - 1 of the tokens that exist
+            const int from = min(max(lo - t0, 0), 32), to = min(max(hi - t0, 0), 32);
+            const uint32_t seen = word & uint32_t((uint64_t(1) << to) - 1) & ~uint32_t((uint64_t(1) << from) - 1);
+            if (__all_sync(0xffffffffu, seen == 0u)) {   // nothing that a row of this warp sees
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const F2 d = Fma2(Make2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, shift2);
-                const float x = Exp2(X(d)), y = Exp2(Y(d));
-                part = Add2(part, Make2(x, y));
-                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[e / 2]) : "f"(y), "f"(x));
-              }
-              const float sum = X(part) + Y(part);
-              if (!__any_sync(0xffffffffu, sum > kLimit)) {
-                total += sum;
-                break;
-              }
-              // a new maximum for the rows that passed it; what was made with the old one is scaled
-              float top = __uint_as_float(v[0]);
-#pragma unroll
-              for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
-              const float to = fminf(shift, kUp - top * scale);
-              const float f = Exp2(to - shift);
-              shift = to;
-              total *= f;
-              if (c == 0) TmemLoadDone(ahead);
-              // the accumulator is free to be changed once the half tile before has been added to it
-              if (j > 0) {
-                ok = ok && BarWait(&sh.o_done[m][u ^ 1], ((parts - 1) >> 1) & 1, quit, a.status_word);
-                __syncwarp();
-                FenceAfter();
-              }
-              Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
+              for (int e = 0; e < 16; ++e) p[e] = 0u;
+              TmemStore16(s_at + c * 16, p);
+              ++c;
+              continue;
             }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if ((seen & (1u << e)) == 0u) v[e] = 0xff800000u;
           }
-          TmemStore16(s_at + c * 16, p);
-        };
-        chunk(buf[0], buf[1], 0);
-        chunk(buf[1], buf[0], 1);
+          const F2 shift2 = Make2(shift, shift);
+          F2 part[2] = {Make2(0.f, 0.f), Make2(0.f, 0.f)};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const F2 d = Fma2(Make2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, shift2);
+            const float x = Exp2(X(d)), y = Exp2(Y(d));
+            part[(e >> 1) & 1] = Add2(part[(e >> 1) & 1], Make2(x, y));
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[e / 2]) : "f"(y), "f"(x));
+          }
+          const F2 both = Add2(part[0], part[1]);
+          const float sum = X(both) + Y(both);
+          if (!__any_sync(0xffffffffu, sum > kLimit)) {
+            total += sum;
+            TmemStore16(s_at + c * 16, p);
+            ++c;
+            continue;
+          }
+          // a new maximum for the rows that passed it; what was made with the old one is scaled, these tokens are done again
+          float top = __uint_as_float(v[0]);
+#pragma unroll
+          for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+          const float to = fminf(shift, kUp - top * scale);
+          const float f = Exp2(to - shift);
+          shift = to;
+          total *= f;
+          if (j > 0) {   // the accumulator is free to be changed once the half tile before has been added to it
+            ok = ok && BarWait(&sh.o_done[m][u ^ 1], ((parts - 1) >> 1) & 1, quit, a.status_word);
+            __syncwarp();
+            FenceAfter();
+          }
+          Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
+        }
         TmemStoreDone();
         FenceBefore();
         BarArrive(&sh.p_full[m][u]);
