@@ -12,8 +12,8 @@
 //                the products: 1760 clocks per half and 64 tokens against 640.)
 //                Tensor memory: two S of each half (64 columns; P overwrites it as halves), O of each half
 //   warps 4-11   softmax, a thread per row: weights 2^(s - m + 7) straight from S with the maximum m of earlier tokens; only
-//                when a row's weights of 32 tokens add up to more than 2^15 is the maximum looked for, and what was made with
-//                the old one rescaled.  Weights go back to tensor memory as the second product's A operand
+//                when a row's weights of 64 tokens add up to more than 2^15 is the maximum looked for, the accumulator rescaled
+//                and the 64 tokens done again.  Weights go back to tensor memory as the second product's A operand.
 //   warps 12-15, 16-19  keys and values, a thread per token: page lookup, codes and params into registers one tile ahead, values
 //                lo + step * code as halves into shared memory in the layout the tensor cores read (128-byte swizzle; keys
 //                K-major, values MN-major: both are rows of channels).
@@ -32,7 +32,7 @@ constexpr int kTokens = 128;                 // per tile,
 constexpr int kPart = 64;                    // and per product: half a tile
 constexpr int kRows = 128;                   // per half: lanes of tensor memory
 constexpr float kUp = 7.f;                   // weights are 2^(score - maximum + 7),
-constexpr float kLimit = 32768.f;            // and their sum over 32 tokens at most 2^15, so that none overflows a half
+constexpr float kLimit = 32768.f;            // and their sum over 64 tokens at most 2^15, so that none overflows a half
 constexpr float kNone = 3.0e38f;             // -maximum + 7 of no scores
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 
@@ -100,26 +100,40 @@ __device__ __forceinline__ bool ElectOne() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
 }
-// A load of 32 columns in two steps; the registers are in the second's operands so that no use moves above it.
-__device__ __forceinline__ void TmemLoadStart(uint32_t at, uint32_t (&v)[32]) {
+// Load and wait in one statement: as two, every register was copied between them.
+__device__ __forceinline__ void TmemLoad32(uint32_t at, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
         "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
         "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(at));
+      : "r"(at)
+      : "memory");
 }
-__device__ __forceinline__ void TmemLoadDone(uint32_t (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                 "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
-                 "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
-                 "+r"(v[31])::"memory");
+__device__ __forceinline__ void TmemLoad64(uint32_t at, uint32_t (&v)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), 
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), 
+        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), 
+        "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), 
+        "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]), 
+        "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), 
+        "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+      : "r"(at)
+      : "memory");
 }
-__device__ __forceinline__ void TmemLoad32(uint32_t at, uint32_t (&v)[32]) {
-  TmemLoadStart(at, v);
-  TmemLoadDone(v);
+__device__ __forceinline__ void TmemStore32(uint32_t at, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), 
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), 
+      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
 }
 __device__ __forceinline__ void TmemStore16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -127,41 +141,26 @@ __device__ __forceinline__ void TmemStore16(uint32_t at, const uint32_t (&v)[16]
                : "memory");
 }
 __device__ __forceinline__ void TmemLoad16(uint32_t at, uint32_t (&v)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
                  "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-               : "r"(at));
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
+               : "r"(at)
+               : "memory");
 }
 __device__ __forceinline__ void TmemStoreDone() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int N> __device__ __forceinline__ void RegistersDown() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void RegistersUp() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// A row's accumulator (o_at 0: there is none yet) and the first `chunks` blocks of 16 columns of its weights times f.
-template <int DIM> __device__ __forceinline__ void Rescale(uint32_t o_at, uint32_t p_at, int chunks, float f) {
-  uint32_t v[16];
-  if (o_at != 0u) {
+// A row's accumulator times f.
+template <int DIM> __device__ __forceinline__ void Rescale(uint32_t o_at, float f) {
 #pragma unroll 1
-    for (int c = 0; c < DIM / 16; ++c) {
-      TmemLoad16(o_at + c * 16, v);
+  for (int c = 0; c < DIM / 16; ++c) {
+    uint32_t v[16];
+    TmemLoad16(o_at + c * 16, v);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-      TmemStore16(o_at + c * 16, v);
-    }
-  }
-  TmemStoreDone();
-#pragma unroll 1
-  for (int c = 0; c < chunks; ++c) {
-    TmemLoad16(p_at + c * 16, v);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
-      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v[e]) : "f"(x.y * f), "f"(x.x * f));
-    }
-    TmemStore16(p_at + c * 16, v);
+    for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+    TmemStore16(o_at + c * 16, v);
   }
   TmemStoreDone();
 }
@@ -608,62 +607,63 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         const int j0 = g.u.begin + g.tile0 * kTokens + j * kPart;
         const uint32_t* there = sh.there[t4 & 3] + 2 * u;
         const uint32_t s_at = s_m + u * kPart;
-        // 32 tokens at a time, a short loop that stays in the instruction cache; P's columns 16 c .. are S's columns of
-        // tokens that have been read already
         const F2 scale2 = Make2(scale, scale);
-        uint32_t v[32], p[16];
+        // of the half tile's tokens, those that exist and that this row sees; all of them in most half tiles
+        uint64_t seen = uint64_t(there[0]) | (uint64_t(there[1]) << 32);
+        const bool masked = j0 < all_begin || j0 + kPart > all_end || seen != ~uint64_t(0);
+        if (masked) {
+          const int from = min(max(lo - j0, 0), 64), to = min(max(hi - j0, 0), 64);
+          seen &= (to == 64 ? ~uint64_t(0) : (uint64_t(1) << to) - 1) & ~(from == 64 ? ~uint64_t(0) : (uint64_t(1) << from) - 1);
+        }
+        uint32_t p[32];
 #pragma unroll 1
-        for (int c = 0; c < 2;) {
-          TmemLoad32(s_at + c * 32, v);
-          const int t0 = j0 + c * 32;
-          const uint32_t word = there[c];
-          if (t0 < all_begin || t0 + 32 > all_end || word != 0xffffffffu) {
-            // bits lo - t0 .. hi - t0 - 1 of the tokens that exist
-            const int from = min(max(lo - t0, 0), 32), to = min(max(hi - t0, 0), 32);
-            const uint32_t seen = word & uint32_t((uint64_t(1) << to) - 1) & ~uint32_t((uint64_t(1) << from) - 1);
-            if (__all_sync(0xffffffffu, seen == 0u)) {   // nothing that a row of this warp sees
+        for (;;) {
+          // P overwrites S only once its weights are known to be good
+          uint32_t v[64];
+          TmemLoad64(s_at, v);
+          if (masked) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) p[e] = 0u;
-              TmemStore16(s_at + c * 16, p);
-              ++c;
-              continue;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if ((seen & (1u << e)) == 0u) v[e] = 0xff800000u;
+            for (int e = 0; e < 64; ++e)
+              if ((uint32_t(seen >> (e & 32)) & (1u << (e & 31))) == 0u) v[e] = 0xff800000u;
           }
           const F2 shift2 = Make2(shift, shift);
-          F2 part[2] = {Make2(0.f, 0.f), Make2(0.f, 0.f)};
+          F2 part[4] = {Make2(0.f, 0.f), Make2(0.f, 0.f), Make2(0.f, 0.f), Make2(0.f, 0.f)};
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < 64; e += 2) {
             const F2 d = Fma2(Make2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, shift2);
             const float x = Exp2(X(d)), y = Exp2(Y(d));
-            part[(e >> 1) & 1] = Add2(part[(e >> 1) & 1], Make2(x, y));
+            part[(e >> 1) & 3] = Add2(part[(e >> 1) & 3], Make2(x, y));
             asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[e / 2]) : "f"(y), "f"(x));
           }
-          const F2 both = Add2(part[0], part[1]);
-          const float sum = X(both) + Y(both);
+          const F2 all = Add2(Add2(part[0], part[1]), Add2(part[2], part[3]));
+          const float sum = X(all) + Y(all);
           if (!__any_sync(0xffffffffu, sum > kLimit)) {
             total += sum;
-            TmemStore16(s_at + c * 16, p);
-            ++c;
-            continue;
+            break;
           }
-          // a new maximum for the rows that passed it; what was made with the old one is scaled, these tokens are done again
-          float top = __uint_as_float(v[0]);
+          // a new maximum for the rows that passed it; the accumulator is scaled, these tokens are done again
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
+            TmemLoad16(s_at + c * 16, w);
+            const uint32_t bits = uint32_t(seen >> (16 * c));
 #pragma unroll
-          for (int e = 1; e < 32; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+            for (int e = 0; e < 16; ++e)
+              if ((bits >> e) & 1u) top = fmaxf(top, __uint_as_float(w[e]));
+          }
           const float to = fminf(shift, kUp - top * scale);
           const float f = Exp2(to - shift);
           shift = to;
           total *= f;
-          if (j > 0) {   // the accumulator is free to be changed once the half tile before has been added to it
+          if (j > 0) {   // once the half tile before has been added to it
             ok = ok && BarWait(&sh.o_done[m][u ^ 1], ((parts - 1) >> 1) & 1, quit, a.status_word);
             __syncwarp();
             FenceAfter();
+            Rescale<DIM>(o_at, f);
           }
-          Rescale<DIM>(j > 0 ? o_at : 0u, s_at, c, f);
         }
+        TmemStore32(s_at, p);
         TmemStoreDone();
         FenceBefore();
         BarArrive(&sh.p_full[m][u]);
