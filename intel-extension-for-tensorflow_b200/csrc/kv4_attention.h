@@ -66,6 +66,22 @@ __device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %
 __device__ __forceinline__ F2 Mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 __device__ __forceinline__ F2 Add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 
+// Two elements of a query row (bf16 or half) times a power of two (or its negative, or zero), as halves.
+__device__ __forceinline__ uint32_t QueryHalf2(uint32_t w, bool bf16, float by) {
+  uint32_t r;
+  if (bf16) {
+    const F2 x = Mul2(Make2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), Make2(by, by));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(Y(x)), "f"(X(x)));
+  } else {
+    uint32_t by2;
+    asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(by2) : "f"(by));
+    asm("mul.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(by2));
+  }
+  return r;
+}
+// The larger magnitudes of two pairs of bf16 (their bits order like their values; NaN counts as large).
+__device__ __forceinline__ uint32_t MaxBits2(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
+
 size_t StepsWorkspace(const AttnArgs& a);
 int LaunchSteps(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st);
 size_t PrefillWorkspace(const AttnArgs& a);

@@ -190,11 +190,12 @@ __device__ __forceinline__ uint4 Values8(uint32_t w, uint32_t step2, uint32_t lo
 
 // Eight outputs, from the codes' order (0 4 1 5 2 6 3 7) back to the channels'.
 __device__ __forceinline__ void StoreOut8(const AttnArgs& a, int bf16, int64_t at, const float (&f)[8]) {
-  union { uint4 x; uint16_t e[8]; } out;
+  union { uint4 x; uint32_t u[4]; uint16_t e[8]; } out;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = f[e < 4 ? 2 * e : 2 * (e - 4) + 1];
-    out.e[e] = bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+  for (int e = 0; e < 4; ++e) {   // channels 2e, 2e + 1
+    const float lo = f[e < 2 ? 4 * e : 4 * e - 7], hi = f[e < 2 ? 4 * e + 2 : 4 * e - 5];
+    if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(out.u[e]) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(out.u[e]) : "f"(hi), "f"(lo));
   }
   uint16_t* to = static_cast<uint16_t*>(a.out) + at;
   if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) *reinterpret_cast<uint4*>(to) = out.x;
@@ -561,15 +562,16 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         };
         float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
         if (s.bf16) {
-          float most = 0.f;
+          uint32_t bits = 0;
 #pragma unroll 1
           for (int p0 = kPieces - kHeld; p0 >= 0; p0 -= kHeld) {   // the first ones last: they stay
             fetch(p0);
 #pragma unroll
             for (int p = 0; p < kHeld; ++p)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x[p].e[e]) << 16)));
+              for (int e = 0; e < 4; ++e) bits = MaxBits2(x[p].u[e], bits);
           }
+          const float most = __uint_as_float(max(bits << 16, bits & 0xffff0000u));
           const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
           if (most > 0.f && most < INFINITY) {
             down *= __uint_as_float(uint32_t(254 - e) << 23);
@@ -585,10 +587,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
 #pragma unroll
           for (int p = 0; p < kHeld; ++p) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float raw = s.bf16 ? __uint_as_float(uint32_t(x[p].e[e]) << 16) : __half2float(__ushort_as_half(x[p].e[e]));
-              x[p].e[e] = __half_as_ushort(__float2half_rn(raw * down));
-            }
+            for (int e = 0; e < 4; ++e) x[p].u[e] = QueryHalf2(x[p].u[e], s.bf16, down);
             const uint32_t* u = x[p].u;
             *reinterpret_cast<uint4*>(to + PieceAt(in_half, p0 + p)) =
                 make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[1], u[3], 0x7632));

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
     const int i = int(QuickDiv(uint32_t(on ? rr : row0), a.div_share)), h = (on ? rr : row0) - i * a.share;
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (q.row0 + i) * a.qt + int64_t(kvh * a.share + h) * a.qh;
     union Piece { uint4 v; uint32_t u[4]; uint16_t e[8]; } x[NG][kW];
-    float most = 0.f;
+    uint32_t bits = 0;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -354,15 +354,15 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
         else
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[g][w].e[e] = src[d + e];
-        if (s.bf16)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(__uint_as_float(uint32_t(x[g][w].e[e]) << 16)));
+        for (int e = 0; e < 4; ++e) bits = MaxBits2(x[g][w].u[e], bits);
       }
     // q * down is exact but for underflow; scores are (codes' product) * up, up > 0
     float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f), up = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
     if (s.bf16) {
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      bits = MaxBits2(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+      bits = MaxBits2(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+      const float most = __uint_as_float(max(bits << 16, bits & 0xffff0000u));
       const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
       if (most > 0.f && most < INFINITY) {
         down *= __uint_as_float(uint32_t(254 - e) << 23);
@@ -378,11 +378,11 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
       for (int w = 0; w < kW; ++w) {
         Piece& y = x[g][w];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float raw = s.bf16 ? __uint_as_float(uint32_t(y.e[e]) << 16) : __half2float(__ushort_as_half(y.e[e]));
-          const float f = raw * down;
-          sum += f;
-          y.e[e] = __half_as_ushort(__float2half_rn(e & 1 ? f * 0.0625f : f));
+        for (int e = 0; e < 4; ++e) {
+          y.u[e] = QueryHalf2(y.u[e], s.bf16, down);
+          const float2 f = Pair(y.u[e]);
+          sum += f.x + f.y;
+          asm("mul.f16x2 %0, %0, %1;" : "+r"(y.u[e]) : "r"(0x2C003C00u));   // odd channels by 1/16
         }
         // a word's codes come out in pairs (j, j + 4)
         const int ks = (g * kW + w) * 2;
