@@ -25,6 +25,25 @@ template <> __device__ __forceinline__ float FromFloat<float>(float v) { return 
 template <> __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half FromFloat<__half>(float v) { return __float2half_rn(v); }
 
+// Pairs of fp32 values handled by one instruction; each is rounded as alone.
+struct F2 { uint64_t v; };
+__device__ __forceinline__ F2 Make2(float x, float y) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ F2 Same2(float x) { return Make2(x, x); }
+__device__ __forceinline__ float X(F2 a) { return __uint_as_float(uint32_t(a.v)); }
+__device__ __forceinline__ float Y(F2 a) { return __uint_as_float(uint32_t(a.v >> 32)); }
+__device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ F2 Mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 Add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 Sub2(F2 a, F2 b) { return Fma2(b, Make2(-1.f, -1.f), a); }
+
+// Two rounded values as one 32-bit word, the first in its low half.
+template <typename T> __device__ __forceinline__ uint32_t Pack16(float lo, float hi) {
+  uint32_t r;
+  if (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // VEC elements moved as one access of VEC * sizeof(T) bytes (1, 2, 4, 8 or 16); the caller guarantees the alignment.
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
 template <typename T, int VEC> __device__ __forceinline__ void LoadVec(const T* p, float (&f)[VEC]) {
@@ -33,10 +52,15 @@ template <typename T, int VEC> __device__ __forceinline__ void LoadVec(const T* 
   for (int i = 0; i < VEC; ++i) f[i] = ToFloat(x.v[i]);
 }
 template <typename T, int VEC> __device__ __forceinline__ void StoreVec(T* p, const float (&f)[VEC]) {
-  Vec<T, VEC> x;
+  union { Vec<T, VEC> x; uint32_t w[(sizeof(T) * VEC + 3) / 4]; } u;
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) x.v[i] = FromFloat<T>(f[i]);
-  *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+    for (int i = 0; i < VEC; i += 2) u.w[i / 2] = Pack16<T>(f[i], f[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) u.x.v[i] = FromFloat<T>(f[i]);
+  }
+  *reinterpret_cast<Vec<T, VEC>*>(p) = u.x;
 }
 
 __device__ __forceinline__ int64_t LoadIndex(const void* p, int is64, int64_t i) {

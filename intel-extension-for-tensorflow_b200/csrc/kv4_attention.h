@@ -56,16 +56,6 @@ __device__ __forceinline__ int RowEnd(const AttnArgs& a, const Seq& s, int i) {
 
 __device__ __forceinline__ float Exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// Pairs of fp32 values handled by one instruction; each is rounded as alone.
-struct F2 { uint64_t v; };
-__device__ __forceinline__ F2 Make2(float x, float y) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
-__device__ __forceinline__ F2 Same2(float x) { return Make2(x, x); }
-__device__ __forceinline__ float X(F2 a) { return __uint_as_float(uint32_t(a.v)); }
-__device__ __forceinline__ float Y(F2 a) { return __uint_as_float(uint32_t(a.v >> 32)); }
-__device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
-__device__ __forceinline__ F2 Mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ F2 Add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-
 // Two elements of a query row (bf16 or half) times a power of two (or its negative, or zero), as halves.
 __device__ __forceinline__ uint32_t QueryHalf2(uint32_t w, bool bf16, float by) {
   uint32_t r;

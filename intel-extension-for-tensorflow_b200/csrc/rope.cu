@@ -7,7 +7,12 @@
 // All three are bound by HBM: two (three) times the tensor's bytes, a handful of operations per element.  A row (one
 // head of one token) is spread over the 4 - 32 threads that hold it in 16-byte pieces; each thread owns both elements of
 // its pairs, so nothing is exchanged for the rotation and a call may work in place.  The angles do not depend on the
-// head: a block takes consecutive rows and forms the cosines and sines of its few tokens once, in shared memory.
+// head: a block takes consecutive tokens, forms their cosines and sines once in shared memory and walks over their rows,
+// with the next four rows per thread on their way to shared memory (gradient: two of each tensor).  At 4 x 16 KB per block
+// that keeps ~100 KB in flight on an SM with a third of the registers that loads to registers would take.
+// Measured: rotation of 16384 tokens, 32 + 8 heads of 128, fp16 (336 MB), 58 us, 5.8 TB/s; norms and rotation of 8192 such
+// tokens, bf16 (168 MB), 37 us, 4.5 TB/s (53 us when every block formed tables and weights for 32 rows); the gradient of
+// 6143 tokens with 16 + 16 heads of 64, bf16 (76 MB), 23 us + 4 us for the sums of the weights' gradients.
 #include <algorithm>
 #include <climits>
 
@@ -17,7 +22,10 @@ namespace itexb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxGradBlocks = 296;  // per side; partial weight gradients: four blocks per SM of a 148-SM device for both
+constexpr int kSms = 148;
+constexpr int kPerSm = 3;              // blocks on an SM at a time
+constexpr int kGradBlocks = 2 * kSms;
+constexpr int kTableBytes = 32 * 1024; // cosines and sines of a block's tokens
 enum { kRope = 0, kNorm = 1, kGrad = 2 };
 
 struct Side {  // queries or keys
@@ -30,13 +38,13 @@ struct Side {  // queries or keys
 struct RopeArgs {
   Side side[2];
   int heads[2];
-  FastDiv div_heads;      // kRope / kNorm: by q_heads + k_heads; kGrad: see div_side
-  FastDiv div_side[2];
-  uint32_t rows;          // kRope / kNorm: tokens * (q_heads + k_heads)
+  FastDiv div_heads;      // by q_heads + k_heads
+  FastDiv div_side[2];    // by q_heads, by k_heads
+  FastDiv div_pairs;
   int64_t tokens;
-  int head_dim, pairs, items, tpr, rows_per_block, block_tokens;
+  int head_dim, pairs, items, tpr, table_tokens;
   int interleaved, pos64, w_dtype;
-  float mscale, sin_sign, eps;
+  float mscale, sin_sign, eps, inv_dim;
   const void* positions;
   const double* inv_freq;
   float* partial;         // kGrad: [2][blocks][head_dim]
@@ -47,272 +55,397 @@ __device__ __forceinline__ float LoadW(const void* w, int dt, int i) {
          : dt == ITEXB_DT_BFLOAT16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]) : __half2float(static_cast<const __half*>(w)[i]);
 }
 
-// cos, sin (times mscale) of the tokens of rows [row0, row1) -> table[token - first][pair]
-__device__ __forceinline__ void FillTable(float2* table, const RopeArgs& a, uint32_t first, uint32_t tokens) {
+// Place of element i of a vector that threads read in pieces of VEC floats: for pieces of 8 all first halves lie before all
+// second halves, so that the 16-byte reads of neighbouring threads are neighbours too (no bank conflicts).
+template <int VEC> __device__ __forceinline__ int Plane(int i, int n) { return VEC == 8 ? ((i >> 2) & 1) * (n / 2) + (i >> 3) * 4 + (i & 3) : i; }
+template <int VEC> __device__ __forceinline__ void LoadPlane(const float* v, int i, int n, float (&f)[VEC]) {
+  if constexpr (VEC == 8) {
+    float lo[4], hi[4];
+    LoadVec<float, 4>(v + (i >> 1), lo);
+    LoadVec<float, 4>(v + n / 2 + (i >> 1), hi);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { f[k] = lo[k]; f[4 + k] = hi[k]; }
+  } else {
+    LoadVec<float, VEC>(v + i, f);
+  }
+}
+
+// cos and sin (times mscale) of `tokens` tokens from `first` on -> cs[token][2][pair]
+template <int VEC> __device__ __forceinline__ void FillTable(float* cs, const RopeArgs& a, uint32_t first, uint32_t tokens) {
   const int n = int(tokens) * a.pairs;
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int t = i / a.pairs, p = i - t * a.pairs;
+    const int t = QuickDiv(i, a.div_pairs), p = i - t * a.pairs;
     const double frac = TurnFraction(LoadIndex(a.positions, a.pos64, int64_t(first) + t), a.inv_freq[p]);
     float s, c;
     sincospif(2.f * float(frac), &s, &c);
-    table[i] = make_float2(c * a.mscale, s * a.mscale * a.sin_sign);
+    float* to = cs + t * 2 * a.pairs + (a.interleaved ? p : Plane<VEC>(p, a.pairs));
+    to[0] = c * a.mscale;
+    to[a.pairs] = s * a.mscale * a.sin_sign;
   }
 }
 
-// Rotates one item: `u`, `v` are its two VEC-element pieces, `cs` the table entries of its first pair.
-template <int VEC> __device__ __forceinline__ void Turn(float (&u)[VEC], float (&v)[VEC], const float2* cs, bool interleaved) {
-  if (VEC > 1 && interleaved) {
+// Rotates item j of a token with the cosines and sines `cs`.
+template <int VEC> __device__ __forceinline__ void Turn(float (&u)[VEC], float (&v)[VEC], const float* cs, int j, const RopeArgs& a) {
+  if constexpr (VEC == 1) {
+    const float x = u[0], y = v[0], c = cs[j], s = cs[a.pairs + j];
+    u[0] = x * c - y * s;
+    v[0] = y * c + x * s;
+  } else if (a.interleaved) {   // each piece holds whole pairs
+    constexpr int H = VEC / 2;
+    float c[2][H], s[2][H];
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-      const float2 p = cs[i], q = cs[VEC / 2 + i];
-      const float a = u[2 * i], b = u[2 * i + 1], c = v[2 * i], d = v[2 * i + 1];
-      u[2 * i] = a * p.x - b * p.y; u[2 * i + 1] = b * p.x + a * p.y;
-      v[2 * i] = c * q.x - d * q.y; v[2 * i + 1] = d * q.x + c * q.y;
+    for (int k = 0; k < 2; ++k) {
+      LoadVec<float, H>(cs + k * (a.pairs / 2) + j * H, c[k]);
+      LoadVec<float, H>(cs + a.pairs + k * (a.pairs / 2) + j * H, s[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const F2 x = Fma2(Make2(-u[2 * i + 1], u[2 * i]), Make2(s[0][i], s[0][i]), Mul2(Make2(u[2 * i], u[2 * i + 1]), Make2(c[0][i], c[0][i])));
+      const F2 y = Fma2(Make2(-v[2 * i + 1], v[2 * i]), Make2(s[1][i], s[1][i]), Mul2(Make2(v[2 * i], v[2 * i + 1]), Make2(c[1][i], c[1][i])));
+      u[2 * i] = X(x); u[2 * i + 1] = Y(x);
+      v[2 * i] = X(y); v[2 * i + 1] = Y(y);
     }
   } else {
+    float c[VEC], s[VEC];
+    LoadPlane<VEC>(cs, j * VEC, a.pairs, c);
+    LoadPlane<VEC>(cs + a.pairs, j * VEC, a.pairs, s);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float2 p = cs[i];
-      const float a = u[i], b = v[i];
-      u[i] = a * p.x - b * p.y; v[i] = b * p.x + a * p.y;
+    for (int i = 0; i < VEC; i += 2) {
+      const F2 x = Make2(u[i], u[i + 1]), y = Make2(v[i], v[i + 1]), cc = Make2(c[i], c[i + 1]), ss = Make2(s[i], s[i + 1]);
+      const F2 nx = Sub2(Mul2(x, cc), Mul2(y, ss)), ny = Fma2(x, ss, Mul2(y, cc));
+      u[i] = X(nx); u[i + 1] = Y(nx);
+      v[i] = X(ny); v[i + 1] = Y(ny);
     }
   }
 }
+// sum + u . v
+template <int VEC> __device__ __forceinline__ float Dot(const float (&u)[VEC], const float (&v)[VEC], float sum) {
+  if constexpr (VEC == 1) return fmaf(u[0], v[0], sum);
+  else {
+    F2 x = Make2(sum, 0.f);
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) x = Fma2(Make2(u[i], u[i + 1]), Make2(v[i], v[i + 1]), x);
+    return X(x) + Y(x);
+  }
+}
+template <int VEC> __device__ __forceinline__ void AddProduct(float (&to)[VEC], const float (&u)[VEC], const float (&v)[VEC]) {
+  if constexpr (VEC == 1) to[0] = fmaf(u[0], v[0], to[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const F2 x = Fma2(Make2(u[i], u[i + 1]), Make2(v[i], v[i + 1]), Make2(to[i], to[i + 1]));
+      to[i] = X(x); to[i + 1] = Y(x);
+    }
+  }
+}
+template <int VEC> __device__ __forceinline__ void AddScaled(float (&to)[VEC], const float (&u)[VEC], float by) {
+  float all[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) all[i] = by;
+  AddProduct<VEC>(to, u, all);
+}
+template <int VEC> __device__ __forceinline__ void Times(float (&u)[VEC], const float (&by)[VEC]) {
+  if constexpr (VEC == 1) u[0] *= by[0];
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const F2 x = Mul2(Make2(u[i], u[i + 1]), Make2(by[i], by[i + 1]));
+      u[i] = X(x); u[i + 1] = Y(x);
+    }
+  }
+}
+template <int VEC> __device__ __forceinline__ void Scale(float (&u)[VEC], float by) {
+  float all[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) all[i] = by;
+  Times<VEC>(u, all);
+}
 
-// Item j of a row: its pieces start at elements o0 and o1; the first pairs / VEC items are rotated.
+// Item j of a row: its pieces start at elements o0 and o1; the first pairs / VEC items are rotated.  Neighbouring items'
+// pieces are neighbours in memory: 16-byte accesses a piece apart would move every 32-byte sector twice.
 struct Item { int o0, o1; bool turned; };
 template <int VEC> __device__ __forceinline__ Item ItemOf(int j, const RopeArgs& a) {
   const int nt = a.pairs / VEC;
-  if (j < nt && !a.interleaved) return {j * VEC, a.pairs + j * VEC, true};
-  return {2 * VEC * j, 2 * VEC * j + VEC, j < nt};   // interleaved pairs, or the elements behind the rotated ones
+  if (VEC == 1 && a.interleaved && j < nt) return {2 * j, 2 * j + 1, true};
+  if (j < nt) return {j * VEC, a.pairs + j * VEC, true};
+  return {2 * a.pairs + (j - nt) * VEC, a.pairs + a.head_dim / 2 + (j - nt) * VEC, false};   // behind the rotated ones
 }
 
-// The weights as fp32 in shared memory: [queries, keys][head_dim].
-__device__ __forceinline__ void FillWeights(float* w, const RopeArgs& a) {
+// The weights as fp32 in shared memory: [queries, keys][head_dim], in Plane order.
+template <int VEC> __device__ __forceinline__ void FillWeights(float* w, const RopeArgs& a) {
   for (int i = threadIdx.x; i < 2 * a.head_dim; i += kThreads) {
-    const int side = i >= a.head_dim;
-    if (a.side[side].w != nullptr) w[i] = LoadW(a.side[side].w, a.w_dtype, i - side * a.head_dim);
+    const int side = i >= a.head_dim, e = i - side * a.head_dim;
+    if (a.side[side].w != nullptr) w[side * a.head_dim + Plane<VEC>(e, a.head_dim)] = LoadW(a.side[side].w, a.w_dtype, e);
   }
 }
-template <int VEC> __device__ __forceinline__ void TimesWeights(float (&u)[VEC], float (&v)[VEC], const float* w, const Item& it) {
+// Pieces times the weights times r.
+template <int VEC> __device__ __forceinline__ void TimesWeights(float (&u)[VEC], float (&v)[VEC], const float* w, const Item& it, int dim, float r) {
   float p[VEC], q[VEC];
-  LoadVec<float, VEC>(w + it.o0, p);
-  LoadVec<float, VEC>(w + it.o1, q);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) { u[i] *= p[i]; v[i] *= q[i]; }
+  LoadPlane<VEC>(w, it.o0, dim, p);   // pieces start at multiples of VEC
+  LoadPlane<VEC>(w, it.o1, dim, q);
+  Scale<VEC>(u, r);
+  Scale<VEC>(v, r);
+  Times<VEC>(u, p);
+  Times<VEC>(v, q);
 }
 
-// A thread's pieces of one row, as loaded.
+// A thread's pieces of one row.
 template <typename T, int VEC, int NI> struct Pieces {
   Vec<T, VEC> u[NI], v[NI];
-  __device__ __forceinline__ void Load(const T* x, int in_row, bool on, const RopeArgs& a) {
-#pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      const int j = in_row + n * a.tpr;
-      if (on && j < a.items) {
-        const Item it = ItemOf<VEC>(j, a);
-        u[n] = *reinterpret_cast<const Vec<T, VEC>*>(x + it.o0);
-        v[n] = *reinterpret_cast<const Vec<T, VEC>*>(x + it.o1);
-      }
-    }
-  }
   __device__ __forceinline__ void Floats(int n, float (&fu)[VEC], float (&fv)[VEC]) const {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { fu[i] = ToFloat(u[n].v[i]); fv[i] = ToFloat(v[n].v[i]); }
   }
 };
 
-// A block's rows are taken in P passes whose loads are all issued before the table is formed: long calls keep 4 x 32 bytes
-// per thread in flight (norms and rotation of 8192 tokens, 168 MB: 55 us with one pass per block).  Short ones take one pass
-// per block and so reach more SMs.
-template <typename T, int VEC, int NI, int MODE, int P>
-__global__ void __launch_bounds__(kThreads) RopeKernel(const __grid_constant__ RopeArgs a) {
-  extern __shared__ float4 s_mem[];
-  float* s_w = reinterpret_cast<float*>(s_mem);                              // kNorm
-  float2* s_table = reinterpret_cast<float2*>(s_w + (MODE == kNorm ? 2 * a.head_dim : 0));
-  const int group = threadIdx.x / a.tpr, in_row = threadIdx.x - group * a.tpr;
-  const int groups = kThreads / a.tpr;
-  const uint32_t row0 = blockIdx.x * uint32_t(a.rows_per_block);
-  const uint32_t row1 = min(a.rows, row0 + uint32_t(a.rows_per_block));
-  const uint32_t first = QuickDiv(row0, a.div_heads);
-  const uint32_t heads = uint32_t(a.heads[0] + a.heads[1]);
-  Pieces<T, VEC, NI> x[P];
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const uint32_t row = row0 + p * groups + group;
-    if (row < row1) {
-      const uint32_t token = QuickDiv(row, a.div_heads);
-      const int head = int(row - token * heads);
-      const int is_k = head >= a.heads[0];
-      const Side& s = a.side[is_k];
-      x[p].Load(static_cast<const T*>(s.x) + int64_t(token) * s.xt + int64_t(head - (is_k ? a.heads[0] : 0)) * s.xh, in_row, true, a);
-    }
+// The pieces of D coming rows, copied to shared memory while the rows before them are worked on.  A thread reads only what
+// it has copied itself, so a ring needs no barrier: Start(s), Commit() for each row; Wait() and Take() when its turn comes.
+template <typename T, int VEC, int NI, int D> struct Ring {
+  using Piece = Vec<T, VEC>;
+  static constexpr int kBytes = D * 2 * NI * kThreads * int(sizeof(Piece));
+  Piece* mine;
+  __device__ __forceinline__ Ring(void* at) : mine(static_cast<Piece*>(at) + threadIdx.x) {}
+  __device__ __forceinline__ static void Copy(Piece* to, const T* from) {
+    if constexpr (sizeof(Piece) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+    else if constexpr (sizeof(Piece) == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+    else *to = *reinterpret_cast<const Piece*>(from);
   }
-  FillTable(s_table, a, first, QuickDiv(row1 - 1, a.div_heads) - first + 1);
-  if (MODE == kNorm) FillWeights(s_w, a);
-  __syncthreads();
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const uint32_t row = row0 + p * groups + group;
-    const bool on = row < row1;
-    if (P > 1 && row0 + p * groups >= row1) break;
-    const uint32_t token = QuickDiv(on ? row : row0, a.div_heads);
-    const int head = int((on ? row : row0) - token * heads);
-    const int is_k = head >= a.heads[0];
-    const Side& s = a.side[is_k];
-    float r = 1.f;
-    if (MODE == kNorm) {
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        if (on && in_row + n * a.tpr < a.items) {
-          float u[VEC], v[VEC];
-          x[p].Floats(n, u, v);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) sum = fmaf(u[i], u[i], fmaf(v[i], v[i], sum));
-        }
-      }
-      for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      r = rsqrtf(sum / float(a.head_dim) + a.eps);
-    }
-    T* y = static_cast<T*>(s.y) + int64_t(token) * s.yt + int64_t(head - (is_k ? a.heads[0] : 0)) * s.yh;
+  __device__ __forceinline__ void Start(int d, const T* x, int in_row, const RopeArgs& a) {
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
       const int j = in_row + n * a.tpr;
-      if (on && j < a.items) {
+      if (j < a.items) {
         const Item it = ItemOf<VEC>(j, a);
-        float u[VEC], v[VEC];
-        x[p].Floats(n, u, v);
-        if (MODE == kNorm) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) { u[i] *= r; v[i] *= r; }
-          TimesWeights<VEC>(u, v, s_w + is_k * a.head_dim, it);
-        }
-        if (it.turned) Turn<VEC>(u, v, s_table + (token - first) * a.pairs + j * VEC, a.interleaved);
-        StoreVec<T, VEC>(y + it.o0, u);
-        StoreVec<T, VEC>(y + it.o1, v);
+        Copy(mine + (d * 2 * NI + 2 * n) * kThreads, x + it.o0);
+        Copy(mine + (d * 2 * NI + 2 * n + 1) * kThreads, x + it.o1);
       }
+    }
+  }
+  __device__ __forceinline__ Pieces<T, VEC, NI> Take(int d) const {
+    Pieces<T, VEC, NI> x;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      x.u[n] = mine[(d * 2 * NI + 2 * n) * kThreads];
+      x.v[n] = mine[(d * 2 * NI + 2 * n + 1) * kThreads];
+    }
+    return x;
+  }
+};
+__device__ __forceinline__ void Commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void Wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rows of consecutive tokens in steps of a block's thread groups.
+struct Walk {
+  uint32_t token, head, dt, dh, heads;
+  __device__ __forceinline__ Walk(uint32_t t0, uint32_t row, uint32_t step, uint32_t heads_, const FastDiv& div) : heads(heads_) {
+    const uint32_t t = QuickDiv(row, div);
+    token = t0 + t;
+    head = row - t * heads;
+    dt = QuickDiv(step, div);
+    dh = step - dt * heads;
+  }
+  __device__ __forceinline__ void Next() {
+    token += dt;
+    head += dh;
+    if (head >= heads) { head -= heads; ++token; }
+  }
+};
+
+// A block's equal part of the tokens, at most as many as its table holds.
+template <typename T, int VEC, int NI, int MODE, int D>
+__global__ void __launch_bounds__(kThreads, kPerSm) RopeKernel(const __grid_constant__ RopeArgs a) {
+  extern __shared__ float4 s_mem[];
+  Ring<T, VEC, NI, D> ring(s_mem);
+  float* s_w = reinterpret_cast<float*>(s_mem) + Ring<T, VEC, NI, D>::kBytes / 4;   // kNorm
+  float* s_table = s_w + (MODE == kNorm ? 2 * a.head_dim : 0);
+  const int group = threadIdx.x / a.tpr, in_row = threadIdx.x - group * a.tpr;
+  const uint32_t groups = kThreads / a.tpr, heads = uint32_t(a.heads[0] + a.heads[1]);
+  const uint32_t t0 = uint32_t(a.tokens * blockIdx.x / gridDim.x), t1 = uint32_t(a.tokens * (blockIdx.x + 1) / gridDim.x);
+  const uint32_t passes = ((t1 - t0) * heads + groups - 1) / groups;
+  Walk now(t0, group, groups, heads, a.div_heads), next = now;
+  auto load = [&](int d) {
+    if (next.token < t1) {
+      const int is_k = int(next.head) >= a.heads[0];
+      const Side& s = a.side[is_k];
+      ring.Start(d, static_cast<const T*>(s.x) + int64_t(next.token) * s.xt + int64_t(int(next.head) - (is_k ? a.heads[0] : 0)) * s.xh, in_row, a);
+    }
+    Commit();
+    next.Next();
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(d);
+  FillTable<VEC>(s_table, a, t0, t1 - t0);
+  if (MODE == kNorm) FillWeights<VEC>(s_w, a);
+  __syncthreads();
+  for (uint32_t pass = 0; pass < passes; pass += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (pass + d >= passes) break;
+      const bool on = now.token < t1;
+      const int is_k = int(now.head) >= a.heads[0];
+      const Side& s = a.side[is_k];
+      Wait<D - 1>();
+      const Pieces<T, VEC, NI> x = ring.Take(d);
+      float r = 1.f;
+      if (MODE == kNorm) {
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+          if (on && in_row + n * a.tpr < a.items) {
+            float u[VEC], v[VEC];
+            x.Floats(n, u, v);
+            sum = Dot<VEC>(u, u, Dot<VEC>(v, v, sum));
+          }
+        }
+        for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        r = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
+      }
+      T* y = static_cast<T*>(s.y) + int64_t(now.token) * s.yt + int64_t(int(now.head) - (is_k ? a.heads[0] : 0)) * s.yh;
+      const float* cs = s_table + (now.token - t0) * 2 * a.pairs;
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        const int j = in_row + n * a.tpr;
+        if (on && j < a.items) {
+          const Item it = ItemOf<VEC>(j, a);
+          float u[VEC], v[VEC];
+          x.Floats(n, u, v);
+          if (MODE == kNorm) TimesWeights<VEC>(u, v, s_w + is_k * a.head_dim, it, a.head_dim, r);
+          if (it.turned) Turn<VEC>(u, v, cs, j, a);
+          StoreVec<T, VEC>(y + it.o0, u);
+          StoreVec<T, VEC>(y + it.o1, v);
+        }
+      }
+      now.Next();
+      load(d);
     }
   }
 }
 
-// blockIdx.y chooses queries or keys; blocks walk the row tiles with a fixed stride, so the partial sums of the weight
-// gradient, and with them its bits, depend on the shape alone.  The next tile's loads are issued before this one's work.
-template <typename T, int VEC, int NI>
-__global__ void __launch_bounds__(kThreads) NormRopeGradKernel(const __grid_constant__ RopeArgs a) {
+// As above, first for the queries and then for the keys, whose weight gradients each thread sums over its rows: the blocks
+// and their parts depend on the shape alone, and with them the bits of those sums.
+template <typename T, int VEC, int NI, int D>
+__global__ void __launch_bounds__(kThreads, 2) NormRopeGradKernel(const __grid_constant__ RopeArgs a) {
   extern __shared__ float4 s_mem[];
-  float* s_w = reinterpret_cast<float*>(s_mem);
-  float2* s_table = reinterpret_cast<float2*>(s_w + 2 * a.head_dim);
-  const int which = blockIdx.y;
-  const Side& s = a.side[which];
-  const uint32_t heads = uint32_t(a.heads[which]);
-  const uint32_t rows = uint32_t(a.tokens) * heads;
+  using Rows = Ring<T, VEC, NI, D>;
+  Rows x_ring(s_mem), g_ring(reinterpret_cast<char*>(s_mem) + Rows::kBytes);
+  float* acc = reinterpret_cast<float*>(s_mem);  // [groups][head_dim], in the rings' place when they are empty
+  float* s_w = acc + 2 * Rows::kBytes / 4;
+  float* s_table = s_w + 2 * a.head_dim;
   const int group = threadIdx.x / a.tpr, in_row = threadIdx.x - group * a.tpr;
   const int groups = kThreads / a.tpr;
-  const uint32_t stride = gridDim.x * uint32_t(groups);
-  float du[NI][VEC], dv[NI][VEC];
+  const uint32_t b0 = uint32_t(a.tokens * blockIdx.x / gridDim.x), b1 = uint32_t(a.tokens * (blockIdx.x + 1) / gridDim.x);
+  const bool refill = b1 - b0 > uint32_t(a.table_tokens);
+  FillWeights<VEC>(s_w, a);
+  for (int which = 0; which < (a.heads[1] > 0 ? 2 : 1); ++which) {
+    const Side& s = a.side[which];
+    const uint32_t heads = uint32_t(a.heads[which]);
+    float du[NI][VEC], dv[NI][VEC];
 #pragma unroll
-  for (int n = 0; n < NI; ++n)
+    for (int n = 0; n < NI; ++n)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) du[n][i] = dv[n][i] = 0.f;
-  FillWeights(s_w, a);
-  Pieces<T, VEC, NI> x, g;
-  auto load = [&](uint32_t row) {
-    if (row < rows) {
-      const uint32_t token = QuickDiv(row, a.div_side[which]);
-      const int64_t h = row - token * heads;
-      x.Load(static_cast<const T*>(s.x) + int64_t(token) * s.xt + h * s.xh, in_row, true, a);
-      g.Load(static_cast<const T*>(s.g) + int64_t(token) * s.gt + h * s.gh, in_row, true, a);
-    }
-  };
-  load(blockIdx.x * uint32_t(groups) + group);
-  for (uint32_t row0 = blockIdx.x * uint32_t(groups); row0 < rows; row0 += stride) {
-    const uint32_t row1 = min(rows, row0 + uint32_t(groups));
-    const uint32_t first = QuickDiv(row0, a.div_side[which]);
-    __syncthreads();
-    FillTable(s_table, a, first, QuickDiv(row1 - 1, a.div_side[which]) - first + 1);
-    __syncthreads();
-    const uint32_t row = row0 + group;
-    const bool on = row < row1;
-    const uint32_t token = QuickDiv(on ? row : row0, a.div_side[which]);
-    const int64_t h = (on ? row : row0) - token * heads;
-    T* y = static_cast<T*>(s.y) + int64_t(token) * s.yt + h * s.yh;
-    const Pieces<T, VEC, NI> cx = x, cg = g;
-    load(row + stride);
-    float sum = 0.f;
+    for (uint32_t t0 = b0; t0 < b1; t0 += uint32_t(a.table_tokens)) {
+      const uint32_t t1 = min(b1, t0 + uint32_t(a.table_tokens));
+      const uint32_t passes = ((t1 - t0) * heads + groups - 1) / groups;
+      Walk now(t0, group, groups, heads, a.div_side[which]), next = now;
+      auto load = [&](int d) {
+        if (next.token < t1) {
+          x_ring.Start(d, static_cast<const T*>(s.x) + int64_t(next.token) * s.xt + int64_t(next.head) * s.xh, in_row, a);
+          g_ring.Start(d, static_cast<const T*>(s.g) + int64_t(next.token) * s.gt + int64_t(next.head) * s.gh, in_row, a);
+        }
+        Commit();
+        next.Next();
+      };
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      if (on && in_row + n * a.tpr < a.items) {
-        float u[VEC], v[VEC];
-        cx.Floats(n, u, v);
+      for (int d = 0; d < D; ++d) load(d);
+      if (which == 0 || refill) {
+        __syncthreads();
+        FillTable<VEC>(s_table, a, t0, t1 - t0);
+        __syncthreads();
+      }
+      for (uint32_t pass = 0; pass < passes; pass += D) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum = fmaf(u[i], u[i], fmaf(v[i], v[i], sum));
+        for (int d = 0; d < D; ++d) {
+          if (pass + d >= passes) break;
+          const bool on = now.token < t1;
+          T* y = static_cast<T*>(s.y) + int64_t(now.token) * s.yt + int64_t(now.head) * s.yh;
+          const float* cs = s_table + (now.token - t0) * 2 * a.pairs;
+          Wait<D - 1>();
+          const Pieces<T, VEC, NI> x = x_ring.Take(d), g = g_ring.Take(d);
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            if (on && in_row + n * a.tpr < a.items) {
+              float u[VEC], v[VEC];
+              x.Floats(n, u, v);
+              sum = Dot<VEC>(u, u, Dot<VEC>(v, v, sum));
+            }
+          }
+          for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float r = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
+          float gu[NI][VEC], gv[NI][VEC];
+          float dot = 0.f;
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            const int j = in_row + n * a.tpr;
+            if (on && j < a.items) {
+              const Item it = ItemOf<VEC>(j, a);
+              float u[VEC], v[VEC];
+              x.Floats(n, u, v);
+              g.Floats(n, gu[n], gv[n]);
+              if (it.turned) Turn<VEC>(gu[n], gv[n], cs, j, a);
+              Scale<VEC>(u, r);
+              Scale<VEC>(v, r);
+              AddProduct<VEC>(du[n], gu[n], u);
+              AddProduct<VEC>(dv[n], gv[n], v);
+              TimesWeights<VEC>(gu[n], gv[n], s_w + which * a.head_dim, it, a.head_dim, r);   // r u
+              dot = Dot<VEC>(gu[n], u, Dot<VEC>(gv[n], v, dot));
+            }
+          }
+          for (int o = a.tpr >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+          dot *= -a.inv_dim;
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            const int j = in_row + n * a.tpr;
+            if (on && j < a.items) {
+              const Item it = ItemOf<VEC>(j, a);
+              float u[VEC], v[VEC];
+              x.Floats(n, u, v);
+              Scale<VEC>(u, r);
+              Scale<VEC>(v, r);
+              AddScaled<VEC>(gu[n], u, dot);
+              AddScaled<VEC>(gv[n], v, dot);
+              StoreVec<T, VEC>(y + it.o0, gu[n]);
+              StoreVec<T, VEC>(y + it.o1, gv[n]);
+            }
+          }
+          now.Next();
+          load(d);
+        }
       }
     }
-    for (int o = a.tpr >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float r = rsqrtf(sum / float(a.head_dim) + a.eps);
-    float gu[NI][VEC], gv[NI][VEC];
-    float dot = 0.f;
+    // the block's partial sums, added in the order of its thread groups
+    Wait<0>();
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
       const int j = in_row + n * a.tpr;
-      if (on && j < a.items) {
+      if (j < a.items) {
         const Item it = ItemOf<VEC>(j, a);
-        float u[VEC], v[VEC];
-        cx.Floats(n, u, v);
-        cg.Floats(n, gu[n], gv[n]);
-        if (it.turned) Turn<VEC>(gu[n], gv[n], s_table + (token - first) * a.pairs + j * VEC, a.interleaved);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          u[i] *= r;
-          v[i] *= r;
-          du[n][i] = fmaf(gu[n][i], u[i], du[n][i]);
-          dv[n][i] = fmaf(gv[n][i], v[i], dv[n][i]);
+          acc[group * a.head_dim + it.o0 + i] = du[n][i];
+          acc[group * a.head_dim + it.o1 + i] = dv[n][i];
         }
-        TimesWeights<VEC>(gu[n], gv[n], s_w + which * a.head_dim, it);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) dot = fmaf(gu[n][i], u[i], fmaf(gv[n][i], v[i], dot));
       }
     }
-    for (int o = a.tpr >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    dot /= float(a.head_dim);
-#pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      const int j = in_row + n * a.tpr;
-      if (on && j < a.items) {
-        const Item it = ItemOf<VEC>(j, a);
-        float u[VEC], v[VEC];
-        cx.Floats(n, u, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          gu[n][i] = r * (gu[n][i] - u[i] * r * dot);
-          gv[n][i] = r * (gv[n][i] - v[i] * r * dot);
-        }
-        StoreVec<T, VEC>(y + it.o0, gu[n]);
-        StoreVec<T, VEC>(y + it.o1, gv[n]);
-      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.head_dim; c += kThreads) {
+      float sum = 0.f;
+      for (int i = 0; i < groups; ++i) sum += acc[i * a.head_dim + c];
+      a.partial[(size_t(which) * gridDim.x + blockIdx.x) * a.head_dim + c] = sum;
     }
-  }
-  // the block's partial sums: rows of one position in the row tile are added in the order of their thread groups
-  __syncthreads();
-  float* acc = reinterpret_cast<float*>(s_mem);  // [groups][head_dim]
-#pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    const int j = in_row + n * a.tpr;
-    if (j < a.items) {
-      const Item it = ItemOf<VEC>(j, a);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        acc[group * a.head_dim + it.o0 + i] = du[n][i];
-        acc[group * a.head_dim + it.o1 + i] = dv[n][i];
-      }
-    }
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < a.head_dim; c += kThreads) {
-    float sum = 0.f;
-    for (int i = 0; i < groups; ++i) sum += acc[i * a.head_dim + c];
-    a.partial[(size_t(which) * gridDim.x + blockIdx.x) * a.head_dim + c] = sum;
+    __syncthreads();
   }
 }
 
@@ -365,12 +498,13 @@ void Fill(RopeArgs& a, const itexb_rope_params_t* p) {
   a.heads[0] = p->q_heads;
   a.heads[1] = p->k_heads;
   a.tokens = p->tokens;
-  a.rows = uint32_t(p->tokens * (p->q_heads + p->k_heads));
   a.div_heads = MakeFastDiv(uint32_t(p->q_heads + p->k_heads));
   a.div_side[0] = MakeFastDiv(uint32_t(p->q_heads));
   a.div_side[1] = MakeFastDiv(uint32_t(std::max(1, p->k_heads)));
   a.head_dim = p->head_dim;
+  a.inv_dim = 1.f / float(p->head_dim);
   a.pairs = p->rotary_dim / 2;
+  a.div_pairs = MakeFastDiv(uint32_t(std::max(1, a.pairs)));
   a.interleaved = p->interleaved != 0;
   a.pos64 = p->positions_dtype == ITEXB_DT_INT64;
   a.mscale = p->mscale;
@@ -393,43 +527,36 @@ int PickVec(const RopeArgs& a, int esz, bool grad) {
   return 1;
 }
 
-int GradBlocks(int64_t tokens, int q_heads, int k_heads, int rows_per_block) {
-  const int64_t most = tokens * std::max(q_heads, k_heads);
-  return int(std::max<int64_t>(1, std::min<int64_t>(kMaxGradBlocks, (most + rows_per_block - 1) / rows_per_block)));
-}
-
-template <typename T, int VEC, int NI, int MODE, int P> int RunPasses(RopeArgs& a, size_t weights, cudaStream_t st) {
-  const int heads = a.heads[0] + a.heads[1];
-  a.rows_per_block = kThreads / a.tpr * P;
-  const size_t smem = weights + size_t(std::min(a.rows_per_block, a.rows_per_block / heads + 2)) * a.pairs * sizeof(float2);
-  auto kernel = RopeKernel<T, VEC, NI, MODE, P>;
-  if (smem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-  kernel<<<(a.rows + a.rows_per_block - 1) / a.rows_per_block, kThreads, smem, st>>>(a);
-  return CheckLaunch("RopeKernel");
-}
+int GradBlocks(int64_t tokens) { return int(std::min<int64_t>(kGradBlocks, tokens)); }
 
 template <typename T, int VEC, int NI, int MODE> int Run(RopeArgs& a, cudaStream_t st) {
   a.items = a.head_dim / (2 * VEC);
   a.tpr = 1;
   while (a.tpr < 32 && a.tpr < a.items) a.tpr *= 2;
-  const int groups = kThreads / a.tpr;
+  const size_t per_token = size_t(std::max(1, a.pairs)) * 2 * sizeof(float);
+  const int64_t most = int64_t(kTableBytes / per_token);
   const size_t weights = size_t(2) * a.head_dim * sizeof(float);
-  if constexpr (MODE == kGrad) {
-    const int least = std::min(a.heads[0], a.heads[1] > 0 ? a.heads[1] : a.heads[0]);
-    const size_t smem = std::max(weights + size_t(std::min(groups, groups / least + 2)) * a.pairs * sizeof(float2), size_t(groups) * a.head_dim * sizeof(float));
-    auto kernel = NormRopeGradKernel<T, VEC, NI>;
+  constexpr int D = NI == 1 ? 4 : 2;   // rows in flight per thread
+  const auto launch = [&](auto kernel, int64_t blocks, size_t ring, const char* what) -> int {
+    a.table_tokens = int(std::min<int64_t>(most, (a.tokens + blocks - 1) / blocks));
+    const size_t smem = ring + (MODE == kRope ? 0 : weights) + a.table_tokens * per_token;
     if (smem > 48 * 1024) ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    const int sides = a.heads[1] > 0 ? 2 : 1;
-    const int blocks = GradBlocks(a.tokens, a.heads[0], a.heads[1], groups);
-    kernel<<<dim3(blocks, sides), kThreads, smem, st>>>(a);
-    ITEXB_RETURN_IF_ERROR(CheckLaunch("NormRopeGradKernel"));
-    WeightGradKernel<<<dim3((a.head_dim + 31) / 32, sides), kSumThreads, 0, st>>>(a, blocks);
+    kernel<<<unsigned(blocks), kThreads, smem, st>>>(a);
+    return CheckLaunch(what);
+  };
+  if constexpr (MODE == kGrad) {
+    constexpr int kHalf = (D + 1) / 2;
+    const int blocks = GradBlocks(a.tokens);
+    ITEXB_RETURN_IF_ERROR(launch(NormRopeGradKernel<T, VEC, NI, kHalf>, blocks, 2 * Ring<T, VEC, NI, kHalf>::kBytes, "NormRopeGradKernel"));
+    WeightGradKernel<<<dim3((a.head_dim + 31) / 32, a.heads[1] > 0 ? 2 : 1), kSumThreads, 0, st>>>(a, blocks);
     return CheckLaunch("WeightGradKernel");
   } else {
-    // four passes where that still gives every SM four blocks, and where the pieces fit the registers
-    constexpr int kPasses = NI == 1 && MODE == kRope ? 4 : 1;
-    if (kPasses > 1 && a.rows >= uint32_t(groups) * kPasses * 148 * 4) return RunPasses<T, VEC, NI, MODE, kPasses>(a, MODE == kNorm ? weights : 0, st);
-    return RunPasses<T, VEC, NI, MODE, 1>(a, MODE == kNorm ? weights : 0, st);
+    // Equal parts for whole waves of blocks.  More waves even out the SMs' different distances to memory, fewer pay less for
+    // the blocks' starts, which cost more with weights: measured at 1, 2, 4 and 8 waves, rotation of 16384 tokens takes 68,
+    // 62, 58 and 59 us (37 tokens a block to 5), norms and rotation of 8192 tokens 39, 41, 44 and 51 us (18 to 2).
+    constexpr int kLeast = MODE == kNorm ? 16 : 8;   // tokens a block has at least before there is a second wave
+    const int64_t wave = kPerSm * kSms, waves = std::max((a.tokens + wave * most - 1) / (wave * most), a.tokens / (wave * kLeast));
+    return launch(RopeKernel<T, VEC, NI, MODE, D>, std::min(a.tokens, wave * std::max<int64_t>(1, waves)), Ring<T, VEC, NI, D>::kBytes, "RopeKernel");
   }
 }
 
@@ -486,7 +613,7 @@ extern "C" int itexb_qk_norm_rope(const itexb_qk_norm_rope_params_t* p, itexb_st
 
 extern "C" size_t itexb_qk_norm_rope_grad_workspace_bytes(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim) {
   if (tokens <= 0 || q_heads <= 0 || k_heads < 0 || head_dim <= 0) return 0;
-  return size_t(2) * size_t(GradBlocks(tokens, q_heads, k_heads, 1)) * size_t(head_dim) * sizeof(float);
+  return size_t(2) * size_t(GradBlocks(tokens)) * size_t(head_dim) * sizeof(float);
 }
 
 extern "C" int itexb_qk_norm_rope_grad(const itexb_qk_norm_rope_grad_params_t* p, itexb_stream_t stream) {
