@@ -67,6 +67,32 @@ __device__ __forceinline__ int64_t LoadIndex(const void* p, int is64, int64_t i)
   return is64 ? __ldg(static_cast<const long long*>(p) + i) : int64_t(__ldg(static_cast<const int*>(p) + i));
 }
 
+// Copies to shared memory that run beside the thread's work (pieces of 16 or 8 bytes; smaller ones are copied at once).
+template <typename P> __device__ __forceinline__ void CopyAhead(P* to, const P* from) {
+  if constexpr (sizeof(P) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+  else if constexpr (sizeof(P) == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+  else *to = *from;
+}
+__device__ __forceinline__ void CommitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void WaitCopies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rows of consecutive tokens in steps of a block's thread groups.
+struct Walk {
+  uint32_t token, head, dt, dh, heads;
+  __device__ __forceinline__ Walk(uint32_t t0, uint32_t row, uint32_t step, uint32_t heads_, const FastDiv& div) : heads(heads_) {
+    const uint32_t t = QuickDiv(row, div);
+    token = t0 + t;
+    head = row - t * heads;
+    dt = QuickDiv(step, div);
+    dh = step - dt * heads;
+  }
+  __device__ __forceinline__ void Next() {
+    token += dt;
+    head += dh;
+    if (head >= heads) { head -= heads; ++token; }
+  }
+};
+
 // Fraction of a turn of position * radians-per-position, in [-1/2, 1/2].  At position 10^6 a 32-bit product would be off
 // by 0.06 rad; the 64-bit one is off by 10^-10.
 __device__ __forceinline__ double TurnFraction(int64_t pos, double inv_freq) {

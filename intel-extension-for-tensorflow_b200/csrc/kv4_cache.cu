@@ -4,8 +4,10 @@
 //
 // Both are bound by HBM (append, head_dim 128, groups of 64, bf16: 256 B in, 72 B out per row).  A thread owns 8
 // consecutive elements, which are one 32-bit word of codes; the 4 - 16 threads of a group exchange minimum and maximum
-// by shuffles, and the rotation of halves its partners.  Every step is a separately rounded fp32 operation on cosines and sines rounded from 64 bits, so the codes are
-// those of the same formulas written with plain fp32 tensor operations.
+// by shuffles, and the rotation of halves its partners.  Every step is a separately rounded fp32 operation on cosines and
+// sines rounded from 64 bits, so the codes are those of the same formulas written with plain fp32 tensor operations.
+// Measured at 16384 tokens, 8 heads of 128, groups of 64, bf16: append 47 us (1.8 TB/s; its ~600 instructions per warp and 4
+// rows of two tensors bound it at 77 % of the issue slots, not the bytes), gather 20 us (4.3 TB/s).
 #include <algorithm>
 #include <climits>
 
@@ -25,13 +27,17 @@ struct RowArgs {
   const void* slots;
   const void* positions;
   const double* inv_freq;
+  FastDiv div_pairs;
   int slots64, pos64, pairs, interleaved, vec;
+  int eights;             // the rotated halves are whole pieces of eight
   float mscale;
   int32_t* status_word;
 };
 
 __device__ __forceinline__ float MinNan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float MaxNan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float MinNan(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float MaxNan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
 // The row of a slot; false where there is none (-1) or it lies outside the cache (reported).
 __device__ __forceinline__ bool RowOf(const RowArgs& a, int64_t slot, bool report, uint32_t* page, uint32_t* off) {
@@ -46,9 +52,9 @@ __device__ __forceinline__ bool RowOf(const RowArgs& a, int64_t slot, bool repor
 
 // Codes and (lo, step) of the group this thread's eight elements belong to; `lanes` threads share the group.
 __device__ __forceinline__ uint32_t Quantize8(const float (&x)[8], int lanes, __half2* params) {
-  float mn = x[0], mx = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) { mn = MinNan(mn, x[i]); mx = MaxNan(mx, x[i]); }
+  float mn = MinNan(MinNan(x[0], x[1], x[2]), x[3], x[4]), mx = MaxNan(MaxNan(x[0], x[1], x[2]), x[3], x[4]);
+  mn = MinNan(MinNan(mn, x[5], x[6]), x[7]);
+  mx = MaxNan(MaxNan(mx, x[5], x[6]), x[7]);
   for (int o = lanes >> 1; o > 0; o >>= 1) {
     mn = MinNan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     mx = MaxNan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -62,120 +68,134 @@ __device__ __forceinline__ uint32_t Quantize8(const float (&x)[8], int lanes, __
     return 0u;
   }
   *params = __halves2half2(lo, step);
-  const float inv = stepf > 0.f ? 1.f / stepf : 0.f;
-  uint32_t w = 0;
+  // All scaled by 1/16, which is exact: saturation to [0, 1] then leaves one bound to apply.  Adding 1.5 * 2^23 rounds to
+  // the nearest even integer, and four codes are summed as digits of one integer below 2^16.
+  const float inv = stepf > 0.f ? 1.f / stepf * 0.0625f : 0.f;
+  const F2 lo2 = Make2(-lof, -lof), one = Make2(1.f, 1.f), sixteen = Make2(16.f, 16.f), magic = Make2(12582912.f, 12582912.f);
+  F2 code[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w |= uint32_t(min(max(__float2int_rn((x[i] - lof) * inv), 0), 15)) << (4 * i);
-  return w;
+  for (int i = 0; i < 4; ++i) {
+    const F2 d = Fma2(Make2(x[2 * i], x[2 * i + 1]), one, lo2);
+    code[i] = Sub2(Fma2(Make2(fminf(__saturatef(X(d) * inv), 0.9375f), fminf(__saturatef(Y(d) * inv), 0.9375f)), sixteen, magic), magic);
+  }
+  const F2 w8 = Make2(256.f, 256.f);
+  const F2 a = Fma2(code[1], w8, code[0]), b = Fma2(code[3], w8, code[2]);
+  return __byte_perm(__float_as_uint(fmaf(Y(a), 16.f, X(a)) + 12582912.f), __float_as_uint(fmaf(Y(b), 16.f, X(b)) + 12582912.f), 0x5410);
 }
 
-// A block's rows are taken in P passes whose loads are all issued before the table is formed, as in rope.cu.
-template <typename T, int DIM, int P>
+// A block takes one row of each tensor per thread group.  Measured with the loads of P such passes issued at once: 47, 52 and
+// 59 us at P = 1, 2 and 4 (fewer warps per SM); with blocks that walk over many rows, copied ahead to shared memory: 48 us,
+// and 1 us more for the 96 tokens of a decoding step.
+template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads) Kv4AppendKernel(const __grid_constant__ RowArgs a) {
-  extern __shared__ float2 s_table[];
-  constexpr int kTpr = DIM / 8, kGroups = kThreads / kTpr, kRows = kGroups * P;
-  const uint32_t row0 = blockIdx.x * uint32_t(kRows);
+  extern __shared__ float4 s_mem[];
+  float* s_table = reinterpret_cast<float*>(s_mem);   // [token][cosines, sines][pairs]
+  constexpr int kTpr = DIM / 8, kRows = kThreads / kTpr;
+  const uint32_t row0 = blockIdx.x * uint32_t(kRows), row = row0 + threadIdx.x / kTpr;
   const uint32_t row1 = min(a.rows, row0 + uint32_t(kRows));
   const uint32_t first = QuickDiv(row0, a.div_heads);
+  const bool on = row < row1;
+  const uint32_t token = QuickDiv(on ? row : row0, a.div_heads);
+  const int head = int((on ? row : row0) - token * uint32_t(a.c.kv_heads));
   const int in_row = threadIdx.x % kTpr, e = in_row * 8;
-  union Raw { T v[8]; uint4 w[sizeof(T) / 2]; };   // eight elements as loaded
-  Raw rk[P], rv[P];
-  int64_t slot[P];
+  union { T v[8]; uint4 w[sizeof(T) / 2]; } rk, rv;   // eight elements as loaded
+  int64_t slot = -1;
+  if (on) {
+    slot = LoadIndex(a.slots, a.slots64, token);
+    const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + int64_t(head) * a.kh + e;
+    const T* vr = static_cast<const T*>(a.v) + int64_t(token) * a.vt + int64_t(head) * a.vh + e;
+    if (a.vec) {
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const uint32_t row = row0 + p * kGroups + threadIdx.x / kTpr;
-    slot[p] = -1;
-    if (row < row1) {
-      const uint32_t token = QuickDiv(row, a.div_heads);
-      const int64_t head = row - token * uint32_t(a.c.kv_heads);
-      slot[p] = LoadIndex(a.slots, a.slots64, token);
-      const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + head * a.kh + e;
-      const T* vr = static_cast<const T*>(a.v) + int64_t(token) * a.vt + head * a.vh + e;
-      if (a.vec) {
-#pragma unroll
-        for (int i = 0; i < int(sizeof(T) / 2); ++i) {
-          rk[p].w[i] = reinterpret_cast<const uint4*>(kr)[i];
-          rv[p].w[i] = reinterpret_cast<const uint4*>(vr)[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { rk[p].v[i] = kr[i]; rv[p].v[i] = vr[i]; }
+      for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+        rk.w[i] = reinterpret_cast<const uint4*>(kr)[i];
+        rv.w[i] = reinterpret_cast<const uint4*>(vr)[i];
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { rk.v[i] = kr[i]; rv.v[i] = vr[i]; }
     }
   }
   if (a.positions != nullptr) {
     const int n = int(QuickDiv(row1 - 1, a.div_heads) - first + 1) * a.pairs;
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int t = i / a.pairs, p = i - t * a.pairs;
+      const int t = QuickDiv(i, a.div_pairs), p = i - t * a.pairs;
       double s, c;
       sincospi(2.0 * TurnFraction(LoadIndex(a.positions, a.pos64, int64_t(first) + t), a.inv_freq[p]), &s, &c);
-      s_table[i] = make_float2(float(c * double(a.mscale)), float(s * double(a.mscale)));
+      // first and second fours of each eight in planes of their own: neighbouring threads' 16-byte reads are neighbours
+      float* to = s_table + t * 2 * a.pairs + (a.eights ? ((p >> 2) & 1) * (a.pairs / 2) + (p >> 3) * 4 + (p & 3) : p);
+      to[0] = float(c * double(a.mscale));
+      to[a.pairs] = float(s * double(a.mscale));
     }
     __syncthreads();
   }
+  uint32_t page = 0, off = 0;
+  const bool keep = on && RowOf(a, slot, in_row == 0 && head == 0, &page, &off);
+  float k[8], v[8];
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const uint32_t row = row0 + p * kGroups + threadIdx.x / kTpr;
-    if (P > 1 && row0 + p * kGroups >= row1) break;
-    const bool on = row < row1;
-    const uint32_t token = QuickDiv(on ? row : row0, a.div_heads);
-    const int head = int((on ? row : row0) - token * uint32_t(a.c.kv_heads));
-    uint32_t page = 0, off = 0;
-    const bool keep = on && RowOf(a, slot[p], in_row == 0 && head == 0, &page, &off);
-    float k[8], v[8];
+  for (int i = 0; i < 8; ++i) { k[i] = on ? ToFloat(rk.v[i]) : 0.f; v[i] = on ? ToFloat(rv.v[i]) : 0.f; }
+  if (a.positions != nullptr) {
+    const float* cs = s_table + (token - first) * 2 * a.pairs;
+    const float* sn = cs + a.pairs;
+    if (a.interleaved) {
+      if (e < 2 * a.pairs) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { k[i] = on ? ToFloat(rk[p].v[i]) : 0.f; v[i] = on ? ToFloat(rv[p].v[i]) : 0.f; }
-    if (a.positions != nullptr) {
-      const float2* cs = s_table + (token - first) * a.pairs;
-      if (a.interleaved) {
-        if (e < 2 * a.pairs) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (e / 2 + i < a.pairs) {
-              const float2 q = cs[e / 2 + i];
-              const float x = k[2 * i], y = k[2 * i + 1];
-              k[2 * i] = x * q.x - y * q.y;
-              k[2 * i + 1] = y * q.x + x * q.y;
-            }
+        for (int i = 0; i < 4; ++i) {
+          if (e / 2 + i < a.pairs) {
+            const float x = k[2 * i], y = k[2 * i + 1], c = cs[e / 2 + i], s = sn[e / 2 + i];
+            k[2 * i] = x * c - y * s;
+            k[2 * i + 1] = y * c + x * s;
           }
         }
-      } else if (a.pairs % 8 == 0) {  // the eight partners are the eight of another thread of the row
-        const int far = a.pairs / 8;
-        const bool turned = in_row < 2 * far, upper = in_row >= far;
-        const int from = int(threadIdx.x % 32) + (turned ? (upper ? -far : far) : 0);
-        float o[8];
+      }
+    } else if (a.eights) {  // the eight partners are the eight of another thread of the row
+      const int far = a.pairs / 8;
+      const bool turned = in_row < 2 * far, upper = in_row >= far;
+      const int from = int(threadIdx.x % 32) + (turned ? (upper ? -far : far) : 0);
+      float o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, k[i], from);
-        if (turned) {
-          const float2* q = cs + (upper ? e - a.pairs : e);
+      for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, k[i], from);
+      if (turned) {
+        const int at = (upper ? e - a.pairs : e) / 2;
+        const F2 sign = upper ? Make2(1.f, 1.f) : Make2(-1.f, -1.f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) k[i] = upper ? k[i] * q[i].x + o[i] * q[i].y : k[i] * q[i].x - o[i] * q[i].y;
-        }
-      } else if (on) {
-        const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + int64_t(head) * a.kh;
+        for (int h = 0; h < 2; ++h) {
+          float c[4], s[4];
+          LoadVec<float, 4>(cs + h * (a.pairs / 2) + at, c);
+          LoadVec<float, 4>(sn + h * (a.pairs / 2) + at, s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (e + i < 2 * a.pairs) {
-            const bool upper = e + i >= a.pairs;
-            const int at = upper ? e + i - a.pairs : e + i;
-            const float o = ToFloat(kr[upper ? at : at + a.pairs]);
-            k[i] = upper ? k[i] * cs[at].x + o * cs[at].y : k[i] * cs[at].x - o * cs[at].y;
+          for (int i = 0; i < 4; i += 2) {
+            const F2 x = Mul2(Make2(k[4 * h + i], k[4 * h + i + 1]), Make2(c[i], c[i + 1]));
+            const F2 y = Mul2(Make2(o[4 * h + i], o[4 * h + i + 1]), Make2(s[i], s[i + 1]));
+            const F2 z = Fma2(y, sign, x);
+            k[4 * h + i] = X(z);
+            k[4 * h + i + 1] = Y(z);
           }
+        }
+      }
+    } else if (on) {
+      const T* kr = static_cast<const T*>(a.k) + int64_t(token) * a.kt + int64_t(head) * a.kh;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (e + i < 2 * a.pairs) {
+          const bool upper = e + i >= a.pairs;
+          const int at = upper ? e + i - a.pairs : e + i;
+          const float o = ToFloat(kr[upper ? at : at + a.pairs]);
+          k[i] = upper ? k[i] * cs[at] + o * sn[at] : k[i] * cs[at] - o * sn[at];
         }
       }
     }
-    const int lanes = a.c.group / 8;
-    __half2 kp, vp;
-    const uint32_t kw = Quantize8(k, lanes, &kp), vw = Quantize8(v, lanes, &vp);
-    if (keep) {
-      const int64_t ci = int64_t(page) * a.c.cp + int64_t(head) * a.c.ch + int64_t(off) * a.c.ct + in_row * 4;
-      *reinterpret_cast<uint32_t*>(a.c.k_codes + ci) = kw;
-      *reinterpret_cast<uint32_t*>(a.c.v_codes + ci) = vw;
-      if (in_row % lanes == 0) {
-        const int64_t pi = int64_t(page) * a.c.pp + int64_t(head) * a.c.ph + int64_t(off) * a.c.pt + in_row / lanes;
-        a.c.k_params[pi] = kp;
-        a.c.v_params[pi] = vp;
-      }
+  }
+  const int lanes = a.c.group / 8;
+  __half2 kp, vp;
+  const uint32_t kw = Quantize8(k, lanes, &kp), vw = Quantize8(v, lanes, &vp);
+  if (keep) {
+    const int64_t ci = int64_t(page) * a.c.cp + int64_t(head) * a.c.ch + int64_t(off) * a.c.ct + in_row * 4;
+    *reinterpret_cast<uint32_t*>(a.c.k_codes + ci) = kw;
+    *reinterpret_cast<uint32_t*>(a.c.v_codes + ci) = vw;
+    if (in_row % lanes == 0) {
+      const int64_t pi = int64_t(page) * a.c.pp + int64_t(head) * a.c.ph + int64_t(off) * a.c.pt + in_row / lanes;
+      a.c.k_params[pi] = kp;
+      a.c.v_params[pi] = vp;
     }
   }
 }
@@ -249,23 +269,23 @@ bool RowsAligned(const void* p, int64_t t, int64_t h, int esz) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (t * esz) % 16 == 0 && (h * esz) % 16 == 0;
 }
 
-template <typename T, int DIM, int P, bool APPEND> int LaunchPasses(const RowArgs& a, cudaStream_t st) {
+template <typename T, int DIM> int LaunchAppend(const RowArgs& a, cudaStream_t st) {
+  constexpr int kRows = kThreads / (DIM / 8);
+  size_t smem = 0;
+  if (a.positions != nullptr) smem = size_t(std::min(kRows, kRows / a.c.kv_heads + 2)) * a.pairs * sizeof(float2);
+  Kv4AppendKernel<T, DIM><<<(a.rows + kRows - 1) / kRows, kThreads, smem, st>>>(a);
+  return CheckLaunch("Kv4AppendKernel");
+}
+template <typename T, int DIM, int P> int LaunchGather(const RowArgs& a, cudaStream_t st) {
   constexpr int kRows = kThreads / (DIM / 8) * P;
-  const unsigned blocks = (a.rows + kRows - 1) / kRows;
-  if (APPEND) {
-    size_t smem = 0;
-    if (a.positions != nullptr) smem = size_t(std::min(kRows, kRows / a.c.kv_heads + 2)) * a.pairs * sizeof(float2);
-    Kv4AppendKernel<T, DIM, P><<<blocks, kThreads, smem, st>>>(a);
-    return CheckLaunch("Kv4AppendKernel");
-  }
-  Kv4GatherKernel<T, DIM, P><<<blocks, kThreads, 0, st>>>(a);
+  Kv4GatherKernel<T, DIM, P><<<(a.rows + kRows - 1) / kRows, kThreads, 0, st>>>(a);
   return CheckLaunch("Kv4GatherKernel");
 }
 template <typename T, int DIM, bool APPEND> int LaunchDim(const RowArgs& a, cudaStream_t st) {
-  // four passes where that still gives every SM four blocks
-  constexpr int kPasses = APPEND ? 1 : 4;
-  if (kPasses > 1 && a.rows >= uint32_t(kThreads / (DIM / 8)) * kPasses * 148 * 4) return LaunchPasses<T, DIM, kPasses, APPEND>(a, st);
-  return LaunchPasses<T, DIM, 1, APPEND>(a, st);
+  if constexpr (APPEND) return LaunchAppend<T, DIM>(a, st);
+  // Four passes where that still gives every SM four blocks: 16384 tokens of 8 heads of 128 take 20 us, with one pass 27.
+  if (a.rows >= uint32_t(kThreads / (DIM / 8)) * 4 * 148 * 4) return LaunchGather<T, DIM, 4>(a, st);
+  return LaunchGather<T, DIM, 1>(a, st);
 }
 template <typename T, bool APPEND> int LaunchType(const RowArgs& a, cudaStream_t st) {
   if (a.c.head_dim == 64) return LaunchDim<T, 64, APPEND>(a, st);
@@ -308,7 +328,9 @@ extern "C" int itexb_kv4_append(const itexb_kv4_append_params_t* p, itexb_stream
   a.pos64 = p->positions_dtype == ITEXB_DT_INT64;
   a.inv_freq = p->inv_freq;
   a.pairs = p->rotary_dim / 2;
+  a.div_pairs = MakeFastDiv(uint32_t(std::max(1, a.pairs)));
   a.interleaved = p->interleaved != 0;
+  a.eights = !a.interleaved && a.pairs % 8 == 0;
   a.mscale = p->mscale;
   a.status_word = p->status_word;
   const int esz = DtypeSize(p->dtype);

@@ -199,25 +199,20 @@ template <typename T, int VEC, int NI> struct Pieces {
 };
 
 // The pieces of D coming rows, copied to shared memory while the rows before them are worked on.  A thread reads only what
-// it has copied itself, so a ring needs no barrier: Start(s), Commit() for each row; Wait() and Take() when its turn comes.
+// it has copied itself, so a ring needs no barrier: Start(s), CommitCopies() for each row; WaitCopies() and Take() when its turn comes.
 template <typename T, int VEC, int NI, int D> struct Ring {
   using Piece = Vec<T, VEC>;
   static constexpr int kBytes = D * 2 * NI * kThreads * int(sizeof(Piece));
   Piece* mine;
   __device__ __forceinline__ Ring(void* at) : mine(static_cast<Piece*>(at) + threadIdx.x) {}
-  __device__ __forceinline__ static void Copy(Piece* to, const T* from) {
-    if constexpr (sizeof(Piece) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-    else if constexpr (sizeof(Piece) == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-    else *to = *reinterpret_cast<const Piece*>(from);
-  }
   __device__ __forceinline__ void Start(int d, const T* x, int in_row, const RopeArgs& a) {
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
       const int j = in_row + n * a.tpr;
       if (j < a.items) {
         const Item it = ItemOf<VEC>(j, a);
-        Copy(mine + (d * 2 * NI + 2 * n) * kThreads, x + it.o0);
-        Copy(mine + (d * 2 * NI + 2 * n + 1) * kThreads, x + it.o1);
+        CopyAhead(mine + (d * 2 * NI + 2 * n) * kThreads, reinterpret_cast<const Piece*>(x + it.o0));
+        CopyAhead(mine + (d * 2 * NI + 2 * n + 1) * kThreads, reinterpret_cast<const Piece*>(x + it.o1));
       }
     }
   }
@@ -231,26 +226,6 @@ template <typename T, int VEC, int NI, int D> struct Ring {
     return x;
   }
 };
-__device__ __forceinline__ void Commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void Wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Rows of consecutive tokens in steps of a block's thread groups.
-struct Walk {
-  uint32_t token, head, dt, dh, heads;
-  __device__ __forceinline__ Walk(uint32_t t0, uint32_t row, uint32_t step, uint32_t heads_, const FastDiv& div) : heads(heads_) {
-    const uint32_t t = QuickDiv(row, div);
-    token = t0 + t;
-    head = row - t * heads;
-    dt = QuickDiv(step, div);
-    dh = step - dt * heads;
-  }
-  __device__ __forceinline__ void Next() {
-    token += dt;
-    head += dh;
-    if (head >= heads) { head -= heads; ++token; }
-  }
-};
-
 // A block's equal part of the tokens, at most as many as its table holds.
 template <typename T, int VEC, int NI, int MODE, int D>
 __global__ void __launch_bounds__(kThreads, kPerSm) RopeKernel(const __grid_constant__ RopeArgs a) {
@@ -269,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) RopeKernel(const __grid_cons
       const Side& s = a.side[is_k];
       ring.Start(d, static_cast<const T*>(s.x) + int64_t(next.token) * s.xt + int64_t(int(next.head) - (is_k ? a.heads[0] : 0)) * s.xh, in_row, a);
     }
-    Commit();
+    CommitCopies();
     next.Next();
   };
 #pragma unroll
@@ -284,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) RopeKernel(const __grid_cons
       const bool on = now.token < t1;
       const int is_k = int(now.head) >= a.heads[0];
       const Side& s = a.side[is_k];
-      Wait<D - 1>();
+      WaitCopies<D - 1>();
       const Pieces<T, VEC, NI> x = ring.Take(d);
       float r = 1.f;
       if (MODE == kNorm) {
@@ -353,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 2) NormRopeGradKernel(const __grid_c
           x_ring.Start(d, static_cast<const T*>(s.x) + int64_t(next.token) * s.xt + int64_t(next.head) * s.xh, in_row, a);
           g_ring.Start(d, static_cast<const T*>(s.g) + int64_t(next.token) * s.gt + int64_t(next.head) * s.gh, in_row, a);
         }
-        Commit();
+        CommitCopies();
         next.Next();
       };
 #pragma unroll
@@ -370,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) NormRopeGradKernel(const __grid_c
           const bool on = now.token < t1;
           T* y = static_cast<T*>(s.y) + int64_t(now.token) * s.yt + int64_t(now.head) * s.yh;
           const float* cs = s_table + (now.token - t0) * 2 * a.pairs;
-          Wait<D - 1>();
+          WaitCopies<D - 1>();
           const Pieces<T, VEC, NI> x = x_ring.Take(d), g = g_ring.Take(d);
           float sum = 0.f;
 #pragma unroll
@@ -425,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2) NormRopeGradKernel(const __grid_c
       }
     }
     // the block's partial sums, added in the order of its thread groups
-    Wait<0>();
+    WaitCopies<0>();
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
