@@ -4,7 +4,7 @@
 // against the 32 pairs per clock that the two products of head_dim 128 allow.
 //
 // A unit of work is 256 query rows of one key/value head (new tokens times the query heads that share it; 128 rows for
-// head_dim 256) against the tokens they see, in tiles of 128.  One block of 640 (512) threads per SM takes an equal, contiguous part
+// head_dim 256) against the tokens they see, in tiles of 128 (64 where keys and values are split).  One block of 640 (512) threads per SM takes an equal, contiguous part
 // of the list of all units' tiles; units that several blocks share are joined by a second kernel:
 //   warps 0, 1   issue tcgen05.mma (f16 operands, fp32 accumulators in tensor memory) for a half of 128 rows each: S = q K^T
 //                and O += P V, 64 tokens at a time.  A half has two S, so that the next one is there before its softmax asks
@@ -17,8 +17,14 @@
 //   warps 12-15, 16-19  keys and values, a thread per token: page lookup, codes and params into registers one tile ahead, values
 //                lo + step * code as halves into shared memory in the layout the tensor cores read (128-byte swizzle; keys
 //                K-major, values MN-major: both are rows of channels).
-// Halves hold a value to 2^-12 of itself; q enters scaled by a power of two per row (see kv4_steps.cu).  The order of
-// channels is the codes' in a word, for q, keys and the output alike.
+// Operands are halves, q scaled by a power of two per row (see kv4_steps.cu).  For bf16 inputs keys and values are rounded to
+// halves once, 2^-12 of themselves, which is nothing next to the results' own rounding (2^-9).  For half inputs, where three such
+// roundings (keys, values, weights) would nearly double the results' error (rms 0.00038 against 0.00021 of their own
+// rounding alone), keys and values are split into two halves each and a tile holds 64 tokens' first halves and behind them
+// the second ones: twice the products, 0.00026.  The order of channels is the codes' in a word, for q, keys and the output alike.
+// Measured, 2048 new tokens after 8192 with 32 / 8 heads of 128: bf16 341 us, 0.91 PFLOP/s (softmax warps: 1650 clocks per 128
+// rows and 64 tokens, the products 1280 for both halves); half 752 us (0.82 PFLOP/s of products).  1024 tokens with head_dim
+// 256: 426 and 1540 us (one stage: the conversion is not hidden).  Six prompts up to 1900, window 1024: bf16 380, half 485 us.
 // Rows of the cache that no query may see are zeros here; a value group stored as NaN is zeros too and makes the rows that see
 // it NaN at the end.  Every wait is bounded.
 #include <algorithm>
@@ -28,8 +34,10 @@
 namespace itexb {
 namespace {
 
-constexpr int kTokens = 128;                 // per tile,
-constexpr int kPart = 64;                    // and per product: half a tile
+constexpr int kTileRows = 128;               // of a tile: its tokens or, where keys and values are split, 64 tokens' rounded
+                                             // values and behind them what the rounding left
+constexpr int kPart = 64;                    // tokens per product
+template <bool SPLIT> constexpr int kTokens = SPLIT ? kPart : kTileRows;   // per tile
 constexpr int kRows = 128;                   // per half: lanes of tensor memory
 constexpr float kUp = 7.f;                   // weights are 2^(score - maximum + 7),
 constexpr float kLimit = 32768.f;            // and their sum over 64 tokens at most 2^15, so that none overflows a half
@@ -43,7 +51,7 @@ template <int DIM> struct Shape {
   static constexpr int kThreads = (3 + kHalves) * 128;
   // registers per thread of these groups; their sum is at most what the launch gives (a multiple of 8 up to 65536 / kThreads)
   static constexpr int kIssueRegs = DIM == 256 ? 80 : 56, kSoftmaxRegs = DIM == 256 ? 176 : 152, kConvertRegs = DIM == 256 ? 128 : 56;
-  static constexpr int kQBytes = kHalves * kRows * DIM * 2, kTileBytes = kTokens * DIM * 2;
+  static constexpr int kQBytes = kHalves * kRows * DIM * 2, kTileBytes = kTileRows * DIM * 2;
   static constexpr int kSmem = kQBytes + 2 * kStages * kTileBytes;
   static constexpr int kOColumn = kHalves * 128;           // of the first half's O; S `u` of half m starts at column 128 m + 64 u
 };
@@ -174,18 +182,28 @@ __device__ __forceinline__ uint32_t AndOr(uint32_t x, uint32_t mask, uint32_t co
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(constant));
   return r;
 }
-// lo + step * code for the codes at two nibbles of a word: the code's bits in the mantissa of 1024 (bits 0-3) or 64 (bits
-// 4-7), the constant subtracted (exact), one rounding in the multiply-add.
-__device__ __forceinline__ uint32_t Value2(uint32_t bits, uint32_t minus, uint32_t step2, uint32_t lo2) {
-  uint32_t c, r;
-  asm("add.f16x2 %0, %1, %2;" : "=r"(c) : "r"(bits), "r"(minus));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(c), "r"(step2), "r"(lo2));
-  return r;
+__device__ __forceinline__ uint32_t HalfAdd2(uint32_t a, uint32_t b) { uint32_t r; asm("add.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t HalfSub2(uint32_t a, uint32_t b) { uint32_t r; asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t HalfMul2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t HalfFma2(uint32_t a, uint32_t b, uint32_t c) { uint32_t r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c)); return r; }
+// What a pair of operands holds of lo + step * code: the value rounded once, or in two parts, the sum of the rounded product
+// and lo as rounded, and what these two roundings left (exact but for its own rounding, 2^-11 of a rounding).
+enum Part { kValue, kSum, kLeft };
+// For the codes at two nibbles of a word: the code's bits in the mantissa of 1024 (bits 0-3) or 64 (bits 4-7), the constant
+// subtracted (exact).
+template <int PART> __device__ __forceinline__ uint32_t Value2(uint32_t bits, uint32_t minus, uint32_t step2, uint32_t lo2) {
+  const uint32_t c = HalfAdd2(bits, minus);
+  if (PART == kValue) return HalfFma2(c, step2, lo2);
+  const uint32_t p = HalfMul2(c, step2), sum = HalfAdd2(p, lo2);
+  if (PART == kSum) return sum;
+  // the product's rounding and the sum's, whichever of its terms is the larger
+  const uint32_t of_p = HalfFma2(c, step2, p ^ 0x80008000u), lo_part = HalfSub2(sum, p), p_part = HalfSub2(sum, lo_part);
+  return HalfAdd2(HalfAdd2(HalfSub2(p, p_part), HalfSub2(lo2, lo_part)), of_p);
 }
-__device__ __forceinline__ uint4 Values8(uint32_t w, uint32_t step2, uint32_t lo2) {
+template <int PART> __device__ __forceinline__ uint4 Values8(uint32_t w, uint32_t step2, uint32_t lo2) {
   const uint32_t u = w >> 8;
-  return make_uint4(Value2(AndOr(w, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2(AndOr(w, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2),
-                    Value2(AndOr(u, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2(AndOr(u, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2));
+  return make_uint4(Value2<PART>(AndOr(w, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2<PART>(AndOr(w, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2),
+                    Value2<PART>(AndOr(u, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2<PART>(AndOr(u, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2));
 }
 
 // Eight outputs, from the codes' order (0 4 1 5 2 6 3 7) back to the channels'.
@@ -231,7 +249,7 @@ template <int DIM, int GROUP> struct Row {
     for (int i = 0; i < NG; ++i) params[i] = 0;
   }
   // -> the row's halves in shared memory
-  __device__ __forceinline__ void Store(uint8_t* tile, int row) const {
+  template <int PART> __device__ __forceinline__ void Store(uint8_t* tile, int row) const {
 #pragma unroll
     for (int i = 0; i < DIM / 32; ++i) {
       const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
@@ -239,7 +257,7 @@ template <int DIM, int GROUP> struct Row {
       for (int k = 0; k < 4; ++k) {
         const int piece = i * 4 + k;
         const uint32_t p = params[piece * 8 / GROUP];
-        *reinterpret_cast<uint4*>(tile + PieceAt(row, piece)) = Values8(w[k], __byte_perm(p, p, 0x3232), __byte_perm(p, p, 0x1010));
+        *reinterpret_cast<uint4*>(tile + PieceAt(row, piece)) = Values8<PART>(w[k], __byte_perm(p, p, 0x3232), __byte_perm(p, p, 0x1010));
       }
     }
   }
@@ -263,7 +281,7 @@ constexpr int kLeastTiles = 2;    // of a block's part, where there is little wo
 // A unit of work: M * 128 query rows of a sequence and key/value head.  The list of units runs over sequences, their row tiles
 // and the heads, in this order.
 struct Unit { int row0, row1, begin, some_begin, end, tiles; };
-template <int ROWS> __device__ __forceinline__ Unit UnitOf(const AttnArgs& a, const Seq& q, int rt) {
+template <int ROWS, bool SPLIT> __device__ __forceinline__ Unit UnitOf(const AttnArgs& a, const Seq& q, int rt) {
   Unit u;
   const int rows = q.nnew * a.share;
   u.row0 = rt * ROWS;
@@ -273,7 +291,7 @@ template <int ROWS> __device__ __forceinline__ Unit UnitOf(const AttnArgs& a, co
   u.some_begin = RowBegin(a, q, int(QuickDiv(uint32_t(u.row0), a.div_share)));
   u.end = RowEnd(a, q, int(QuickDiv(uint32_t(u.row1 - 1), a.div_share)));
   u.begin = u.some_begin & ~15;
-  u.tiles = max(1, (u.end - u.begin + kTokens - 1) / kTokens);   // rows that see nothing are one empty tile
+  u.tiles = max(1, (u.end - u.begin + kTokens<SPLIT> - 1) / kTokens<SPLIT>);   // rows that see nothing are one empty tile
   return u;
 }
 
@@ -293,10 +311,11 @@ struct Shared {   // behind the operand tiles
   Segment seg[20];
 };
 
-template <int DIM, int GROUP>
+template <int DIM, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const __grid_constant__ PrefillArgs s) {
   using H = Shape<DIM>;
   constexpr int M = H::kHalves, ST = H::kStages, NG = DIM / GROUP, ROWS = M * kRows, kThreads = H::kThreads;
+  constexpr int kParts = kTokens<SPLIT> / kPart;   // of a tile
   const AttnArgs& a = s.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* const s_q = smem;
@@ -320,7 +339,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
       Seq q{};
       for (int64_t p = p0; p < p1; ++p) {
         if (p == p0 || rt == 0) q = SeqOf(a, b, blockIdx.x == 0 && rt == 0);
-        if (!visit(b, rt, q, UnitOf<ROWS>(a, q, rt))) return;
+        if (!visit(b, rt, q, UnitOf<ROWS, SPLIT>(a, q, rt))) return;
         if (++rt == s.row_tiles) { rt = 0; ++b; }
       }
     };
@@ -413,10 +432,10 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
     if (wk.left <= 0) { g.tile0 = g.tile1 = 0; return; }
     if (wk.fresh) {
       g.q = SeqOf(a, wk.b, false);
-      g.u = UnitOf<ROWS>(a, g.q, wk.rt);
+      g.u = UnitOf<ROWS, SPLIT>(a, g.q, wk.rt);
       while (g.u.tiles == 0) {   // a sequence has fewer row tiles than the longest
         if (++wk.rt == s.row_tiles) { wk.rt = 0; g.q = SeqOf(a, ++wk.b, false); }
-        g.u = UnitOf<ROWS>(a, g.q, wk.rt);
+        g.u = UnitOf<ROWS, SPLIT>(a, g.q, wk.rt);
       }
       wk.fresh = false;
     }
@@ -453,32 +472,39 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
       const uint32_t s_d = __shfl_sync(0xffffffffu, tmem, 0) + m * 128, o_d = s_d + H::kOColumn + m * (DIM - 128);
       const uint32_t q_low = DescLow(SmemAt(s_q), 16) + m * (kRows * DIM * 2 / 16), k_low = DescLow(SmemAt(s_k), 16), v_low = DescLow(SmemAt(s_v), 128 * 128);
       uint32_t t = 0;            // tiles of the block
-      uint32_t parts = 0;        // half tiles of this half whose weights have been multiplied; even between tiles
+      uint32_t parts = 0;        // 64 tokens each: those of this half whose weights have been multiplied; S by their parity
       uint32_t segs = 0;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = __all_sync(0xffffffffu, ok && BarWait(bar, parity & 1, quit, a.status_word)); };
-      // S of half tile u of tile `tile`
-      auto scores = [&](uint32_t tile, int u) {
+      // S number u, of part `at` of tile `tile`
+      auto scores = [&](uint32_t tile, int at, int u) {
         FenceAfter();
         if (ElectOne()) {
-          const uint32_t ka = k_low + (tile % ST) * (H::kTileBytes / 16) + u * (kPart * 128 / 16), d = s_d + u * kPart;
+          const uint32_t ka = k_low + (tile % ST) * (H::kTileBytes / 16) + at * (kPart * 128 / 16), d = s_d + u * kPart;
           MmaSmem<false>(d, q_low, ka, kIdescS);
 #pragma unroll
           for (int k = 1; k < DIM / 16; ++k) {
             constexpr int kBlock = 128 * 128 / 16;
             MmaSmem<true>(d, q_low + (k / 4) * kBlock + (k % 4) * 2, ka + (k / 4) * kBlock + (k % 4) * 2, kIdescS);
           }
+          if (SPLIT) {
+#pragma unroll
+            for (int k = 0; k < DIM / 16; ++k) {
+              constexpr int kBlock = 128 * 128 / 16;
+              MmaSmem<true>(d, q_low + (k / 4) * kBlock + (k % 4) * 2, ka + kPart * 128 / 16 + (k / 4) * kBlock + (k % 4) * 2, kIdescS);
+            }
+          }
           Commit(&sh.s_full[m][u]);
           BarArrive(&sh.s_full[m][u]);
-          if (u == 1) Commit(&sh.k_empty[tile % ST]);
+          if (at == kParts - 1) Commit(&sh.k_empty[tile % ST]);
         }
         __syncwarp();
       };
       while (ok && next_segment()) {
-        const int n = __shfl_sync(0xffffffffu, 2 * (g.tile1 - g.tile0), 0), halves = __shfl_sync(0xffffffffu, g.halves, 0);
+        const int n = __shfl_sync(0xffffffffu, kParts * (g.tile1 - g.tile0), 0), halves = __shfl_sync(0xffffffffu, g.halves, 0);
         if (m >= halves) {
           // no rows here: the tiles are let through one by one, since a barrier's parity tells only neighbouring phases apart
-          for (int j = 0; j < n / 2 && ok; ++j, ++t) {
+          for (int j = 0; j < n / kParts && ok; ++j, ++t) {
             if (!wait(&sh.k_full[t % ST], t / ST)) break;
             if (ElectOne()) BarArrive(&sh.k_empty[t % ST]);
             if (!wait(&sh.v_full[t % ST], t / ST)) break;
@@ -488,34 +514,39 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
           continue;
         }
         // the half's last weights of the segment before have been multiplied, its next rows of q are there
-        if (parts > 0) wait(&sh.o_done[m][1], (parts - 1) >> 1);
+        if (parts > 0) wait(&sh.o_done[m][(parts - 1) & 1], (parts - 1) >> 1);
         wait(&sh.q_full[m], segs++);
         if (!wait(&sh.k_full[t % ST], t / ST)) break;
-        scores(t, 0);
+        scores(t, 0, parts & 1);
         for (int j = 0; j < n; ++j, ++parts) {
-          const int u = j & 1;
+          const int u = parts & 1, at = j % kParts;   // at: part of tile t
+          const bool last = at == kParts - 1;
           if (j + 1 < n) {
-            // S of the half tile after this one goes where the weights of the one before it were
-            if (u == 1) wait(&sh.k_full[(t + 1) % ST], (t + 1) / ST);
+            // S of the part after this one goes where the weights of the one before it were
+            if (last) wait(&sh.k_full[(t + 1) % ST], (t + 1) / ST);
             if (j > 0) wait(&sh.o_done[m][u ^ 1], (parts - 1) >> 1);
             if (!ok) break;
-            scores(t + u, u ^ 1);
+            scores(t + last, last ? 0 : at + 1, u ^ 1);
           }
-          if (u == 0) wait(&sh.v_full[t % ST], t / ST);
+          if (at == 0) wait(&sh.v_full[t % ST], t / ST);
           if (!wait(&sh.p_full[m][u], parts >> 1)) break;
           FenceAfter();
           if (ElectOne()) {
-            const uint32_t va = v_low + (t % ST) * (H::kTileBytes / 16) + u * (kPart * 128 / 16), p = s_d + u * kPart;
+            const uint32_t va = v_low + (t % ST) * (H::kTileBytes / 16) + at * (kPart * 128 / 16), p = s_d + u * kPart;
             if (j > 0) MmaTmem<true>(o_d, p, va, kIdescO);
             else MmaTmem<false>(o_d, p, va, kIdescO);
 #pragma unroll
             for (int k = 1; k < kPart / 16; ++k) MmaTmem<true>(o_d, p + k * 8, va + k * 128, kIdescO);
+            if (SPLIT) {
+#pragma unroll
+              for (int k = 0; k < kPart / 16; ++k) MmaTmem<true>(o_d, p + k * 8, va + (kPart / 16 + k) * 128, kIdescO);
+            }
             Commit(&sh.o_done[m][u]);
             BarArrive(&sh.o_done[m][u]);
-            if (u == 1) Commit(&sh.v_empty[t % ST]);
+            if (last) Commit(&sh.v_empty[t % ST]);
           }
           __syncwarp();
-          t += u;
+          t += last;
         }
       }
       // nothing in flight when tensor memory is given back
@@ -529,7 +560,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
     const int m = (warp - 4) >> 2, in_half = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_m = tmem + lanes + m * 128, o_at = tmem + lanes + H::kOColumn + m * DIM;
-    uint32_t parts = 0, t4 = 0;   // half tiles of this half; all tiles of the block
+    uint32_t parts = 0, t4 = 0;   // 64 tokens each: of this half; all tiles of the block
     bool ok = true;
     while (ok && next_segment()) {
       const int n = g.tile1 - g.tile0;
@@ -597,14 +628,14 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         BarArrive(&sh.q_full[m]);
       }
       float shift = kNone, total = 0.f;       // weights are 2^(score * scale + shift)
-      for (int j = 0; j < 2 * n && ok; ++j, ++parts) {
-        const int u = j & 1;
+      for (int j = 0; j < kParts * n && ok; ++j, ++parts) {
+        const int u = parts & 1, at = j % kParts;
         ok = BarWait(&sh.s_full[m][u], (parts >> 1) & 1, quit, a.status_word);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         FenceAfter();
-        const int j0 = g.u.begin + g.tile0 * kTokens + j * kPart;
-        const uint32_t* there = sh.there[t4 & 3] + 2 * u;
+        const int j0 = g.u.begin + g.tile0 * kTokens<SPLIT> + j * kPart;
+        const uint32_t* there = sh.there[t4 & 3] + 2 * at;
         const uint32_t s_at = s_m + u * kPart;
         const F2 scale2 = Make2(scale, scale);
         // of the half tile's tokens, those that exist and that this row sees; all of them in most half tiles
@@ -666,9 +697,9 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         TmemStoreDone();
         FenceBefore();
         BarArrive(&sh.p_full[m][u]);
-        t4 += u;
+        t4 += at == kParts - 1;
       }
-      ok = __all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, BarWait(&sh.o_done[m][1], ((parts - 1) >> 1) & 1, quit, a.status_word));
+      ok = __all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, BarWait(&sh.o_done[m][(parts - 1) & 1], ((parts - 1) >> 1) & 1, quit, a.status_word));
       if (!ok) break;
       FenceAfter();
       uint32_t nan_groups = 0;
@@ -732,7 +763,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
     auto place = [&]() {   // of the tile that `ahead` stands at, and one on
       Place x{-1, 0, 0};
       if (!more) return x;
-      const int tok = g.u.begin + ahead * kTokens + t;
+      const int tok = g.u.begin + ahead * kTokens<SPLIT> + (SPLIT ? t % kPart : t);
       x.kvh = g.kvh;
       if (tok >= g.u.some_begin && tok < g.u.end) {
         const int col = int(QuickDiv(uint32_t(tok), a.c.div_page));
@@ -771,7 +802,8 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
         if (lane == 0) sh.there[n & 3][w] = there;
       }
-      row.Store(tiles + (n % ST) * H::kTileBytes, t);
+      if (SPLIT && t >= kPart) row.template Store<kLeft>(tiles + (n % ST) * H::kTileBytes, t);
+      else row.template Store<SPLIT ? kSum : kValue>(tiles + (n % ST) * H::kTileBytes, t);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       BarArrive(&full[n % ST]);
       load(next);
@@ -829,16 +861,16 @@ size_t PartBytes(const AttnArgs& a) {
   return size_t(kMaxBlocks) * 2 * rows * (size_t(a.c.head_dim) * sizeof(float) + sizeof(float2));
 }
 
-template <int DIM, int GROUP> int LaunchGroup(PrefillArgs& s, cudaStream_t st) {
+template <int DIM, int GROUP, bool SPLIT> int LaunchGroup(PrefillArgs& s, cudaStream_t st) {
   using H = Shape<DIM>;
   constexpr int kSmem = H::kSmem + int(sizeof(Shared)), ROWS = H::kHalves * kRows;
-  auto kernel = PrefillKernel<DIM, GROUP>;
+  auto kernel = PrefillKernel<DIM, GROUP, SPLIT>;
   ITEXB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const int64_t rows = int64_t(s.a.max_new) * s.a.share;
   s.row_tiles = int((rows + ROWS - 1) / ROWS);
   int64_t span = std::min<int64_t>(s.a.max_kept, int64_t(s.a.table_cols) * s.a.c.page_size);
   if (s.a.window > 0) span = std::min<int64_t>(span, int64_t(s.a.window) + s.a.max_new);
-  const int64_t most = (span / kTokens + 2) * s.a.num_seqs * s.row_tiles * s.a.c.kv_heads;   // tiles
+  const int64_t most = (span / kTokens<SPLIT> + 2) * s.a.num_seqs * s.row_tiles * s.a.c.kv_heads;   // tiles
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(std::min<int64_t>(std::min(kMaxBlocks, SmCount()), std::max<int64_t>(1, most / kLeastTiles))));
   cfg.blockDim = dim3(H::kThreads);
@@ -859,11 +891,16 @@ template <int DIM, int GROUP> int LaunchGroup(PrefillArgs& s, cudaStream_t st) {
   ITEXB_CUDA(cudaLaunchKernelEx(&cfg, PrefillJoinKernel<DIM>, s));
   return CheckLaunch("PrefillJoinKernel");
 }
-template <int DIM> int LaunchDim(PrefillArgs& s, cudaStream_t st) {
-  if (s.a.c.group == 32) return LaunchGroup<DIM, 32>(s, st);
-  if (s.a.c.group == 64) return LaunchGroup<DIM, 64>(s, st);
-  if constexpr (DIM >= 128) return LaunchGroup<DIM, 128>(s, st);
+template <int DIM, bool SPLIT> int LaunchDim(PrefillArgs& s, cudaStream_t st) {
+  if (s.a.c.group == 32) return LaunchGroup<DIM, 32, SPLIT>(s, st);
+  if (s.a.c.group == 64) return LaunchGroup<DIM, 64, SPLIT>(s, st);
+  if constexpr (DIM >= 128) return LaunchGroup<DIM, 128, SPLIT>(s, st);
   return SetError(ITEXB_INTERNAL, "kv4_attention: group above head_dim");
+}
+template <bool SPLIT> int Launch(PrefillArgs& s, cudaStream_t st) {
+  if (s.a.c.head_dim == 64) return LaunchDim<64, SPLIT>(s, st);
+  if (s.a.c.head_dim == 128) return LaunchDim<128, SPLIT>(s, st);
+  return LaunchDim<256, SPLIT>(s, st);
 }
 
 }  // namespace
@@ -877,9 +914,7 @@ int LaunchPrefill(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st
   s.part_o = static_cast<float*>(workspace);
   s.part_l = reinterpret_cast<float2*>(s.part_o + size_t(kMaxBlocks) * 2 * (a.c.head_dim == 256 ? 1 : 2) * kRows * a.c.head_dim);
   s.heads = reinterpret_cast<Head*>(static_cast<uint8_t*>(workspace) + PartBytes(a));
-  if (a.c.head_dim == 64) return LaunchDim<64>(s, st);
-  if (a.c.head_dim == 128) return LaunchDim<128>(s, st);
-  return LaunchDim<256>(s, st);
+  return s.bf16 ? Launch<false>(s, st) : Launch<true>(s, st);
 }
 
 }  // namespace itexb
