@@ -58,7 +58,7 @@ def test_norm_rope_refuses(mods):
     refused(lib, L, "qk_norm_rope_grad", L.QkNormRopeGradParams(n, PTR, 128, 64, PTR, 64, 64, PTR, PTR, 0), "NULL gradient or workspace")
     assert lib.itexb_rope(C.byref(rope_params(L, tokens=0, q=0, q_out=0)), None) == L.OK         # nothing to do, nothing launched
     assert lib.itexb_qk_norm_rope_grad_workspace_bytes(0, 8, 8, 64) == 0
-    assert lib.itexb_qk_norm_rope_grad_workspace_bytes(3, 2, 1, 64) == 2 * 6 * 64 * 4
+    assert lib.itexb_qk_norm_rope_grad_workspace_bytes(3, 2, 1, 64) == 2 * 3 * 64 * 4
 
 
 def cache_params(L, **kw):

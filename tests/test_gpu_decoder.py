@@ -176,6 +176,32 @@ def test_qk_norm_rope_backward_against_differences(K):
         assert abs(got - want) <= 3e-5 * size
 
 
+@pytest.mark.parametrize("tokens, heads, dim, dtype", [(20011, 1, 256, torch.bfloat16), (10007, 1, 256, torch.float32), (4099, 3, 64, torch.float16)])
+def test_long_calls(K, tokens, heads, dim, dtype):
+    """Blocks of many tokens, several waves of them, tables formed in several turns: every row is right, and so are the sums."""
+    freq = 10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64, device="cuda") * 2 / dim)
+    pos = torch.randperm(tokens, device="cuda")
+    q, k = randn(1, tokens, heads, dim, dtype=dtype), randn(2, tokens, heads, dim, dtype=dtype)
+    w = [1 + 0.2 * randn(s, dim) for s in (3, 4)]
+    g = [randn(s, tokens, heads, dim, dtype=dtype) for s in (5, 6)]
+    turned = K.rope(q, pos, freq, k=k)
+    grads = K.qk_norm_rope_backward(*g, q, k, *w, pos, freq, eps=1e-5)
+    for i, (x, y) in enumerate(zip((q, k), turned)):
+        want, size = R.rotate(x.double(), pos, freq)
+        within(y, want, size * R.ROT + out_tol(want, dtype))
+        xd, wd = x.double(), w[i].double()
+        r = (xd.pow(2).mean(-1, keepdim=True) + 1e-5).rsqrt()
+        hat = xd * r
+        t, size = R.rotate(g[i].double(), pos, freq, sign=-1.0)
+        u, ub = t * wd, size * wd.abs()
+        dx = r * (u - hat * (u * hat).mean(-1, keepdim=True))
+        bound = r * (ub + hat.abs() * (ub * hat.abs()).mean(-1, keepdim=True)) * (R.ROT + (2 * dim + 16) * 2.0 ** -24)
+        within(grads[i], dx, bound + out_tol(dx, dtype))
+        # fp32: a thread's rows (at most 68 tokens' of a block, one after another), then at most 64 threads' sums; 64 bits behind that
+        dw, bound = (t * hat).sum((0, 1)), (size * hat.abs()).sum((0, 1)) * (R.ROT + (dim / 2 + 68 * heads + 64 + 32) * 2.0 ** -24)
+        within(grads[2 + i], dw, bound + out_tol(dw, torch.float32))
+
+
 def test_gradient_of_no_tokens_is_zero(K):
     e, w = torch.empty((0, 2, 64), device="cuda"), torch.ones(64, device="cuda")
     freq = torch.ones(32, dtype=torch.float64, device="cuda")
@@ -502,6 +528,60 @@ def test_attention_beyond_32_bit_offsets(kv4):
         q = randn(3, new, 4, dim, dtype=torch.bfloat16)
         got = cache.attention(q, table, torch.tensor([n], dtype=torch.int32, device="cuda"), max_new=new)
         R.check_attention(got, *R.attention(cache, q, table, [n], [0, new]), new, "far pages")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("most", [1, 8, 23])
+def test_attention_of_many_sequences(kv4, most, dtype):
+    """More sequences than a block has threads, most of them short or idle."""
+    new = [(7 * b) % (most + 1) for b in range(330)]
+    new[5] = most
+    kept = [n + (37 * b) % 90 if n else 0 for b, n in enumerate(new)]
+    cache = filled(kv4, sum(-(-n // 16) for n in kept) + 1, 16, 1, 64, 64)
+    attend(kv4, cache, new, kept, 4, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attention_prompts_of_all_lengths(kv4, dim, dtype):
+    """Odd and even numbers of tiles follow each other in a block's part, with one half of rows and with two."""
+    new = [1, 63, 64, 65, 127, 129, 190, 0, 257, 33, 320, 5]
+    kept = [n + (0, 64, 130, 3)[b % 4] if n else 0 for b, n in enumerate(new)]
+    cache = filled(kv4, sum(-(-n // 16) for n in kept) + 1, 16, 3, dim, 64)
+    attend(kv4, cache, new, kept, 6, dtype)
+    attend(kv4, cache, new, kept, 6, dtype, window=50)
+
+
+@pytest.mark.parametrize("share, new", [(4, 8), (3, 11), (32, 1), (33, 1)])
+def test_attention_on_both_sides_of_the_choice_of_kernel(kv4, share, new):
+    cache = filled(kv4, 40, 16, 2, 128, 128)
+    attend(kv4, cache, [new, 1], [300, 200], 2 * share, torch.float16)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-4])
+@pytest.mark.parametrize("new", [2, 70])
+def test_attention_of_any_scale(kv4, scale, new):
+    cache = filled(kv4, 30, 16, 2, 64, 32)
+    for dtype in (torch.float16, torch.bfloat16):
+        attend(kv4, cache, [new, 1], [300, 100], 8, dtype, scale=scale)
+
+
+def test_a_captured_prompt_replays(kv4):
+    """Lengths, tables and rows are read at each replay; max_new and max_kept only bound them."""
+    cache = filled(kv4, 120, 16, 2, 128, 64)
+    q, kept, starts = randn(1, 300, 8, 128, dtype=torch.float16), ints([0, 0]), ints([0, 0, 0])
+    table = tables([900, 900], 16, 120)
+    out = torch.empty_like(q)
+    cache.attention(q, table, kept, q_starts=starts, max_new=200, max_kept=900, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.attention(q, table, kept, q_starts=starts, max_new=200, max_kept=900, out=out)
+    for new, have in (([200, 100], [900, 100]), ([1, 0], [1, 0]), ([70, 130], [500, 130]), ([0, 1], [30, 30])):
+        kept.copy_(ints(have))
+        starts.copy_(ints([0, new[0], sum(new)]))
+        g.replay()
+        want, size, dots = R.attention(cache, q, table, have, [0, new[0], sum(new)])
+        R.check_attention(out, want, size, dots, sum(new), (new, have))
 
 
 def test_attention_strided_queries_and_outputs(kv4):
