@@ -276,7 +276,7 @@ struct PrefillArgs {
   Head* heads;             // [blocks]
 };
 constexpr int kMaxBlocks = 148;
-constexpr int kLeastTiles = 2;    // of a block's part, where there is little work
+constexpr int kLeastTiles = 2;    // of a block's part, where there is little work: 64 tokens after 960 take 26 us with 1 or 2, 29 with 4
 
 // A unit of work: M * 128 query rows of a sequence and key/value head.  The list of units runs over sequences, their row tiles
 // and the heads, in this order.

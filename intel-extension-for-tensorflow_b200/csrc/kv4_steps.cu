@@ -27,6 +27,8 @@
 // which every block takes an equal, contiguous part; a (sequence, head) that ends inside a block's part is written by it, the
 // others are joined from at most one result per block by a second kernel.  (One block per 2048 tokens instead left a fifth of
 // the machine idle behind the longest contexts, and smaller chunks cost more at their ends than they evened out.)
+// Measured, single tokens, 32 / 8 heads of 128, groups of 64: 64 sequences up to 8192 (421 MB) 103 us, 4.1 TB/s over the call, 5.3
+// while tiles stream; bound by issue slots (58 % busy) and the dependent steps of a tile with three warps per scheduler.
 #include <algorithm>
 
 #include "kv4_attention.h"
@@ -37,7 +39,8 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;                       // tokens
 constexpr int kMaxBlocks = 740;                 // five per SM of a 148-SM device
-constexpr int kLeastTiles = 8;                  // of a block's part, where there is little work
+constexpr int kLeastTiles = 8;                  // of a block's part, where there is little work: 5 sequences of up to 700
+                                                // tokens take 14.4 us on the device with 4 or 8, 14.6 with 16
 constexpr float kRescale = 4.f;                 // scores may pass the running maximum by 4 before it moves,
 constexpr float kShift = 2.f;                   // so weights are 2^(score - maximum - 2), at most 4
 constexpr float kNone = -3.0e38f;               // the maximum of no scores
@@ -121,8 +124,10 @@ __device__ __forceinline__ void StoreOut(const AttnArgs& a, int bf16, int64_t at
 // PAGE16: pages hold a multiple of 16 tokens, so a tile lies in one page.
 // At least so many blocks share an SM (registers): what keeps 16 warps on it for the common shape.
 template <int DIM, int GROUP, int NT> constexpr int kShareSm = DIM == 64 ? (NT == 1 ? 4 : 3) : DIM == 128 ? (NT == 1 ? 3 : 2) : 2;
-// Tiles a warp works on at a time, where registers allow: two give each other something to do and share the bookkeeping.
-template <int DIM, int NT> constexpr int kTogether = DIM < 256 && NT == 1 ? 2 : 1;
+// Tiles a warp works on at a time.  Two give each other something to do and share the bookkeeping, but cost registers and so
+// warps.  Measured with one and with two: head_dim 128, 64 sequences up to 8192 110, 103 us, one of 131072 48, 44; head_dim 64,
+// 24 sequences of 3000 with 5 tokens each 35, 39 us (groups of 64: 31, 36), 64 sequences with one each 72, 76.
+template <int DIM, int NT> constexpr int kTogether = DIM == 128 && NT == 1 ? 2 : 1;
 template <int DIM, int NT> constexpr int kStagesOf = kTogether<DIM, NT> == 2 ? 3 : 4;
 
 template <int DIM, int GROUP, int NT, bool PAGE16>
