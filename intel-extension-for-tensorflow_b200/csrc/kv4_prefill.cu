@@ -13,7 +13,7 @@
 //                Tensor memory: two S of each half (64 columns; P overwrites it as halves), O of each half
 //   warps 4-11   softmax, a thread per row: weights 2^(s - m + 7) straight from S with the maximum m of earlier tokens; only
 //                when a row's weights of 64 tokens add up to more than 2^15 is the maximum looked for, the accumulator rescaled
-//                and the 64 tokens done again.  Weights go back to tensor memory as the second product's A operand.
+//                and the 64 tokens done again, once.  Weights go back to tensor memory as the second product's A operand.
 //   warps 12-15, 16-19  keys and values, a thread per token: page lookup, codes and params into registers one tile ahead, values
 //                lo + step * code as halves into shared memory in the layout the tensor cores read (128-byte swizzle; keys
 //                K-major, values MN-major: both are rows of channels).
@@ -41,7 +41,11 @@ template <bool SPLIT> constexpr int kTokens = SPLIT ? kPart : kTileRows;   // pe
 constexpr int kRows = 128;                   // per half: lanes of tensor memory
 constexpr float kUp = 7.f;                   // weights are 2^(score - maximum + 7),
 constexpr float kLimit = 32768.f;            // and their sum over 64 tokens at most 2^15, so that none overflows a half
-constexpr float kNone = 3.0e38f;             // -maximum + 7 of no scores
+constexpr float kNone = 3.0e38f;             // -maximum + 7 of no scores; -kNone: the largest of no products
+constexpr float kFarthest = 2.9e38f;         // of some scores at most
+// Scores this large (of any row of a warp) have their maximum taken off before they are scaled: 7 - maximum as one fp32 number
+// would be off by 2^-25 of the maximum, in all weights alike, but where the maximum moves and where parts are joined.
+constexpr float kFar = 1024.f;
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 
 template <int DIM> struct Shape {
@@ -159,6 +163,11 @@ __device__ __forceinline__ void TmemStoreDone() { asm volatile("tcgen05.wait::st
 
 template <int N> __device__ __forceinline__ void RegistersDown() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void RegistersUp() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// The power of two that goes into the weights of a row whose largest product so far is `ref`.
+__device__ __forceinline__ float ShiftOf(float ref, float scale) {
+  return ref <= -kNone ? kNone : fminf(fmaxf(fmaf(-ref, scale, kUp), -kFarthest), kFarthest);
+}
 
 // A row's accumulator times f.
 template <int DIM> __device__ __forceinline__ void Rescale(uint32_t o_at, float f) {
@@ -606,7 +615,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
           const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
           if (most > 0.f && most < INFINITY) {
             down *= __uint_as_float(uint32_t(254 - e) << 23);
-            scale = fmaxf(scale * __uint_as_float(uint32_t(e) << 23), 1e-37f);
+            scale = fminf(fmaxf(scale * __uint_as_float(uint32_t(e) << 23), 1e-37f), kNone);
           }
         } else {
           fetch(0);
@@ -627,7 +636,9 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         BarArrive(&sh.q_full[m]);
       }
-      float shift = kNone, total = 0.f;       // weights are 2^(score * scale + shift)
+      // Weights are 2^((v - ref) * scale + 7) of a row's products v; ref is the largest of them, as of when it was last looked for.
+      float ref = -kNone, shift = kNone, total = 0.f;
+      bool far = false;                       // the warp's rows: ref is taken off first, else as 2^(v * scale + ShiftOf(ref))
       for (int j = 0; j < kParts * n && ok; ++j, ++parts) {
         const int u = parts & 1, at = j % kParts;
         ok = BarWait(&sh.s_full[m][u], (parts >> 1) & 1, quit, a.status_word);
@@ -647,14 +658,15 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         }
         uint32_t p[32];
 #pragma unroll 1
-        for (;;) {
+        for (bool again = false;; again = true) {   // twice at most: with ref the maximum, no weight is above 2^7 but by rounding
           // P overwrites S only once its weights are known to be good
           uint32_t v[64];
           TmemLoad64(s_at, v);
-          if (masked) {
+          if (masked || far) {
+            const float off = far ? ref : 0.f;
 #pragma unroll
             for (int e = 0; e < 64; ++e)
-              if ((uint32_t(seen >> (e & 32)) & (1u << (e & 31))) == 0u) v[e] = 0xff800000u;
+              v[e] = (uint32_t(seen >> (e & 32)) & (1u << (e & 31))) == 0u ? 0xff800000u : __float_as_uint(__uint_as_float(v[e]) - off);
           }
           const F2 shift2 = Make2(shift, shift);
           F2 part[4] = {Make2(0.f, 0.f), Make2(0.f, 0.f), Make2(0.f, 0.f), Make2(0.f, 0.f)};
@@ -667,7 +679,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
           }
           const F2 all = Add2(Add2(part[0], part[1]), Add2(part[2], part[3]));
           const float sum = X(all) + Y(all);
-          if (!__any_sync(0xffffffffu, sum > kLimit)) {
+          if (again || !__any_sync(0xffffffffu, sum > kLimit)) {
             total += sum;
             break;
           }
@@ -682,9 +694,10 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
             for (int e = 0; e < 16; ++e)
               if ((bits >> e) & 1u) top = fmaxf(top, __uint_as_float(w[e]));
           }
-          const float to = fminf(shift, kUp - top * scale);
-          const float f = Exp2(to - shift);
-          shift = to;
+          const float to = fmaxf(ref, top), f = Exp2((ref - to) * scale);
+          ref = to;
+          far = __any_sync(0xffffffffu, to > -kNone && fabsf(to * scale) > kFar);
+          shift = far ? kUp : ShiftOf(ref, scale);
           total *= f;
           if (j > 0) {   // once the half tile before has been added to it
             ok = ok && BarWait(&sh.o_done[m][u ^ 1], ((parts - 1) >> 1) & 1, quit, a.status_word);
@@ -715,7 +728,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
       const bool whole = g.tile1 - g.tile0 == g.u.tiles;
       const int64_t slot = int64_t(blockIdx.x) * 2 + (g.tile0 == 0);
       const int in_unit = m * kRows + in_half;
-      if (!whole) s.part_l[slot * ROWS + in_unit] = make_float2(shift, total);
+      if (!whole) s.part_l[slot * ROWS + in_unit] = make_float2(ShiftOf(ref, scale), total);
       float4* const part_to = reinterpret_cast<float4*>(s.part_o) + slot * (DIM / 4) * ROWS + in_unit;
       const float inv = total == 0.f ? 0.f : 1.f / total;
       const int64_t at = (g.q.row0 + i) * a.ot + int64_t(h) * a.oh;

@@ -1,0 +1,104 @@
+"""The decoder operators at the edges of what they take, on the GPU: scores, values and steps of any size, bounds that tell the
+roundings of one type from another's."""
+import importlib
+import math
+
+import pytest
+import torch
+
+import decoder_bounds as B
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K(itex):
+    return importlib.import_module("itex_b200.kernels")
+
+
+@pytest.fixture(scope="module")
+def kv4(itex):
+    return importlib.import_module("itex_b200.kv4")
+
+
+def randn(seed, *shape, dtype=torch.float32):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda").to(dtype)
+
+
+def ints(v, dtype=torch.int32):
+    return torch.tensor(v, dtype=dtype, device="cuda")
+
+
+def table_of(pages, seed=5):
+    return torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).to(torch.int32)[None].cuda()
+
+
+# ------------------------------------------------------------------------------------------------------ scores of any size
+
+def far_scores(kv4, dim, kept, sign, seed=3):
+    """A cache whose keys are the same whole number in every channel, so that products with queries of ones are exact; the largest is
+    there three times (at the first, a middle and the last token), one less than it once."""
+    pages = -(-kept // 16)
+    cache = kv4.Kv4Cache.allocate(pages, 16, 1, dim, 32)
+    a = torch.randint(-1000, 1000, (kept,), generator=torch.Generator().manual_seed(seed)).double()
+    a[[0, kept // 2, kept - 1]] = 1001.0
+    a[kept // 3] = 1000.0
+    if sign < 0:      # all scores far below zero
+        a = a - 1024.0
+    table = table_of(pages)
+    j = torch.arange(kept, device="cuda")
+    slots = table[0].long()[j // 16] * 16 + j % 16
+    k = a.cuda().float()[:, None, None].expand(kept, 1, dim).contiguous()
+    cache.append(k, randn(seed, kept, 1, dim), slots)
+    assert torch.equal(cache.gather(slots, torch.float32)[0], k)
+    return cache, table
+
+
+def check_far_scores(kv4, dtype, dim, power, sign, new, kept=700):
+    cache, table = far_scores(kv4, dim, kept, sign)
+    q = torch.ones((new, 1, dim), device="cuda", dtype=dtype)
+    scale = 2.0 ** power / (1024.0 * dim)         # scores up to 2^power
+    out = cache.attention(q, table, ints([kept]), max_new=new, max_kept=kept, scale=scale)
+    r = B.attention(cache, q, table, [kept], [0, new], scale=scale)
+    # products are exact; scale * log2(e) is off by 2^-23 of itself, which enters through differences of scores that count (below 32);
+    # up to scores of 2^10 7 - maximum is rounded to 2^-14, twice
+    B.check(out, r, score=torch.full_like(r["dots"], 2.0 ** -13), context=(power, sign))
+
+
+POWERS = [3, 9, 10, 11, 16, 24, 27, 28, 29, 30, 34, 40, 60, 120]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", POWERS)
+@pytest.mark.parametrize("dim", [64, 256])
+def test_many_rows_with_scores_of_any_size(kv4, dtype, dim, power, sign):
+    """Scores far beyond what an fp32 exponent resolves: equal largest ones share the output, all others are nothing."""
+    check_far_scores(kv4, dtype, dim, power, sign, new=70)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_rows_with_queries_of_any_finite_value(kv4, dtype):
+    """Rows of a padded batch may hold anything: the largest numbers of the type, both signs, mixed with ordinary rows and with keys that
+    answer them with both signs.  Finite queries give finite shares, and the ordinary rows are right beside them."""
+    cache = kv4.Kv4Cache.allocate(12, 16, 2, 128, 64)
+    n, new = 190, 64
+    loud = 1.0 + 999.0 * (torch.arange(128, device="cuda") % 23 == 5)
+    cache.append(randn(1, n, 2, 128) * loud, randn(2, n, 2, 128), torch.arange(n, device="cuda"))
+    table = torch.arange(12, dtype=torch.int32, device="cuda")[None]
+    q = randn(3, new, 4, 128, dtype=dtype)
+    plain = cache.attention(q, table, ints([n]), max_new=new)
+    wild = q.clone()
+    size = torch.finfo(dtype).max * 2.0 ** -torch.arange(32, dtype=torch.float64, device="cuda")
+    wild[1::2] = torch.where(wild[1::2] > 0, size[:, None, None], -size[:, None, None]).to(dtype)
+    out = cache.attention(wild, table, ints([n]), max_new=new)
+    assert torch.isfinite(out).all()
+    v = cache.gather(torch.arange(n, device="cuda"), torch.float32)[1].abs().amax()
+    assert float(out.float().abs().max()) <= float(v) * (1 + 2.0 ** -7)
+    # a warp takes its maxima off either way for all its rows: ordinary rows agree to the roundings of both
+    r = B.attention(cache, q, table, [n], [0, new])
+    tol = B.tolerance(r, dtype)
+    for x in (plain, out):
+        assert ((x.double() - r["out"]).abs() <= tol)[0::2].all()
