@@ -43,7 +43,8 @@ constexpr int kLeastTiles = 8;                  // of a block's part, where ther
                                                 // tokens take 14.4 us on the device with 4 or 8, 14.6 with 16
 constexpr float kRescale = 4.f;                 // scores may pass the running maximum by 4 before it moves,
 constexpr float kShift = 2.f;                   // so weights are 2^(score - maximum - 2), at most 4
-constexpr float kNone = -3.0e38f;               // the maximum of no scores
+constexpr float kNone = -3.0e38f;               // the maximum of no scores or products
+constexpr float kFarthest = 2.9e38f;            // magnitude of a maximum of some scores at most
 
 struct StepArgs {
   AttnArgs a;
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
         up = fmaxf(up * __uint_as_float(uint32_t(e) << 23), 1e-37f);
       }
     }
-    up *= kUnit;
+    up = fminf(up * kUnit, -kNone);
     scale[nt] = Make2(__shfl_sync(0xffffffffu, up, (2 * c) * 4), __shfl_sync(0xffffffffu, up, (2 * c + 1) * 4));
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
 
   float o[NT][DIM / 16][4], middle[NT][NG][4];   // sums times 2^-24; the odd channels' (2, 3) are 16 times as large
   F2 zsum[NT][NG], l[NT];
-  F2 down[NT];                 // -(running maximum) - kShift
+  F2 under[NT];                // -(running maximum) of the products: taken off before they are scaled, which is exact for scores of any size
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
       zsum[nt][g] = Same2(0.f);
       middle[nt][g][0] = middle[nt][g][1] = middle[nt][g][2] = middle[nt][g][3] = 0.f;
     }
-    down[nt] = Same2(-kNone - kShift);
+    under[nt] = Same2(-kNone);
     l[nt] = Same2(0.f);
   }
 
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          d[h][nt][k] = Fma2(Make2(t[h][nt][2 * k], t[h][nt][2 * k + 1]), scale[nt], down[nt]);
+          d[h][nt][k] = Fma2(Add2(Make2(t[h][nt][2 * k], t[h][nt][2 * k + 1]), under[nt]), scale[nt], Same2(-kShift));
           over = fmaxf(over, fmaxf(X(d[h][nt][k]), Y(d[h][nt][k])));
         }
     if (__any_sync(0xffffffffu, over > kRescale - kShift)) {
@@ -508,18 +509,17 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
         float f[2], to[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float was = e ? Y(down[nt]) : X(down[nt]);
+          const float was = e ? Y(under[nt]) : X(under[nt]);
           float top = -INFINITY;
 #pragma unroll
           for (int h = 0; h < TT; ++h) top = fmaxf(top, fmaxf(t[h][nt][e], t[h][nt][e + 2]));
-          top *= e ? Y(scale[nt]) : X(scale[nt]);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          to[e] = fminf(was, -kShift - top);
-          f[e] = Exp2(to[e] - was);
+          to[e] = fminf(was, -top);
+          f[e] = Exp2((to[e] - was) * (e ? Y(scale[nt]) : X(scale[nt])));
         }
-        down[nt] = Make2(to[0], to[1]);
+        under[nt] = Make2(to[0], to[1]);
         const F2 f2 = Make2(f[0], f[1]);
         l[nt] = Mul2(l[nt], f2);
 #pragma unroll
@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
 #pragma unroll
         for (int h = 0; h < TT; ++h)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) d[h][nt][k] = Fma2(Make2(t[h][nt][2 * k], t[h][nt][2 * k + 1]), scale[nt], down[nt]);
+          for (int k = 0; k < 2; ++k)
+            d[h][nt][k] = Fma2(Add2(Make2(t[h][nt][2 * k], t[h][nt][2 * k + 1]), under[nt]), scale[nt], Same2(-kShift));
       }
     }
 #pragma unroll
@@ -632,7 +633,8 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
       float sum = e ? Y(l[nt]) : X(l[nt]);
       for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       const int row = warp * kRows + nt * 8 + 2 * c + e;
-      if (r == 0) s_ml[row] = make_float2(-kShift - (e ? Y(down[nt]) : X(down[nt])), sum);
+      const float top = -(e ? Y(under[nt]) : X(under[nt]));
+      if (r == 0) s_ml[row] = make_float2(top <= kNone ? kNone : fminf(fmaxf(top * (e ? Y(scale[nt]) : X(scale[nt])), -kFarthest), kFarthest), sum);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float z = e ? Y(zsum[nt][g]) : X(zsum[nt][g]);

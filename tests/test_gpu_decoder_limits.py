@@ -102,3 +102,26 @@ def test_many_rows_with_queries_of_any_finite_value(kv4, dtype):
     tol = B.tolerance(r, dtype)
     for x in (plain, out):
         assert ((x.double() - r["out"]).abs() <= tol)[0::2].all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", POWERS)
+@pytest.mark.parametrize("dim, new", [(64, 1), (128, 3), (256, 12)])
+def test_few_rows_with_scores_of_any_size(kv4, dtype, dim, new, power, sign):
+    check_far_scores(kv4, dtype, dim, power, sign, new)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_few_rows_with_queries_of_any_finite_value(kv4, dtype):
+    """As for many rows; each query row here is alone in its sequence."""
+    cache = kv4.Kv4Cache.allocate(12, 16, 2, 128, 64)
+    n, seqs = 190, 32
+    loud = 1.0 + 999.0 * (torch.arange(128, device="cuda") % 23 == 5)
+    cache.append(randn(1, n, 2, 128) * loud, randn(2, n, 2, 128), torch.arange(n, device="cuda"))
+    table = torch.arange(12, dtype=torch.int32, device="cuda")[None].expand(seqs, 12)
+    size = torch.finfo(dtype).max * 2.0 ** -torch.arange(seqs, dtype=torch.float64, device="cuda")
+    wild = torch.where(randn(3, seqs, 4, 128) > 0, size[:, None, None], -size[:, None, None]).to(dtype)
+    out = cache.attention(wild, table, ints([n] * seqs), max_new=1)
+    v = cache.gather(torch.arange(n, device="cuda"), torch.float32)[1].abs().amax()
+    assert torch.isfinite(out).all() and float(out.float().abs().max()) <= float(v) * (1 + 2.0 ** -7)
