@@ -12,8 +12,9 @@
 // (A constant's mantissa or-ed around the code, 1024 + c, costs as much, and taking the constant out again either three
 // digits, in sums over 128 Ki tokens, or an addition per two codes.)
 // q enters as half: for bf16 inputs each row is scaled by a power of two to at most 2, so that elements within 2^-14 of the
-// row's largest stay exact and the others are off by 2^-25 of it.  p is kept at most 4 (see kRescale), p * step is then
-// below 2^15.1 for every step a half can hold; small products lose bits only where they are 2^-11 of the largest or less.
+// row's largest stay exact and the others are off by 2^-25 of it.  p is kept at most 4 (see kRescale); p * step is a half
+// times a power of two per group of channels that follows the largest step the warp has seen (see kLimitField): steps of any size
+// fit, and a product is off by 2^-11 of itself or 2^-25 of the largest, 2^-40 of it where steps are alike.
 //
 // A warp owns tiles of 16 tokens and keeps its own running maximum, so warps meet only at the end of a block's part.  Both
 // products run on mma.m16n8k16 with the cache as the 16-row operand (16 tokens, 16 channels) and up to 8 query rows of the
@@ -27,7 +28,7 @@
 // which every block takes an equal, contiguous part; a (sequence, head) that ends inside a block's part is written by it, the
 // others are joined from at most one result per block by a second kernel.  (One block per 2048 tokens instead left a fifth of
 // the machine idle behind the longest contexts, and smaller chunks cost more at their ends than they evened out.)
-// Measured, single tokens, 32 / 8 heads of 128, groups of 64: 64 sequences up to 8192 (421 MB) 103 us, 4.1 TB/s over the call, 5.3
+// Measured, single tokens, 32 / 8 heads of 128, groups of 64: 64 sequences up to 8192 (421 MB) 104 us, 4.0 TB/s over the call, 5.3
 // while tiles stream; bound by issue slots (58 % busy) and the dependent steps of a tile with three warps per scheduler.
 #include <algorithm>
 
@@ -45,6 +46,14 @@ constexpr float kRescale = 4.f;                 // scores may pass the running m
 constexpr float kShift = 2.f;                   // so weights are 2^(score - maximum - 2), at most 4
 constexpr float kNone = -3.0e38f;               // the maximum of no scores or products
 constexpr float kFarthest = 2.9e38f;            // magnitude of a maximum of some scores at most
+
+// Limits of a group's steps, as the word (lo, step) of a step they stay below: 2^26 times a half's exponent bits, so with 2^E the
+// limit, its steps are multiplied by 2^(13 - E), products with weights up to 4 are below 2^15.  A step that reaches the limit moves
+// it to 8 to 16 times the largest step.
+constexpr uint32_t kLimitField = 26, kLimitMost = 31u << kLimitField;   // 2^16: no step reaches it
+__device__ __forceinline__ float LiftOf(uint32_t limit) { return __uint_as_float((155u << 23) - (limit >> 3)); }        // 2^(13 - E)
+__device__ __forceinline__ float UnitOf(uint32_t limit) { return __uint_as_float((123u << 23) + (limit >> 3)); }        // 2^24 / 2^(13 - E)
+__device__ __forceinline__ float Dropped(uint32_t from, uint32_t to) { return __uint_as_float((127u << 23) - ((to - from) >> 3)); }
 
 struct StepArgs {
   AttnArgs a;
@@ -411,9 +420,12 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
     }
   }
 
-  float o[NT][DIM / 16][4], middle[NT][NG][4];   // sums times 2^-24; the odd channels' (2, 3) are 16 times as large
+  float o[NT][DIM / 16][4], middle[NT][NG][4];   // sums times 2^-24 and the group's lift; the odd channels' (2, 3) are 16 times as large
   F2 zsum[NT][NG], l[NT];
+  uint32_t limit[NG];          // of the steps of values; the o and middle of a group are times LiftOf it
   F2 under[NT];                // -(running maximum) of the products: taken off before they are scaled, which is exact for scores of any size
+#pragma unroll
+  for (int g = 0; g < NG; ++g) limit[g] = 0u;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -432,6 +444,31 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
   const uint32_t value_at0 = kCodes + PieceAt<DIM>(2 * c, r * (GROUP / 16) / 16) + r * (GROUP / 16) % 16;
   const uint32_t value_at1 = kCodes + PieceAt<DIM>(2 * c + 1, r * (GROUP / 16) / 16) + r * (GROUP / 16) % 16;
   const uint32_t pars_at = 2 * kCodes + r * (NG * 4);
+  // Moves the limits of groups whose finite steps reach them.
+  auto raise = [&](auto part, const uint32_t st, const int j0, const uint32_t ok) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int x = 0; x < 2 * TT; ++x) {
+        const int in = (x >> 1) * kTile + (x & 1) * 8 + r, j = j0 + in;
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + st + (x >> 1) * kTileBytes + pars_at + kPars + (x & 1) * (8 * NG * 4) + 4 * g) & 0x7fffffffu;
+        if (w < kLimitMost && (!decltype(part)::value || (((ok >> in) & 1u) != 0u && j >= some_begin && j < some_end))) most = max(most, w);
+      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 4));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
+      const uint32_t to = most >= limit[g] ? min((most >> kLimitField) + 4u, 31u) << kLimitField : limit[g];
+      const float f = Dropped(limit[g], to);
+      limit[g] = to;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        middle[nt][g][0] *= f; middle[nt][g][1] *= f;
+#pragma unroll
+        for (int x = g * (GROUP / 16); x < (g + 1) * (GROUP / 16); ++x) { o[nt][x][0] *= f; o[nt][x][1] *= f; o[nt][x][2] *= f; o[nt][x][3] *= f; }
+      }
+    }
+  };
   auto compute = [&](auto part, const uint32_t st, const int j0, const uint32_t ok) {
     float t[TT][NT][4];
     uint32_t seen = 0xffffffffu;     // bit 16 h + 4 nt + 2 * (token r + 8) + column
@@ -545,6 +582,29 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
         l[nt] = Add2(l[nt], Add2(Make2(t[h][nt][0], t[h][nt][1]), Make2(t[h][nt][2], t[h][nt][3])));
       }
 
+    // ---- steps of values, of tokens that some row sees, against the limits
+    uint32_t most[NG];
+#pragma unroll
+    for (int h = 0; h < TT; ++h) {
+      bool in0 = true, in1 = true;
+      if constexpr (decltype(part)::value) {
+        const int j = j0 + h * kTile + r;
+        in0 = ((ok >> (16 * h + r)) & 1u) != 0u && j >= some_begin && j < some_end;
+        in1 = ((ok >> (16 * h + r + 8)) & 1u) != 0u && j + 8 >= some_begin && j + 8 < some_end;
+      }
+      uint32_t vp0[NG], vp1[NG];
+      Lds<NG>(vp0, smem + st + h * kTileBytes + pars_at + kPars);
+      Lds<NG>(vp1, smem + st + h * kTileBytes + pars_at + kPars + 8 * NG * 4);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t x = max(in0 ? vp0[g] : 0u, in1 ? vp1[g] : 0u);
+        most[g] = h == 0 ? x : max(most[g], x);
+      }
+    }
+    bool reached = false;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) reached = reached || most[g] >= limit[g];
+    if (__any_sync(0xffffffffu, reached)) raise(part, st, j0, ok);
 #pragma unroll
     for (int h = 0; h < TT; ++h) {
     const uint32_t sh = st + h * kTileBytes;
@@ -555,24 +615,27 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float2 p0 = Pair(vp0[g]), p1 = Pair(vp1[g]);
+      const float lift = LiftOf(limit[g]), step0 = p0.y * lift, step1 = p1.y * lift;
       uint32_t b0[NT], b1[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float mid[2] = {fmaf(8.f, p0.y, p0.x), fmaf(8.f, p1.y, p1.x)};
-        float w[4], z[2] = {X(zsum[nt][g]), Y(zsum[nt][g])};
+        float w[4];
+        if constexpr (decltype(part)::value) {  // an unseen row's lo and step may be anything
+          float z[2] = {X(zsum[nt][g]), Y(zsum[nt][g])};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float step = e < 2 ? p0.y : p1.y;
-          if constexpr (decltype(part)::value) {  // an unseen row's lo and step may be anything
+          for (int e = 0; e < 4; ++e) {
             const bool on = ((seen >> (16 * h + 4 * nt + e)) & 1u) != 0u;
-            w[e] = on ? t[h][nt][e] * step : 0.f;
+            w[e] = on ? t[h][nt][e] * (e < 2 ? step0 : step1) : 0.f;
             z[e & 1] = on ? fmaf(t[h][nt][e], mid[e >> 1], z[e & 1]) : z[e & 1];
-          } else {
-            w[e] = t[h][nt][e] * step;
-            z[e & 1] = fmaf(t[h][nt][e], mid[e >> 1], z[e & 1]);
           }
+          zsum[nt][g] = Make2(z[0], z[1]);
+        } else {
+          const F2 t0 = Make2(t[h][nt][0], t[h][nt][1]), t1 = Make2(t[h][nt][2], t[h][nt][3]);
+          const F2 w0 = Mul2(t0, Same2(step0)), w1 = Mul2(t1, Same2(step1));
+          w[0] = X(w0); w[1] = Y(w0); w[2] = X(w1); w[3] = Y(w1);
+          zsum[nt][g] = Fma2(t1, Same2(mid[1]), Fma2(t0, Same2(mid[0]), zsum[nt][g]));
         }
-        zsum[nt][g] = Make2(z[0], z[1]);
         b0[nt] = Transpose8x8(PackHalf(w[0], w[1]));
         b1[nt] = Transpose8x8(PackHalf(w[2], w[3]));
         const uint32_t eights[4] = {kMiddle, kMiddle, kMiddle, kMiddle};
@@ -637,6 +700,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
       if (r == 0) s_ml[row] = make_float2(top <= kNone ? kNone : fminf(fmaxf(top * (e ? Y(scale[nt]) : X(scale[nt])), -kFarthest), kFarthest), sum);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
+        const float unit = UnitOf(limit[g]);
         float z = e ? Y(zsum[nt][g]) : X(zsum[nt][g]);
         for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
 #pragma unroll
@@ -644,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
           const int d = g * GROUP + r * (GROUP / 8) + x * 2;
           const float *v = o[nt][g * (GROUP / 16) + x];
           *reinterpret_cast<float2*>(s_o + row * DIM + d) =
-              make_float2(fmaf(v[e] - middle[nt][g][e], kUnit, z), fmaf(fmaf(v[e + 2], 0.0625f, -middle[nt][g][e]), kUnit, z));
+              make_float2(fmaf(v[e] - middle[nt][g][e], unit, z), fmaf(fmaf(v[e + 2], 0.0625f, -middle[nt][g][e]), unit, z));
         }
       }
     }

@@ -125,3 +125,71 @@ def test_few_rows_with_queries_of_any_finite_value(kv4, dtype):
     out = cache.attention(wild, table, ints([n] * seqs), max_new=1)
     v = cache.gather(torch.arange(n, device="cuda"), torch.float32)[1].abs().amax()
     assert torch.isfinite(out).all() and float(out.float().abs().max()) <= float(v) * (1 + 2.0 ** -7)
+
+
+# ------------------------------------------------------------------------------------------------------ values of any size
+
+def check_values(kv4, dtype, dim, group, gains, new, seed=1, heads=4, keys=1.0, norm=None, **kw):
+    """Attention over values of standard deviation gains[token, channel]."""
+    n = gains.shape[0]
+    pages = -(-n // 16)
+    cache = kv4.Kv4Cache.allocate(pages, 16, 2, dim, group)
+    table = table_of(pages)
+    j = torch.arange(n, device="cuda")
+    slots = table[0].long()[j // 16] * 16 + j % 16
+    v = randn(seed + 1, n, 2, dim) * gains.cuda().float()[:, None, :]
+    cache.append(randn(seed, n, 2, dim) * keys, v.clamp(-60000.0, 60000.0), slots)
+    q = randn(seed + 2, new, heads, dim, dtype=dtype)
+    out = cache.attention(q, table, ints([n]), max_new=new, max_kept=n, **kw)
+    B.check(out, B.attention(cache, q, table, [n], [0, new], **kw), norm=norm, context=(dim, group, new))
+
+
+SHAPES = [(64, 64), (128, 32), (128, 128), (256, 64)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gain", [1.0, 1e-3, 3e-4, 1e-4, 1e-5, 300.0, 15000.0])
+@pytest.mark.parametrize("dim, group", SHAPES)
+@pytest.mark.parametrize("new", [1, 6])
+def test_few_rows_with_values_of_any_size(kv4, dtype, gain, dim, group, new):
+    """The product of a weight and a step keeps its digits whatever the steps are.  Below 0.1 a half's output has fewer digits of its own."""
+    norm = 2.1e-3 if dtype == torch.bfloat16 else (3.3e-4 if gain >= 1.0 else None)
+    check_values(kv4, dtype, dim, group, torch.full((417, dim), gain), new, norm=norm)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, group", SHAPES)
+@pytest.mark.parametrize("kind", ["rising", "falling", "groups", "one"])
+def test_few_rows_with_values_of_all_sizes_at_once(kv4, dtype, dim, group, kind):
+    n = 600
+    if kind == "groups":            # neighbouring groups of channels far apart
+        gains = (1e-5 * 10.0 ** (9.0 * torch.arange(dim, dtype=torch.float64).div(group, rounding_mode="floor") * group / dim)).expand(n, dim)
+    elif kind == "one":             # a single loud token late in the context
+        gains = torch.full((n, dim), 1e-3, dtype=torch.float64)
+        gains[500] = 5000.0
+    else:
+        gains = (10.0 ** torch.linspace(-5.0, 4.0, n, dtype=torch.float64))[:, None].expand(n, dim)
+        gains = gains.flip(0) if kind == "falling" else gains
+    for new in (1, 5):
+        check_values(kv4, dtype, dim, group, gains, new)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tail, power", [(3000, 20), (3000, 23), (50000, 17), (50000, 21)])
+def test_few_rows_with_one_token_above_a_long_tail(kv4, dtype, tail, power):
+    """One token's weight is 2^power times that of each other; their values are alike, so what is lost of each is lost of the sum."""
+    dim, n = 128, tail + 1
+    pages = -(-n // 16)
+    cache = kv4.Kv4Cache.allocate(pages, 16, 1, dim, 64)
+    slots = torch.arange(n, device="cuda")
+    k = torch.zeros((n, 1, dim), device="cuda")
+    k[7] = 1.0
+    v = 0.9 + 0.1 * torch.rand((n, 1, dim), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    v[..., 0::64], v[7] = -1.0, 0.0                       # ranges of 2 around values near their upper end; the one token's is zero
+    cache.append(k, v, slots)
+    q = torch.ones((1, 2, dim), dtype=dtype, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    scale = power * math.log(2.0) / dim
+    out = cache.attention(q, table, ints([n]), max_new=1, max_kept=n, scale=scale)
+    r = B.attention(cache, q, table, [n], [0, 1], scale=scale)
+    B.check(out, r, score=torch.full_like(r["dots"], power * 2.0 ** -21), context=(tail, power))
