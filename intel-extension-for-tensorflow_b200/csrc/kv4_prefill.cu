@@ -200,20 +200,25 @@ __device__ __forceinline__ uint32_t HalfFma2(uint32_t a, uint32_t b, uint32_t c)
 enum Part { kValue, kSum, kLeft };
 // For the codes at two nibbles of a word: the code's bits in the mantissa of 1024 (bits 0-3) or 64 (bits 4-7), the constant
 // subtracted (exact).
-template <int PART> __device__ __forceinline__ uint32_t Value2(uint32_t bits, uint32_t minus, uint32_t step2, uint32_t lo2) {
+template <int PART> __device__ __forceinline__ uint32_t Value2(uint32_t bits, uint32_t minus, uint32_t step2, uint32_t then2, uint32_t lo2) {
   const uint32_t c = HalfAdd2(bits, minus);
   if (PART == kValue) return HalfFma2(c, step2, lo2);
-  const uint32_t p = HalfMul2(c, step2), sum = HalfAdd2(p, lo2);
-  if (PART == kSum) return sum;
+  const uint32_t p = HalfMul2(c, step2);
+  if (PART == kSum) return HalfFma2(p, then2, lo2);
+  const uint32_t sum = HalfAdd2(p, lo2);
   // the product's rounding and the sum's, whichever of its terms is the larger
   const uint32_t of_p = HalfFma2(c, step2, p ^ 0x80008000u), lo_part = HalfSub2(sum, p), p_part = HalfSub2(sum, lo_part);
   return HalfAdd2(HalfAdd2(HalfSub2(p, p_part), HalfSub2(lo2, lo_part)), of_p);
 }
-template <int PART> __device__ __forceinline__ uint4 Values8(uint32_t w, uint32_t step2, uint32_t lo2) {
+template <int PART> __device__ __forceinline__ uint4 Values8(uint32_t w, uint32_t step2, uint32_t then2, uint32_t lo2) {
   const uint32_t u = w >> 8;
-  return make_uint4(Value2<PART>(AndOr(w, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2<PART>(AndOr(w, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2),
-                    Value2<PART>(AndOr(u, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, lo2), Value2<PART>(AndOr(u, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, lo2));
+  return make_uint4(Value2<PART>(AndOr(w, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, then2, lo2),
+                    Value2<PART>(AndOr(w, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, then2, lo2),
+                    Value2<PART>(AndOr(u, 0x000F000Fu, 0x64006400u), 0xE400E400u, step2, then2, lo2),
+                    Value2<PART>(AndOr(u, 0x00F000F0u, 0x54005400u), 0xD400D400u, step2, then2, lo2));
 }
+// |step| of 2048 or |lo| of 32768 and more: below, neither a rounded product (30720 at most) nor its sum with lo passes 65504.
+__device__ __forceinline__ bool Wide(uint32_t p) { return (p & 0x7fff0000u) >= 0x68000000u || (p & 0x7fffu) >= 0x7800u; }
 
 // Eight outputs, from the codes' order (0 4 1 5 2 6 3 7) back to the channels'.
 __device__ __forceinline__ void StoreOut8(const AttnArgs& a, int bf16, int64_t at, const float (&f)[8]) {
@@ -265,8 +270,14 @@ template <int DIM, int GROUP> struct Row {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int piece = i * 4 + k;
-        const uint32_t p = params[piece * 8 / GROUP];
-        *reinterpret_cast<uint4*>(tile + PieceAt(row, piece)) = Values8<PART>(w[k], __byte_perm(p, p, 0x3232), __byte_perm(p, p, 0x1010));
+        uint32_t p = params[piece * 8 / GROUP], then2 = 0x3c003c00u;   // 1
+        uint32_t step2 = __byte_perm(p, p, 0x3232), lo2 = __byte_perm(p, p, 0x1010);
+        if (PART != kValue && Wide(p)) {   // of a wide group the first part is the value, the second nothing
+          then2 = step2;
+          step2 = PART == kSum ? 0x3c003c00u : 0u;
+          lo2 = PART == kSum ? lo2 : 0u;
+        }
+        *reinterpret_cast<uint4*>(tile + PieceAt(row, piece)) = Values8<PART>(w[k], step2, then2, lo2);
       }
     }
   }

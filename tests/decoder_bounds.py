@@ -5,7 +5,8 @@ Every term is a worst case, U = half a step of a half, 2^-11, unless said otherw
   weights   a weight is a half.  The few-row kernel (at most 32 query rows of a key/value head) multiplies it with a value's
             distance from the middle of its group's range, lo + 8 step, the middle itself being added in fp32; the many-row
             kernel with the value.
-  values    a half, once, in the many-row kernel for bf16 queries; otherwise exact or off by U^2
+  values    a half, once, in the many-row kernel for bf16 queries and for groups whose products with codes could pass the largest half;
+            otherwise exact or off by U^2
   scores    keys as the values; queries are off by 2^-24 of the row's largest magnitude; sums in fp32.  A score's error enters
             a weight and the sum it is divided by.
   sums      fp32: a product of a weight with at most 15 + 8 steps, or with a value, is off by 2^-23 of the running sum at each
@@ -39,6 +40,7 @@ def attention(cache, q, table, kept, starts, causal=True, window=0, scale=None):
     share = q.shape[1] // cache.kv_heads
     r = {n: torch.zeros(q.shape, dtype=torch.float64, device=q.device) for n in ("out", "v", "off", "step")}
     r["dots"] = torch.zeros(q.shape[:2] + (1,), dtype=torch.float64, device=q.device)
+    r["wide"] = any(bool(((p[..., 1].abs() >= 2048) | (p[..., 0].abs() >= 32768)).any()) for p in (cache.k_params, cache.v_params))
     r["kept"], r["many"] = max(kept), max(b - a for a, b in zip(starts, starts[1:])) * share > 32
     for b, n_kept in enumerate(kept):
         a, e = starts[b], starts[b + 1]
@@ -63,7 +65,7 @@ def attention(cache, q, table, kept, starts, causal=True, window=0, scale=None):
 
 def tolerance(r, dtype, score=None):
     """Bound of each output's error; score: of the scores' errors where it is known better than from `dots`."""
-    one = r["many"] and dtype == torch.bfloat16        # keys and values as one half each
+    one = r["many"] and (dtype == torch.bfloat16 or r["wide"])        # keys and values as one half each
     if score is None:
         score = r["dots"] * ((HALF if one else 2.0 ** -21) + 2.0 ** -16)
     far = r["v"] if r["many"] else r["off"]

@@ -193,3 +193,21 @@ def test_few_rows_with_one_token_above_a_long_tail(kv4, dtype, tail, power):
     out = cache.attention(q, table, ints([n]), max_new=1, max_kept=n, scale=scale)
     r = B.attention(cache, q, table, [n], [0, 1], scale=scale)
     B.check(out, r, score=torch.full_like(r["dots"], power * 2.0 ** -21), context=(tail, power))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gain", [1.0, 1e-3, 3e-4, 1e-4, 1e-5, 300.0, 15000.0])
+@pytest.mark.parametrize("dim, group", SHAPES)
+def test_many_rows_with_values_of_any_size(kv4, dtype, gain, dim, group):
+    """Groups whose range is wider than the largest half are right too: each of their values is one."""
+    norm = 2.1e-3 if dtype == torch.bfloat16 else (3.3e-4 if 1.0 <= gain <= 300.0 else None)
+    check_values(kv4, dtype, dim, group, torch.full((417, dim), gain), 60, norm=norm)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, group", SHAPES)
+@pytest.mark.parametrize("new", [1, 60])
+def test_keys_of_wide_range(kv4, dtype, dim, group, new):
+    check_values(kv4, dtype, dim, group, torch.ones(300, dim), new, keys=12000.0, scale=1e-5)
+    gains = torch.where(torch.arange(dim) < group, 1e-3, 14000.0).double().expand(300, dim)
+    check_values(kv4, dtype, dim, group, gains, new)
