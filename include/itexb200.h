@@ -523,8 +523,11 @@ ITEXB_API int itexb_qk_norm_rope_grad(const itexb_qk_norm_rope_grad_params_t* p,
 /* A paged key/value cache held in 4 bits.  A row is one token of one key/value head: head_dim / 2 bytes of codes
  * (element 2i in the low, 2i + 1 in the high nibble of byte i) and, for every `group` consecutive elements, a pair of
  * halves (lo, step): element = lo + step * code.  Written as: lo = half(min), step = half(max(0, (max - lo) / 15)),
- * code = clamp(rne((x - lo) * (1 / step)), 0, 15) in fp32 (step 0: code 0); a group that holds a NaN or an infinity, or
- * whose lo or step does not fit a finite half, is stored as NaN.  Row `o` of page `g` for head `h` lies at
+ * code = clamp(rne((x - lo) * (1 / step)), 0, 15) in fp32 (step 0: code 0).  All values of a pair are halves' size: the
+ * step is the next lower half where lo + 15 step would round to an infinite one (enough for any group of finite halves); a
+ * group where it still does, or that holds a NaN or an infinity, is stored as NaN.  (What attention gives the rows that see a pair of a caller's own
+ * making which passes halves is not defined; the others keep theirs.)  Row `o` of page `g` for head
+ * `h` lies at
  *   codes  + g * codes_page_stride + h * codes_head_stride + o * codes_token_stride              (bytes, multiples of 16)
  *   params + g * params_page_stride + h * params_head_stride + o * params_token_stride           (pairs)
  * so pages may be laid out head by head or token by token.  A row's pairs must be aligned to their size, up to 16

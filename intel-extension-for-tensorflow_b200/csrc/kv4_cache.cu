@@ -2,6 +2,9 @@
 //
 //   lo = half(min of the group), step = half(max(0, (max - lo) / 15)), code = clamp(rne((x - lo) * (1 / step)), 0, 15)
 //
+// The step is the next lower half where lo + 15 step would not round to a finite half, which is enough for every group of
+// finite halves; where it still does not, or a group holds a NaN or an infinity, the pair is NaN.
+//
 // Both are bound by HBM (append, head_dim 128, groups of 64, bf16: 256 B in, 72 B out per row).  A thread owns 8
 // consecutive elements, which are one 32-bit word of codes; the 4 - 16 threads of a group exchange minimum and maximum
 // by shuffles, and the rotation of halves its partners.  Every step is a separately rounded fp32 operation on cosines and
@@ -17,6 +20,7 @@ namespace itexb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr float kPastHalf = 65520.f;   // rounds to an infinite half
 
 struct RowArgs {
   Kv4View c;
@@ -61,11 +65,15 @@ __device__ __forceinline__ uint32_t Quantize8(const float (&x)[8], int lanes, __
   }
   const __half lo = __float2half_rn(mn);
   const float lof = __half2float(lo);
-  const __half step = __float2half_rn(fmaxf((mx - lof) / 15.f, 0.f));
-  const float stepf = __half2float(step);
-  if (!isfinite(lof) || !isfinite(stepf)) {
-    *params = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
-    return 0u;
+  __half step = __float2half_rn(fmaxf((mx - lof) / 15.f, 0.f));
+  float stepf = __half2float(step);
+  if (!(fmaf(15.f, stepf, lof) < kPastHalf)) {   // rare; NaN comes here too
+    step = __ushort_as_half(uint16_t(__half_as_ushort(step) - 1));
+    stepf = __half2float(step);
+    if (!isfinite(lof) || !(fmaf(15.f, stepf, lof) < kPastHalf)) {
+      *params = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
+      return 0u;
+    }
   }
   *params = __halves2half2(lo, step);
   // All scaled by 1/16, which is exact: saturation to [0, 1] then leaves one bound to apply.  Adding 1.5 * 2^23 rounds to

@@ -25,8 +25,8 @@
 // Measured, 2048 new tokens after 8192 with 32 / 8 heads of 128: bf16 341 us, 0.91 PFLOP/s (softmax warps: 1650 clocks per 128
 // rows and 64 tokens, the products 1280 for both halves); half 752 us (0.82 PFLOP/s of products).  1024 tokens with head_dim
 // 256: 426 and 1540 us (one stage: the conversion is not hidden).  Six prompts up to 1900, window 1024: bf16 380, half 485 us.
-// Rows of the cache that no query may see are zeros here; a value group stored as NaN is zeros too and makes the rows that see
-// it NaN at the end.  Every wait is bounded.
+// Rows of the cache that no query may see are zeros here; a value group stored as NaN, or whose values pass the largest half, is
+// zeros too and makes the rows that see it NaN at the end.  Every wait is bounded.
 #include <algorithm>
 
 #include "kv4_attention.h"
@@ -282,7 +282,11 @@ template <int DIM, int GROUP> struct Row {
     }
   }
 };
-__device__ __forceinline__ bool NotFinite(uint32_t half2) { return (half2 & 0x7c00u) == 0x7c00u || (half2 & 0x7c000000u) == 0x7c000000u; }
+// A pair (lo, step) stored as NaN, or of values that are no finite halves: lo + 15 step or step is not one.
+__device__ __forceinline__ bool BadPair(uint32_t p) {
+  const uint32_t x = HalfFma2(__byte_perm(p, 0u, 0x4432), 0x4B804B80u, __byte_perm(p, p, 0x3210));   // (step, 0) * 15 + (lo, step)
+  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
+}
 
 struct Head {              // the unit that a block goes on with at its start, for the joining kernel
   int b, kvh, row0;        // b < 0: it starts with a unit of its own
@@ -323,7 +327,7 @@ struct Shared {   // behind the operand tiles
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], drained[2];
   uint32_t tmem;
   volatile int quit;
-  int nan_values;          // some value group is stored as NaN
+  int nan_values;          // some value group is a BadPair
   uint32_t there[4][4];    // of the last four tiles: tokens that exist, 32 per word
   int64_t sums[20], left;
   int b, rt, kvh, tile;    // where this block's part begins
@@ -732,7 +736,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
           const int col = int(QuickDiv(uint32_t(t), a.c.div_page)), page = __ldg(a.table + int64_t(g.b) * a.table_stride + col);
           if (page < 0 || page >= a.c.num_pages) continue;
           const __half2* at = a.c.v_params + int64_t(page) * a.c.pp + int64_t(g.kvh) * a.c.ph + int64_t(t - col * a.c.page_size) * a.c.pt;
-          for (int x = 0; x < NG; ++x) nan_groups |= uint32_t(NotFinite(__ldg(reinterpret_cast<const uint32_t*>(at + x)))) << x;
+          for (int x = 0; x < NG; ++x) nan_groups |= uint32_t(BadPair(__ldg(reinterpret_cast<const uint32_t*>(at + x)))) << x;
         }
       }
       __syncwarp();
@@ -820,7 +824,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
         bool bad = false;
 #pragma unroll
         for (int x = 0; x < NG; ++x)
-          if (NotFinite(row.params[x])) { row.params[x] = 0; bad = true; }
+          if (BadPair(row.params[x])) { row.params[x] = 0; bad = true; }
         if (bad) sh.nan_values = 1;
       } else {
         const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);

@@ -211,3 +211,63 @@ def test_keys_of_wide_range(kv4, dtype, dim, group, new):
     check_values(kv4, dtype, dim, group, torch.ones(300, dim), new, keys=12000.0, scale=1e-5)
     gains = torch.where(torch.arange(dim) < group, 1e-3, 14000.0).double().expand(300, dim)
     check_values(kv4, dtype, dim, group, gains, new)
+
+
+def test_append_of_ranges_at_the_end_of_halves(kv4):
+    """Any group of finite halves is stored as halves; what passes them by more than a lower step makes up for is stored as NaN."""
+    ends = [(-65504.0, 65504.0, True), (0.0, 65504.0, True), (-65504.0, 65519.0, True), (-65519.0, -65500.0, True), (65504.0, 65504.0, True), (60000.0, 65519.9, True),
+            (-40000.0, 40000.0, True),
+            (0.0, 65521.0, True),      # 65521 / 15 rounds to 4368, 15 times that to infinity; 15 * 4364 = 65460 does not
+            (-3.0, 70000.0, False), (0.0, 900000.0, False), (-65504.0, 900000.0, False), (-65521.0, 0.0, False),
+            (0.0, math.inf, False), (-math.inf, 0.0, False), (0.0, 3e38, False), (-3e38, 3e38, False)]
+    n, group = len(ends), 64
+    x = torch.rand((n, 1, 128), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    for i, (low, high, _) in enumerate(ends):
+        if math.isfinite(low) and math.isfinite(high):
+            x[i, 0, :group] = low + (high - low) * x[i, 0, :group].double()
+        x[i, 0, 11], x[i, 0, 42] = low, high
+    cache = kv4.Kv4Cache.allocate(2, 16, 1, 128, group)
+    slots = torch.arange(n, device="cuda")
+    cache.append(x, x, slots)
+    k, v = cache.gather(slots, torch.float32)
+    half = cache.gather(slots, torch.float16)[0]
+    assert torch.equal(k.view(torch.int32), v.view(torch.int32)) and torch.isfinite(k[..., group:]).all()
+    for i, (low, high, fits) in enumerate(ends):
+        got = k[i, 0, :group].double()
+        if not fits:
+            assert torch.isnan(got).all()
+            continue
+        assert torch.isfinite(half[i]).all()
+        lo, step = (float(cache.k_params[0, 0, i, 0, e]) for e in (0, 1))
+        assert lo + 15 * step < 65520
+        # half a step, and what the roundings of lo and step move: step down by up to one unit, 2^-10 of it, 15 times
+        off = (got - x[i, 0, :group].double()).abs().amax()
+        assert off <= step * (0.5 + 15 * 2.0 ** -10 + 2.0 ** -20) + abs(lo) * 2.0 ** -11
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [3, 60])
+@pytest.mark.parametrize("pair", [(60000.0, 3000.0), (65504.0, 65504.0), (-60000.0, 65504.0), (math.inf, 0.0), (0.0, math.inf), (math.nan, math.nan)])
+def test_pairs_past_halves_touch_no_other_row(kv4, dtype, new, pair):
+    n = 150
+    cache = kv4.Kv4Cache.allocate(10, 16, 2, 128, 64)
+    cache.append(randn(1, n, 2, 128), randn(2, n, 2, 128), torch.arange(n, device="cuda"))
+    q, table = randn(3, new, 4, 128, dtype=dtype), torch.arange(10, dtype=torch.int32, device="cuda")[None]
+    clean = cache.attention(q, table, ints([n]), max_new=new)
+    tol = B.tolerance(B.attention(cache, q, table, [n], [0, new]), dtype)
+    page, off = (n - 1) // 16, (n - 1) % 16
+    for side in (cache.v_params, cache.k_params):
+        side[page, 0, off, 1] = torch.tensor(pair, dtype=torch.float16, device="cuda")
+        out = cache.attention(q, table, ints([n]), max_new=new)
+        assert torch.equal(out[-1, 2:], clean[-1, 2:])
+        if new > 3:
+            assert torch.equal(out[:-1], clean[:-1])
+        else:
+            # The few-row kernel scales a group's steps by one power of two for all rows of a warp, so that the largest is at least 2^9: a
+            # product of a weight and a small step is then off by up to 2^-25 of its unit, 2^-34 of the largest step in the weights'
+            # unit, where a row's weights add up to 2^-2 at least.  At 8 steps' distance, over n tokens: n * step * 2^-29.  All rows of a
+            # warp move their maxima together, so that the weights' roundings differ too: each result is within `tolerance`.
+            s = pair[1] if math.isfinite(pair[1]) else 0.0
+            assert ((out.double() - clean.double()).abs() <= n * s * 2.0 ** -29 + 2.0 * tol)[:-1].all()
+        if math.isnan(pair[0]):
+            assert torch.isnan(out[-1, :2]).any(-1).all()
