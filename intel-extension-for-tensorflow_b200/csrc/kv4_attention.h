@@ -56,7 +56,11 @@ __device__ __forceinline__ int RowEnd(const AttnArgs& a, const Seq& s, int i) {
 
 __device__ __forceinline__ float Exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// Two elements of a query row (bf16 or half) times a power of two (or its negative, or zero), as halves.
+// Two elements of a query row (bf16 or half).
+__device__ __forceinline__ float2 QueryPair(uint32_t w, bool bf16) {
+  return bf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// The same times a power of two (or its negative, or zero), as halves; for halves it is 1.
 __device__ __forceinline__ uint32_t QueryHalf2(uint32_t w, bool bf16, float by) {
   uint32_t r;
   if (bf16) {
@@ -69,7 +73,7 @@ __device__ __forceinline__ uint32_t QueryHalf2(uint32_t w, bool bf16, float by) 
   }
   return r;
 }
-// The larger magnitudes of two pairs of bf16 (their bits order like their values; NaN counts as large).
+// The larger magnitudes of two pairs of bf16 or halves (their bits order like their values; NaN counts as large).
 __device__ __forceinline__ uint32_t MaxBits2(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
 
 size_t StepsWorkspace(const AttnArgs& a);

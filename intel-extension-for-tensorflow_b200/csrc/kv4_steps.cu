@@ -11,8 +11,8 @@
 // the rounding of (p step) is relative to what a value differs from it.
 // (A constant's mantissa or-ed around the code, 1024 + c, costs as much, and taking the constant out again either three
 // digits, in sums over 128 Ki tokens, or an addition per two codes.)
-// q enters as half: for bf16 inputs each row is scaled by a power of two to at most 2, so that elements within 2^-14 of the
-// row's largest stay exact and the others are off by 2^-25 of it.  p is kept at most 4 (see kRescale); p * step is a half
+// q enters as half: each row is scaled by a power of two to between 2^14 and 2^15, so that elements of 2^-24 of the row's largest
+// and more stay exact (odd channels, over 16) and the others are off by 2^-35 of it.  p is kept at most 4 (see kRescale); p * step is a half
 // times a power of two per group of channels that follows the largest step the warp has seen (see kLimitField): steps of any size
 // fit, and a product is off by 2^-11 of itself or 2^-25 of the largest, 2^-40 of it where steps are alike.
 //
@@ -375,15 +375,14 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
       }
     // q * down is exact but for underflow; scores are (codes' product) * up, up > 0
     float down = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f), up = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-    if (s.bf16) {
-      bits = MaxBits2(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
-      bits = MaxBits2(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-      const float most = __uint_as_float(max(bits << 16, bits & 0xffff0000u));
-      const int e = min(max(int(__float_as_uint(most) >> 23), 1), 253);
-      if (most > 0.f && most < INFINITY) {
-        down *= __uint_as_float(uint32_t(254 - e) << 23);
-        up = fmaxf(up * __uint_as_float(uint32_t(e) << 23), 1e-37f);
-      }
+    bits = MaxBits2(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+    bits = MaxBits2(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+    const float2 most2 = QueryPair(bits, s.bf16);
+    const float most = most2.x > most2.y ? most2.x : most2.y;      // NaN: nothing to scale
+    if (most > 0.f && most < INFINITY) {
+      const int e = max(int(__float_as_uint(most) >> 23), 15);
+      down *= __uint_as_float(uint32_t(268 - e) << 23);            // 2^(14 - exponent)
+      up = fmaxf(up * __uint_as_float(uint32_t(e - 14) << 23), 1e-37f);
     }
     up = fminf(up * kUnit, -kNone);
     scale[nt] = Make2(__shfl_sync(0xffffffffu, up, (2 * c) * 4), __shfl_sync(0xffffffffu, up, (2 * c + 1) * 4));
@@ -395,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, kShareSm<DIM, GROUP, NT>) StepsKerne
         Piece& y = x[g][w];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y.u[e] = QueryHalf2(y.u[e], s.bf16, down);
+          const float2 in = QueryPair(y.u[e], s.bf16);
+          y.u[e] = PackHalf(in.x * down, in.y * down);
           const float2 f = Pair(y.u[e]);
           sum += f.x + f.y;
           asm("mul.f16x2 %0, %0, %1;" : "+r"(y.u[e]) : "r"(0x2C003C00u));   // odd channels by 1/16

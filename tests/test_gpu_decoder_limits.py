@@ -271,3 +271,29 @@ def test_pairs_past_halves_touch_no_other_row(kv4, dtype, new, pair):
             assert ((out.double() - clean.double()).abs() <= n * s * 2.0 ** -29 + 2.0 * tol)[:-1].all()
         if math.isnan(pair[0]):
             assert torch.isnan(out[-1, :2]).any(-1).all()
+
+
+# ----------------------------------------------------------------------------------------------------- queries of any size
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-3, 1e-4, 2e-5, 1000.0])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_queries_of_any_size(kv4, dtype, size, dim, new):
+    """Small queries with a large scale: no channel loses digits."""
+    n = 260
+    cache = kv4.Kv4Cache.allocate(17, 16, 2, dim, 64)
+    slots = torch.arange(n, device="cuda")
+    cache.append(randn(1, n, 2, dim), randn(2, n, 2, dim), slots)
+    q = randn(3, new, 6, dim) * size
+    q[:, 1, :dim // 2] *= 64.0                   # rows with a loud and a quiet half
+    q[:, 3] *= 1.0 + 500.0 * (torch.arange(dim, device="cuda") % 16 == 0)
+    q[:, 1], q[:, 3] = q[:, 1] * 0.02, q[:, 3] * 0.004
+    q = q.to(dtype)
+    scale = 2.0 / (size * dim ** 0.5)
+    table = torch.arange(17, dtype=torch.int32, device="cuda")[None]
+    out = cache.attention(q, table, ints([n]), max_new=new, scale=scale)
+    r = B.attention(cache, q, table, [n], [0, new], scale=scale)
+    # fp32 sums of up to 256 products, 16 at a time, in two roundings each: 2^-19 of the sum of magnitudes
+    score = None if r["many"] else r["dots"] * 2.0 ** -18
+    B.check(out, r, score=score, norm=2.1e-3 if dtype == torch.bfloat16 and new < 60 else None, context=(size, dim, new))
