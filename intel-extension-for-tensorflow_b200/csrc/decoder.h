@@ -47,11 +47,13 @@ template <typename T> __device__ __forceinline__ uint32_t Pack16(float lo, float
 // VEC elements moved as one access of VEC * sizeof(T) bytes (1, 2, 4, 8 or 16); the caller guarantees the alignment.
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
 template <typename T, int VEC> __device__ __forceinline__ void LoadVec(const T* p, float (&f)[VEC]) {
+  static_assert(sizeof(T) * VEC <= 16, "no wider access than the alignment that is asked of tensors");
   const Vec<T, VEC> x = *reinterpret_cast<const Vec<T, VEC>*>(p);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) f[i] = ToFloat(x.v[i]);
 }
 template <typename T, int VEC> __device__ __forceinline__ void StoreVec(T* p, const float (&f)[VEC]) {
+  static_assert(sizeof(T) * VEC <= 16, "no wider access than the alignment that is asked of tensors");
   union { Vec<T, VEC> x; uint32_t w[(sizeof(T) * VEC + 3) / 4]; } u;
   if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
 #pragma unroll

@@ -784,7 +784,14 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) JoinKernel(cons
   for (int i = warp; i < parts; i += WARPS) {
     const float2 ml = s.part_ml[at(i)];
     float v[E];
-    LoadVec<float, E>(s.part_o + at(i) * DIM + lane * E, v);
+    constexpr int kPiece = E < 4 ? E : 4;
+#pragma unroll
+    for (int e = 0; e < E; e += kPiece) {
+      float x[kPiece];
+      LoadVec<float, kPiece>(s.part_o + at(i) * DIM + lane * E + e, x);
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) v[e + k] = x[k];
+    }
     const float f = PartWeight(ml.x, ml.y, top);
     sum = fmaf(ml.y, f, sum);
 #pragma unroll

@@ -297,3 +297,25 @@ def test_queries_of_any_size(kv4, dtype, size, dim, new):
     # fp32 sums of up to 256 products, 16 at a time, in two roundings each: 2^-19 of the sum of magnitudes
     score = None if r["many"] else r["dots"] * 2.0 ** -18
     B.check(out, r, score=score, norm=2.1e-3 if dtype == torch.bfloat16 and new < 60 else None, context=(size, dim, new))
+
+
+# ------------------------------------------------------------------------------------------------------------- the boundary
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_workspace_aligned_to_sixteen_bytes_and_no_more(kv4, dim, new):
+    """One sequence that many blocks share, so that their results go through the workspace; nothing before or behind it is written."""
+    n = 5000
+    cache = kv4.Kv4Cache.allocate(320, 16, 2, dim, 32)
+    cache.append(randn(1, n, 2, dim), randn(2, n, 2, dim), torch.arange(n, device="cuda"))
+    q, table = randn(3, new, 4, dim, dtype=torch.bfloat16), torch.arange(320, dtype=torch.int32, device="cuda")[None]
+    want = cache.attention(q, table, ints([n]), max_new=new)
+    with pytest.raises(RuntimeError, match="workspace of") as refusal:
+        cache.attention(q, table, ints([n]), max_new=new, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    need = int(str(refusal.value).split("workspace of ")[1].split()[0])
+    hold = torch.full((need + 128,), 0x5A, dtype=torch.uint8, device="cuda")
+    at = (16 - hold.data_ptr()) % 32                 # 16 bytes past a multiple of 32
+    got = cache.attention(q, table, ints([n]), max_new=new, workspace=hold[at:at + need])
+    assert torch.equal(got, want) and (hold[:at] == 0x5A).all() and (hold[at + need:] == 0x5A).all()
+    with pytest.raises(RuntimeError, match="16-byte aligned workspace"):
+        cache.attention(q, table, ints([n]), max_new=new, workspace=hold[at + 8:at + 8 + need])
