@@ -327,7 +327,7 @@ struct Shared {   // behind the operand tiles
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], drained[2];
   uint32_t tmem;
   volatile int quit;
-  int nan_values;          // some value group is a BadPair
+  int bad_tile;            // the block's last tile so far with a value group that is a BadPair, -1: none
   uint32_t there[4][4];    // of the last four tiles: tokens that exist, 32 per word
   int64_t sums[20], left;
   int b, rt, kvh, tile;    // where this block's part begins
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
       }
     }
     sh.quit = 0;
-    sh.nan_values = 0;
+    sh.bad_tile = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
     const int m = (warp - 4) >> 2, in_half = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_m = tmem + lanes + m * 128, o_at = tmem + lanes + H::kOColumn + m * DIM;
-    uint32_t parts = 0, t4 = 0;   // 64 tokens each: of this half; all tiles of the block
+    uint32_t parts = 0, t4 = 0;   // 64 tokens each: of this half; all tiles of the block so far
     bool ok = true;
     while (ok && next_segment()) {
       const int n = g.tile1 - g.tile0;
@@ -731,12 +731,26 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
       if (!ok) break;
       FenceAfter();
       uint32_t nan_groups = 0;
-      if (sh.nan_values != 0) {   // rare: find the value groups that are NaN among the tokens this row sees
-        for (int t = lo; t < hi; ++t) {
-          const int col = int(QuickDiv(uint32_t(t), a.c.div_page)), page = __ldg(a.table + int64_t(g.b) * a.table_stride + col);
-          if (page < 0 || page >= a.c.num_pages) continue;
-          const __half2* at = a.c.v_params + int64_t(page) * a.c.pp + int64_t(g.kvh) * a.c.ph + int64_t(t - col * a.c.page_size) * a.c.pt;
-          for (int x = 0; x < NG; ++x) nan_groups |= uint32_t(BadPair(__ldg(reinterpret_cast<const uint32_t*>(at + x)))) << x;
+      // Rare: find the value groups that are NaN among this part's tokens, a lane looking at one of 32, and keep those that this row
+      // sees.  (The tile may be of a segment behind this one, whose conversion is ahead: then there are none to find.)
+      if (__any_sync(0xffffffffu, *const_cast<volatile int*>(&sh.bad_tile) >= int(t4) - n)) {
+        const int from = max(g.u.some_begin, g.u.begin + g.tile0 * kTokens<SPLIT>), to = min(g.u.end, g.u.begin + g.tile1 * kTokens<SPLIT>);
+#pragma unroll 1
+        for (int t0 = from; t0 < to; t0 += 32) {
+          const int t = t0 + lane;
+          uint32_t bad = 0;
+          if (t < to) {
+            const int col = int(QuickDiv(uint32_t(t), a.c.div_page)), page = __ldg(a.table + int64_t(g.b) * a.table_stride + col);
+            if (page >= 0 && page < a.c.num_pages) {
+              const __half2* at = a.c.v_params + int64_t(page) * a.c.pp + int64_t(g.kvh) * a.c.ph + int64_t(t - col * a.c.page_size) * a.c.pt;
+              for (int x = 0; x < NG; ++x) bad |= uint32_t(BadPair(__ldg(reinterpret_cast<const uint32_t*>(at + x)))) << x;
+            }
+          }
+          for (uint32_t left = __ballot_sync(0xffffffffu, bad != 0u); left != 0u; left &= left - 1u) {
+            const int k = __ffs(int(left)) - 1;
+            const uint32_t of_k = __shfl_sync(0xffffffffu, bad, k);
+            if (t0 + k >= lo && t0 + k < hi) nan_groups |= of_k;
+          }
         }
       }
       __syncwarp();
@@ -825,7 +839,7 @@ __global__ void __launch_bounds__(Shape<DIM>::kThreads, 1) PrefillKernel(const _
 #pragma unroll
         for (int x = 0; x < NG; ++x)
           if (BadPair(row.params[x])) { row.params[x] = 0; bad = true; }
-        if (bad) sh.nan_values = 1;
+        if (bad) atomicMax(&sh.bad_tile, int(n));
       } else {
         const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
         if (lane == 0) sh.there[n & 3][w] = there;

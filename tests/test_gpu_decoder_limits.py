@@ -319,3 +319,61 @@ def test_a_workspace_aligned_to_sixteen_bytes_and_no_more(kv4, dim, new):
     assert torch.equal(got, want) and (hold[:at] == 0x5A).all() and (hold[at + need:] == 0x5A).all()
     with pytest.raises(RuntimeError, match="16-byte aligned workspace"):
         cache.attention(q, table, ints([n]), max_new=new, workspace=hold[at + 8:at + 8 + need])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, group", [(64, 32), (128, 64), (256, 128)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_value_groups_stored_as_nan_reach_the_rows_that_see_them_and_no_other(kv4, dtype, dim, group, window):
+    """Many rows, several sequences and heads, units that blocks share: NaN exactly where a visible token's group is NaN."""
+    new, kept, share, kvh, page = [300, 5, 129], [900, 40, 129], 2, 2, 16
+    need = [-(-n // page) for n in kept]
+    cache = kv4.Kv4Cache.allocate(sum(need), page, kvh, dim, group)
+    rows = sum(need) * page
+    cache.append(randn(1, rows, kvh, dim), randn(2, rows, kvh, dim), torch.arange(rows, device="cuda"))
+    table = torch.full((3, max(need)), -1, dtype=torch.int32)
+    for b in range(3):
+        table[b, :need[b]] = torch.arange(sum(need[:b]), sum(need[:b + 1]), dtype=torch.int32)
+    starts = [0, 300, 305, 434]
+    q = randn(3, starts[-1], kvh * share, dim, dtype=dtype)
+
+    def go():
+        return cache.attention(q, table.cuda(), ints(kept), q_starts=ints(starts), max_new=300, max_kept=900, window=window)
+
+    clean = go()
+    assert torch.isfinite(clean).all()
+    expect = torch.zeros(clean.shape, dtype=torch.bool, device="cuda")
+    for b, tok, h, g in [(0, 0, 0, 0), (0, 613, 1, 1), (0, 613, 1, 0), (0, 899, 0, 1), (1, 38, 0, 1), (2, 64, 1, 0), (2, 127, 1, 1)]:
+        cache.v_params[int(table[b, tok // page]), h, tok % page, g] = math.nan
+        place = torch.arange(new[b], device="cuda") + kept[b] - new[b]
+        sees = (place >= tok) & ((place - window < tok) if window else True)
+        expect[starts[b]:starts[b + 1], h * share:(h + 1) * share, g * group:(g + 1) * group] |= sees[:, None, None]
+    out = go()
+    assert torch.equal(torch.isnan(out), expect) and torch.equal(out[~expect], clean[~expect])
+
+
+def test_a_value_group_stored_as_nan_costs_little(kv4):
+    """One NaN group at the start of a long list of sequences: the other segments of a block do not look for it."""
+    seqs, new, kept = 64, 64, 2048
+    cache = kv4.Kv4Cache.allocate(seqs * kept // 64, 64, 8, 128, 64)
+    rows = seqs * kept
+    for at in range(0, rows, 1 << 14):
+        cache.append(randn(1, 1 << 14, 8, 128, dtype=torch.bfloat16), randn(2, 1 << 14, 8, 128, dtype=torch.bfloat16), torch.arange(at, at + (1 << 14), device="cuda"))
+    table = torch.arange(rows // 64, dtype=torch.int32, device="cuda").view(seqs, -1)
+    q = randn(3, seqs * new, 32, 128, dtype=torch.bfloat16)
+
+    def time():
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        best = math.inf
+        for _ in range(6):
+            a.record()
+            cache.attention(q, table, ints([kept] * seqs), max_new=new, max_kept=kept)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    clean = time()
+    for b in range(seqs):                # a head's first segment in each block or so
+        cache.v_params[int(table[b, 3]), 0, 5, 0] = math.nan
+    assert time() <= 2.0 * clean
