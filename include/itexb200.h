@@ -507,7 +507,8 @@ ITEXB_API int itexb_qk_norm_rope(const itexb_qk_norm_rope_params_t* p, itexb_str
 
 /* Gradient of itexb_qk_norm_rope.  n describes the forward call (r.q, r.k its inputs); n.r.q_out / n.r.k_out receive the
  * inputs' gradients, q_grad / k_grad are the outputs' gradients (dtype n.r.dtype), d_q_weight / d_k_weight the weights'
- * gradients [head_dim] in w_dtype, summed over tokens and heads in a fixed order (equal calls give equal bits).
+ * gradients [head_dim] in w_dtype, summed over tokens and heads in a fixed order (equal calls give equal bits); zeros without
+ * tokens, or for d_k_weight (then optional) without key heads.
  * workspace: device scratch of itexb_qk_norm_rope_grad_workspace_bytes(). */
 typedef struct itexb_qk_norm_rope_grad_params {
   itexb_qk_norm_rope_params_t n;

@@ -598,13 +598,15 @@ extern "C" int itexb_qk_norm_rope_grad(const itexb_qk_norm_rope_grad_params_t* p
   ITEXB_RETURN_IF_ERROR(CheckNorm(&n, what));
   ITEXB_REQUIRE(p->d_q_weight && (n.r.k_heads == 0 || p->d_k_weight), ITEXB_INVALID_ARGUMENT, "%s: NULL weight gradient", what);
   cudaStream_t st = AsCuda(stream);
-  if (n.r.tokens == 0) {  // sums over nothing
-    const size_t bytes = size_t(n.r.head_dim) * DtypeSize(n.w_dtype);
+  ITEXB_REQUIRE(n.r.tokens == 0 || (p->q_grad && (n.r.k_heads == 0 || p->k_grad) && p->workspace), ITEXB_INVALID_ARGUMENT,
+                "%s: NULL gradient or workspace", what);
+  // sums over nothing
+  const size_t bytes = size_t(n.r.head_dim) * DtypeSize(n.w_dtype);
+  if (p->d_k_weight && (n.r.tokens == 0 || n.r.k_heads == 0)) ITEXB_CUDA(cudaMemsetAsync(p->d_k_weight, 0, bytes, st));
+  if (n.r.tokens == 0) {
     ITEXB_CUDA(cudaMemsetAsync(p->d_q_weight, 0, bytes, st));
-    if (n.r.k_heads > 0) ITEXB_CUDA(cudaMemsetAsync(p->d_k_weight, 0, bytes, st));
     return ITEXB_OK;
   }
-  ITEXB_REQUIRE(p->q_grad && (n.r.k_heads == 0 || p->k_grad) && p->workspace, ITEXB_INVALID_ARGUMENT, "%s: NULL gradient or workspace", what);
   RopeArgs a{};
   Fill(a, &n.r);
   a.sin_sign = -1.f;  // the rotation's transpose

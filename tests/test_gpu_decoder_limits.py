@@ -377,3 +377,19 @@ def test_a_value_group_stored_as_nan_costs_little(kv4):
     for b in range(seqs):                # a head's first segment in each block or so
         cache.v_params[int(table[b, 3]), 0, 5, 0] = math.nan
     assert time() <= 2.0 * clean
+
+
+@pytest.mark.parametrize("tokens", [0, 7])
+def test_the_gradient_of_no_key_heads_is_zero(K, tokens):
+    """Every output of the call is written, the weights' gradients of heads that are not there too."""
+    q, g = randn(1, tokens, 2, 64), randn(2, tokens, 2, 64)
+    none = torch.empty((tokens, 0, 64), device="cuda")
+    w = torch.ones(64, device="cuda")
+    pos, freq = torch.arange(tokens, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
+    marks = [torch.full((64,), 7.0, device="cuda") for _ in range(64)]      # what the allocator hands out again
+    torch.cuda.synchronize()
+    del marks
+    dq, dk, dwq, dwk = K.qk_norm_rope_backward(g, none, q, none, w, w, pos, freq)
+    assert dk.shape == none.shape and torch.equal(dwk, torch.zeros_like(w))
+    both = K.qk_norm_rope_backward(g, g, q, q, w, w, pos, freq)
+    assert torch.equal(dq, both[0]) and torch.equal(dwq, both[2])
