@@ -586,7 +586,7 @@ ITEXB_API int itexb_kv4_gather(const itexb_kv4_gather_params_t* p, itexb_stream_
  * j % page_size of page block_table[b * table_stride + j / page_size].
  * new_b = q_starts[b + 1] - q_starts[b], its rows q_starts[b] .. of q and out; q_starts == NULL: new_b = max_new, rows
  * b * max_new ...  Rows of `out` that belong to no sequence are left as they were.  max_new and max_kept are upper bounds
- * the launch is sized by; a sequence beyond them (or beyond the table) is cut there and reported, a page outside the cache
+ * the launch is sized by; a sequence beyond them (or beyond the table, or 2^31 - 4097 tokens) is cut there and reported, a page outside the cache
  * is not read: its rows count as not visible, and it is reported.
  * workspace: device scratch of itexb_kv4_attention_workspace_bytes() for the same params (it depends on shapes and bounds
  * only).  Calls that may run at the same time need workspaces of their own. */

@@ -21,6 +21,8 @@ struct AttnArgs {
   FastDiv div_share;
 };
 
+constexpr int kMostKept = 0x7fffffff - 4096;   // tokens of a sequence
+
 struct Seq { int64_t row0; int nnew, kept; };
 
 // Lengths of sequence b, cut to the launch's bounds; what is cut off is reported.
@@ -32,7 +34,8 @@ __device__ __forceinline__ Seq SeqOf(const AttnArgs& a, int b, bool report) {
     s.row0 = __ldg(a.q_starts + b);
     n = int64_t(__ldg(a.q_starts + b + 1)) - s.row0;
   }
-  const int64_t most = min(int64_t(a.max_kept), int64_t(a.table_cols) * a.c.page_size);
+  // tiles are rounded up in 32 bits behind the last token
+  const int64_t most = min(min(int64_t(a.max_kept), int64_t(a.table_cols) * a.c.page_size), int64_t(kMostKept));
   int64_t kept = __ldg(a.kept + b);
   const bool bad = n < 0 || n > a.max_new || s.row0 < 0 || s.row0 + n > a.total_rows || kept < 0 || kept > most;
   if (bad) {

@@ -393,3 +393,24 @@ def test_the_gradient_of_no_key_heads_is_zero(K, tokens):
     assert dk.shape == none.shape and torch.equal(dwk, torch.zeros_like(w))
     both = K.qk_norm_rope_backward(g, g, q, q, w, w, pos, freq)
     assert torch.equal(dq, both[0]) and torch.equal(dwq, both[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("page", [256, 20])
+@pytest.mark.parametrize("new", [1, 40])
+def test_contexts_up_to_the_last_length(kv4, dtype, page, new):
+    """Places of tokens near 2^31, through a table that repeats its pages; longer contexts are cut to the longest and reported."""
+    cache = kv4.Kv4Cache.allocate(8, page, 2, 128, 64)
+    n = 8 * page
+    cache.append(randn(1, n, 2, 128), randn(2, n, 2, 128), torch.arange(n, device="cuda"))
+    longest = 2 ** 31 - 4097
+    table = (torch.arange(-(-2 ** 31 // page), dtype=torch.int32, device="cuda") % 8)[None]
+    q = randn(3, new, 4, 128, dtype=dtype)
+    for kept, told in ((longest, False), (longest - 9, False), (longest + 1, True), (2 ** 31 - 1, True)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = cache.attention(q, table, ints([kept]), max_new=new, window=100, status=status)
+        assert int(status) == (kv4.STATUS_BAD_INDEX if told else 0)
+        # the same rows in a context of as many periods as a window needs
+        short = min(kept, longest) % (16 * n) + 16 * n
+        r = B.attention(cache, q, table, [short], [0, new], window=100)
+        B.check(out, r, context=kept)
