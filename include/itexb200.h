@@ -596,7 +596,7 @@ typedef struct itexb_kv4_attention_params {
   int32_t num_seqs, q_heads;
   int32_t causal, window;
   int32_t max_new, max_kept;
-  float scale;
+  float scale;                   /* finite, of any sign */
   int64_t total_rows;            /* rows of q and out */
   const void* q; int64_t q_token_stride, q_head_stride;
   void* out;     int64_t out_token_stride, out_head_stride;

@@ -1,4 +1,6 @@
 // itexb_kv4_attention: argument checks and the choice of kernel.
+#include <cmath>
+
 #include "kv4_attention.h"
 
 using namespace itexb;
@@ -33,6 +35,7 @@ int CheckAttention(const itexb_kv4_attention_params_t* p, AttnArgs* a) {
   a->causal = p->causal != 0; a->window = p->window; a->max_new = p->max_new; a->max_kept = p->max_kept;
   a->q_aligned = reinterpret_cast<uintptr_t>(p->q) % 16 == 0 && p->q_token_stride % 8 == 0 && p->q_head_stride % 8 == 0;
   a->scale_log2 = p->scale * 1.4426950408889634f;
+  ITEXB_REQUIRE(std::isfinite(a->scale_log2), ITEXB_INVALID_ARGUMENT, "%s: scale must be finite, got %g", what, double(p->scale));
   a->div_share = MakeFastDiv(uint32_t(a->share));
   return ITEXB_OK;
 }
