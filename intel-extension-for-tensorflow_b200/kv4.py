@@ -31,7 +31,8 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, trained
       "linear"    all frequencies divided by factor
       "base"      base raised so that the slowest pair is divided by factor, the fastest kept
       "by_parts"  pairs that turn fewer than `slow` times over `trained` positions divided by factor, those that turn more
-                  than `fast` times kept, a linear ramp over the pair's index between; mscale = 0.1 ln(factor) + 1
+                  than `fast` times kept, a linear ramp over the pair's index between (its ends on whole indexes, the upper one
+                  behind the last pair where that turns more than `slow` times); mscale = 0.1 ln(factor) + 1
       "by_length" the same two ends with the ramp linear in the number of turns; mscale = 1"""
     if rotary_dim < 2 or rotary_dim % 2 != 0:
         raise ValueError("rotary_dim must be even and positive, got %r" % (rotary_dim,))
@@ -51,7 +52,7 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, trained
             raise ValueError("fast > slow > 0 and trained > 0 are needed, got %r, %r, %r" % (fast, slow, trained))
         if scaling == "by_parts":
             at = [rotary_dim * math.log(trained / (turns * 2.0 * math.pi)) / (2.0 * math.log(base)) for turns in (fast, slow)]
-            low, high = max(0.0, math.floor(at[0])), min(rotary_dim / 2.0 - 1.0, math.ceil(at[1]))
+            low, high = max(0.0, math.floor(at[0])), min(rotary_dim - 1.0, math.ceil(at[1]))
             stretch = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
             mscale = 0.1 * math.log(factor) + 1.0
         else:
