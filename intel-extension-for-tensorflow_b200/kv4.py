@@ -67,7 +67,8 @@ class Kv4Cache:
     """The cache's four tensors: codes uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16
     [pages, kv_heads, page_size, head_dim / group, 2], for keys and for values.  The first three dimensions may have any
     strides (a token-major cache is passed as its transpose(1, 2)); keys and values share them.  The object holds no state
-    besides the tensors: which page belongs to which sequence is the caller's block table."""
+    besides the tensors, which are its own for good (k_codes, k_params, v_codes, v_params; read-only attributes, as are the sizes):
+    which page belongs to which sequence is the caller's block table."""
 
     def __init__(self, k_codes, k_params, v_codes, v_params):
         self.dev = K.device_of(k_codes, k_params, v_codes, v_params)
@@ -82,10 +83,17 @@ class Kv4Cache:
         if ps[:3] != cs[:3] or ps[4] != 2 or groups < 1 or ct[3] != 1 or pt[4] != 1 or (groups > 1 and pt[3] != 2) or (pt[0] | pt[1] | pt[2]) & 1 \
                 or 2 * row % groups != 0:
             raise ValueError("codes %s and params %s do not describe one cache with dense rows" % (tuple(cs), tuple(ps)))
-        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.group = pages, heads, page_size, 2 * row, 2 * row // groups
-        self._c = (pages, page_size, heads, 2 * row, self.group, 0, k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(),
-                   ct[0], ct[1], ct[2], pt[0] // 2, pt[1] // 2, pt[2] // 2)
+        self._tensors = (k_codes, k_params, v_codes, v_params)
+        self._sizes = (pages, page_size, heads, 2 * row, 2 * row // groups, 0)
+        self._strides = (ct[0], ct[1], ct[2], pt[0] // 2, pt[1] // 2, pt[2] // 2)
+
+    k_codes, k_params, v_codes, v_params = (property(lambda self, i=i: self._tensors[i]) for i in range(4))
+    num_pages, page_size, kv_heads, head_dim, group = (property(lambda self, i=i: self._sizes[i]) for i in range(5))
+
+    def _cache(self):
+        """The C struct's fields.  Addresses are those of now: a tensor's storage may be replaced, its sizes and strides may not."""
+        kc, kp, vc, vp = self._tensors
+        return (*self._sizes, kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(), *self._strides)
 
     @classmethod
     def allocate(cls, num_pages, page_size, kv_heads, head_dim, group=64, device="cuda", token_major=False):
@@ -116,7 +124,7 @@ class Kv4Cache:
         if positions is not None:
             pos, pdt = K._vector(positions, "positions", K._INDEX_DT, n), K._INDEX_DT[positions.dtype]
             freq, rot = K._vector(inv_freq, "inv_freq", K._FLOAT64), 2 * inv_freq.shape[0]
-        K.launch(L.load().itexb_kv4_append, L.pack_kv4_append(*self._c, n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
+        K.launch(L.load().itexb_kv4_append, L.pack_kv4_append(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
                                                               int(interleaved), mscale, _status(status)), self.dev)
 
     def gather(self, slots, dtype=torch.bfloat16, *, out_k=None, out_v=None, status=None):
@@ -129,7 +137,7 @@ class Kv4Cache:
         n, kp, vp = self._kv(k, v, "gather")
         if n != tokens:
             raise ValueError("gather: %d rows for %d slots" % (n, tokens))
-        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._c, n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status)),
+        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status)),
                  self.dev)
         return k, v
 
@@ -167,7 +175,7 @@ class Kv4Cache:
             op = K._rows(out, "out")
         else:
             op = K._rows(out, "out", q)
-        args = (*self._c, K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
+        args = (*self._cache(), K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
                 rows, *qp, *op, block_table.data_ptr(), tst[0], cols, kp, sp, _status(status))
         lib = L.load()
         if workspace is None:

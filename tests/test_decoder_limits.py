@@ -45,3 +45,10 @@ def test_by_parts_stretches_pairs_by_their_turns(mods, trained, base):
             assert math.isclose(f[i].item(), plain / factor, rel_tol=1e-12)
         if turns > slow and low < i < high:
             assert plain / factor < f[i].item() < plain
+
+
+@pytest.mark.parametrize("name", ["k_codes", "k_params", "v_codes", "v_params", "num_pages", "page_size", "kv_heads", "head_dim", "group"])
+def test_a_cache_keeps_its_tensors_and_sizes(mods, name):
+    cache = object.__new__(mods[3].Kv4Cache)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, torch.zeros(4))

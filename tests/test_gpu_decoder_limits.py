@@ -414,3 +414,21 @@ def test_contexts_up_to_the_last_length(kv4, dtype, page, new):
         short = min(kept, longest) % (16 * n) + 16 * n
         r = B.attention(cache, q, table, [short], [0, new], window=100)
         B.check(out, r, context=kept)
+
+
+def test_a_cache_follows_its_tensors(kv4):
+    """A tensor's storage may move; its old place is not written any more."""
+    cache = kv4.Kv4Cache.allocate(2, 16, 2, 64, 32)
+    assert (cache.num_pages, cache.page_size, cache.kv_heads, cache.head_dim, cache.group) == (2, 16, 2, 64, 32)
+    k, v, slots = randn(1, 5, 2, 64), randn(2, 5, 2, 64), torch.arange(5, device="cuda")
+    old = [t.data.clone() for t in (cache.k_codes, cache.k_params, cache.v_codes, cache.v_params)]
+    held = []
+    for t in (cache.k_codes, cache.k_params, cache.v_codes, cache.v_params):
+        held.append(t.detach())
+        t.data = t.data.clone()
+    cache.append(k, v, slots)
+    assert all(torch.equal(a, b) for a, b in zip(held, old))
+    fresh = kv4.Kv4Cache.allocate(2, 16, 2, 64, 32)
+    fresh.append(k, v, slots)
+    assert torch.equal(cache.k_codes, fresh.k_codes) and torch.equal(cache.v_params, fresh.v_params)
+    assert all(torch.equal(a, b) for a, b in zip(cache.gather(slots), fresh.gather(slots)))
