@@ -9,8 +9,9 @@ A decoder layer's step between its QKV linear and its output linear, on columns 
     out = cache.attention(q, block_table, kept, max_new=1, max_kept=8192)
 
 Every method is one call into the C-ABI (layer 2 of include/itexb200.h, where the row format is defined) on torch's current
-stream; none of them synchronises, and all may be captured into a CUDA graph.  Kernels report indexes outside the cache
-through an optional device int32 `status` (STATUS_BAD_INDEX) instead of following them.
+stream; none of them synchronises (but check), and all may be captured into a CUDA graph.  Kernels report indexes outside the
+cache, and waits that expired, through a device int32 `status` instead of following them: the call's, else the cache's own, which
+Kv4Cache.check reads.
 """
 import math
 
@@ -68,10 +69,13 @@ class Kv4Cache:
     [pages, kv_heads, page_size, head_dim / group, 2], for keys and for values.  The first three dimensions may have any
     strides (a token-major cache is passed as its transpose(1, 2)); keys and values share them.  The object holds no state
     besides the tensors, which are its own for good (k_codes, k_params, v_codes, v_params; read-only attributes, as are the sizes):
-    which page belongs to which sequence is the caller's block table."""
+    which page belongs to which sequence is the caller's block table.  status: one int32 (zero) on the same device for what calls
+    without a status word of their own report; without it (a cache that allocate did not make) such calls skip in silence."""
 
-    def __init__(self, k_codes, k_params, v_codes, v_params):
-        self.dev = K.device_of(k_codes, k_params, v_codes, v_params)
+    def __init__(self, k_codes, k_params, v_codes, v_params, status=None):
+        self.dev = K.device_of(k_codes, k_params, v_codes, v_params, status)
+        _status(status)
+        self.status = status
         cs, ps, ct, pt = k_codes.shape, k_params.shape, k_codes.stride(), k_params.stride()
         if len(cs) != 4 or len(ps) != 5 or k_codes.dtype != torch.uint8 or k_params.dtype != torch.float16:
             raise ValueError("codes must be uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16 [.., head_dim / group, 2]")
@@ -103,7 +107,18 @@ class Kv4Cache:
         for _ in range(2):
             made.append(torch.zeros(dims + (head_dim // 2,), dtype=torch.uint8, device=device))
             made.append(torch.zeros(dims + (head_dim // group, 2), dtype=torch.float16, device=device))
-        return cls(*[t.transpose(1, 2) if token_major else t for t in made])
+        return cls(*[t.transpose(1, 2) if token_major else t for t in made], status=torch.zeros(1, dtype=torch.int32, device=device))
+
+    def check(self):
+        """Waits for the calls of torch's current stream and raises RuntimeError if one without a status word of its own has reported
+        something since the last check; the first report is kept, and cleared here."""
+        if self.status is None:
+            raise ValueError("this cache was made without a status word")
+        code = int(self.status)
+        if code != 0:
+            self.status.zero_()
+            raise RuntimeError({STATUS_BAD_INDEX: "a slot, page, length or row offset outside its tensor was skipped",
+                                STATUS_WAIT_EXPIRED: "a bounded wait ran out; the output is incomplete"}.get(code, "status %d" % code))
 
     def _kv(self, k, v, what):
         kp, vp = K._rows(k, "k"), K._rows(v, "v", k)
@@ -125,7 +140,7 @@ class Kv4Cache:
             pos, pdt = K._vector(positions, "positions", K._INDEX_DT, n), K._INDEX_DT[positions.dtype]
             freq, rot = K._vector(inv_freq, "inv_freq", K._FLOAT64), 2 * inv_freq.shape[0]
         K.launch(L.load().itexb_kv4_append, L.pack_kv4_append(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
-                                                              int(interleaved), mscale, _status(status)), self.dev)
+                                                              int(interleaved), mscale, _status(status, self.status)), self.dev)
 
     def gather(self, slots, dtype=torch.bfloat16, *, out_k=None, out_v=None, status=None):
         """-> (k, v) [len(slots), kv_heads, head_dim]: the values that rows `slots` stand for, zeros for slot -1."""
@@ -137,7 +152,7 @@ class Kv4Cache:
         n, kp, vp = self._kv(k, v, "gather")
         if n != tokens:
             raise ValueError("gather: %d rows for %d slots" % (n, tokens))
-        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status)),
+        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status, self.status)),
                  self.dev)
         return k, v
 
@@ -176,7 +191,7 @@ class Kv4Cache:
         else:
             op = K._rows(out, "out", q)
         args = (*self._cache(), K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
-                rows, *qp, *op, block_table.data_ptr(), tst[0], cols, kp, sp, _status(status))
+                rows, *qp, *op, block_table.data_ptr(), tst[0], cols, kp, sp, _status(status, self.status))
         lib = L.load()
         if workspace is None:
             need = lib.itexb_kv4_attention_workspace_bytes(L.pack_kv4_attention(*args, 0, 0))
@@ -190,7 +205,8 @@ class Kv4Cache:
 _INT32 = {torch.int32: 0}
 
 
-def _status(t):
+def _status(t, own=None):
+    t = own if t is None else t
     if t is None:
         return 0
     if t.dtype != torch.int32 or t.numel() != 1:

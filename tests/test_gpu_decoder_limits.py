@@ -432,3 +432,40 @@ def test_a_cache_follows_its_tensors(kv4):
     fresh.append(k, v, slots)
     assert torch.equal(cache.k_codes, fresh.k_codes) and torch.equal(cache.v_params, fresh.v_params)
     assert all(torch.equal(a, b) for a, b in zip(cache.gather(slots), fresh.gather(slots)))
+
+
+def test_a_cache_tells_what_its_calls_skipped(kv4):
+    """Without a status word of the call, reports go to the cache's own; with one, to that alone; a captured call reports at replay."""
+    cache = kv4.Kv4Cache.allocate(4, 16, 2, 64, 32)
+    k, v = randn(1, 2, 2, 64), randn(2, 2, 2, 64)
+    q, table = randn(3, 2, 4, 64, dtype=torch.bfloat16), ints([[0, 1]])
+    good, bad = ints([0, 1]), ints([0, 64])
+    cache.append(k, v, good)
+    cache.gather(good)
+    cache.attention(q, table, ints([2]))
+    cache.check()
+    for call in (lambda **kw: cache.append(k, v, bad, **kw), lambda **kw: cache.gather(bad, **kw), lambda **kw: cache.attention(q, table, ints([33]), **kw),
+                 lambda **kw: cache.attention(q, ints([[4, 1]]), ints([2]), **kw)):
+        own = ints([0])
+        call(status=own)
+        cache.check()
+        assert int(own) == kv4.STATUS_BAD_INDEX
+        call()
+        with pytest.raises(RuntimeError, match="outside its tensor"):
+            cache.check()
+        cache.check()
+    slots = good.clone()
+    cache.append(k, v, slots)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.append(k, v, slots)
+    slots.copy_(bad)
+    g.replay()
+    with pytest.raises(RuntimeError, match="outside its tensor"):
+        cache.check()
+    plain = kv4.Kv4Cache(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params)
+    plain.append(k, v, bad)
+    with pytest.raises(ValueError, match="without a status word"):
+        plain.check()
+    with pytest.raises(ValueError, match="one int32"):
+        kv4.Kv4Cache(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, status=ints([0, 0]))
