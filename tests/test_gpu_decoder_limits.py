@@ -469,3 +469,47 @@ def test_a_cache_tells_what_its_calls_skipped(kv4):
         plain.check()
     with pytest.raises(ValueError, match="one int32"):
         kv4.Kv4Cache(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, status=ints([0, 0]))
+
+
+# ------------------------------------------------------------------------------------------- bounds that tell types apart
+
+@pytest.mark.parametrize("dtype, norm", [(torch.float16, 3.3e-4), (torch.bfloat16, 2.1e-3)])
+@pytest.mark.parametrize("dim, group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 64), (256, 128)])
+@pytest.mark.parametrize("new, kept, window", [([1, 1], [1500, 77], 0), ([5, 2], [700, 33], 0), ([60, 200], [900, 200], 0), ([70, 130], [333, 600], 64)])
+def test_errors_are_those_of_the_type(kv4, dtype, norm, dim, group, new, kept, window):
+    """The 2-norm of the error against 64 bits.  An output's own rounding is uniform within half a step, whose size relative to the value
+    varies over a binade: 2^-11 (2^-8) / 3^1/2 times 0.74 is 2.1e-4 (1.7e-3).  Weights rounded to halves (and, for bf16 in the many-row
+    kernel, keys and values) add 1.2e-4 to 2.1e-4 each before averaging over tokens; one half per operand for half inputs would make the sum
+    3.8e-4."""
+    pages = [-(-n // 16) for n in kept]
+    cache = kv4.Kv4Cache.allocate(sum(pages), 16, 2, dim, group)
+    loud = 1.0 + 2.0 * (torch.arange(dim, device="cuda") % 23 == 5)
+    rows = sum(pages) * 16
+    cache.append(randn(1, rows, 2, dim) * loud, randn(2, rows, 2, dim), torch.arange(rows, device="cuda"))
+    order = torch.randperm(sum(pages), generator=torch.Generator().manual_seed(4)).to(torch.int32)
+    table = torch.full((2, max(pages)), -1, dtype=torch.int32)
+    table[0, :pages[0]], table[1, :pages[1]] = order[:pages[0]], order[pages[0]:]
+    table, starts = table.cuda(), [0, new[0], sum(new)]
+    q = randn(3, starts[-1], 8, dim, dtype=dtype)
+    out = cache.attention(q, table, ints(kept), q_starts=ints(starts), max_new=max(new), max_kept=max(kept), window=window)
+    B.check(out, B.attention(cache, q, table, kept, starts, window=window), norm=norm, context=(dim, group, new))
+
+
+@pytest.mark.parametrize("dim, group", [(64, 32), (128, 64), (256, 128)])
+@pytest.mark.parametrize("new", [1, 6, 60])
+def test_small_steps_on_a_large_common_value(kv4, dim, group, new):
+    """Half inputs: what is left of a value beside its first half is as large as the differences between tokens, for keys as for values."""
+    n = 300
+    cache = kv4.Kv4Cache.allocate(19, 16, 2, dim, group)
+    # lo near 1, 15 steps of 2^-12 each: a half near 1 resolves 2^-10
+    base = 1.0 + torch.randint(0, 16, (n, 2, dim), generator=torch.Generator().manual_seed(1)).cuda() * 2.0 ** -12
+    base[..., 0::group], base[..., 1::group] = 1.0, 1.0 + 15 * 2.0 ** -12
+    cache.append(base.float(), base.flip(0).float(), torch.arange(n, device="cuda"))
+    q = randn(3, new, 4, dim, dtype=torch.float16)
+    q -= q.float().mean(-1, keepdim=True).half()          # scores of the common value are small, their differences count
+    scale = 300.0 / dim ** 0.5
+    table = torch.arange(19, dtype=torch.int32, device="cuda")[None]
+    out = cache.attention(q, table, ints([n]), max_new=new, scale=scale)
+    r = B.attention(cache, q, table, [n], [0, new], scale=scale)
+    # keys off by 2^-21 where they are two halves, fp32 sums of 16 products at a time: 2^-19 of the sum of magnitudes in all
+    B.check(out, r, score=r["dots"] * 2.0 ** -19, context=(dim, group, new))
