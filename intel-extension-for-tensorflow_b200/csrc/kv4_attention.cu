@@ -8,8 +8,8 @@ using namespace itexb;
 namespace {
 
 // Rows that share their keys and values, above which the kernel of whole 128-token tiles is taken; the other reads the cache
-// once for every 16 rows.  Measured (rows: one kernel, the other), 32 sequences of 4096 tokens, 32 / 8 heads of 128: 16 rows 74,
-// 137 us; 24 rows 128, 137; 32 rows 131, 137; 64 rows 244, 138.  One sequence of 10240: 32 rows 31, 40 us; 64 rows 37, 40.
+// once for every 16 rows.  Measured (rows: one kernel, the other), 32 sequences of 4096 tokens, 32 / 8 heads of 128: 16 rows 75,
+// 137 us; 24 rows 129, 137; 32 rows 132, 137; 64 rows 244, 138.  One sequence of 10240: 32 rows 31, 40 us; 64 rows 37, 40.
 // head_dim 256: 32 rows 38, 53 us; 64 rows 58, 54; head_dim 64: 32 rows 30, 34 us; 64 rows 30, 34.
 constexpr int kFewRows = 32;
 bool IsPrefill(const AttnArgs& a) { return int64_t(a.max_new) * a.share > kFewRows; }

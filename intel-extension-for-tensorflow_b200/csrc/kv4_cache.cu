@@ -9,7 +9,7 @@
 // consecutive elements, which are one 32-bit word of codes; the 4 - 16 threads of a group exchange minimum and maximum
 // by shuffles, and the rotation of halves its partners.  Every step is a separately rounded fp32 operation on cosines and
 // sines rounded from 64 bits, so the codes are those of the same formulas written with plain fp32 tensor operations.
-// Measured at 16384 tokens, 8 heads of 128, groups of 64, bf16: append 47 us (1.8 TB/s; its 614 instructions per warp and 2
+// Measured at 16384 tokens, 8 heads of 128, groups of 64, bf16: append 48 us (1.8 TB/s; its 620 instructions per warp and 2
 // rows of keys and values bound it at 82 % of the issue slots, not the bytes), gather 20 us (4.3 TB/s).
 #include <algorithm>
 #include <climits>

@@ -22,9 +22,10 @@
 // roundings (keys, values, weights) would nearly double the results' error (rms 0.00038 against 0.00021 of their own
 // rounding alone), keys and values are split into two halves each and a tile holds 64 tokens' first halves and behind them
 // the second ones: twice the products, 0.00026.  The order of channels is the codes' in a word, for q, keys and the output alike.
-// Measured, 2048 new tokens after 8192 with 32 / 8 heads of 128: bf16 341 us, 0.91 PFLOP/s (softmax warps: 1650 clocks per 128
-// rows and 64 tokens, the products 1280 for both halves); half 752 us (0.82 PFLOP/s of products).  1024 tokens with head_dim
-// 256: 426 and 1540 us (one stage: the conversion is not hidden).  Six prompts up to 1900, window 1024: bf16 380, half 485 us.
+// Measured with warm caches, 2048 new tokens after 8192 with 32 / 8 heads of 128: bf16 344 us, 0.90 PFLOP/s (softmax warps: 1650
+// clocks per 128 rows and 64 tokens, the products 1280 for both halves); half 769 us (0.80 PFLOP/s of products).  1024 tokens with
+// head_dim 256: 431 and 1548 us (one stage: the conversion is not hidden).  Six prompts up to 1900, window 1024: bf16 385, half 496
+// us.  With cold ones 377 us for the first, bf16.
 // Rows of the cache that no query may see are zeros here; a value group stored as NaN, or whose values pass the largest half, is
 // zeros too and makes the rows that see it NaN at the end.  Every wait is bounded.
 #include <algorithm>

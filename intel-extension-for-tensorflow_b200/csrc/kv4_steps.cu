@@ -28,8 +28,7 @@
 // which every block takes an equal, contiguous part; a (sequence, head) that ends inside a block's part is written by it, the
 // others are joined from at most one result per block by a second kernel.  (One block per 2048 tokens instead left a fifth of
 // the machine idle behind the longest contexts, and smaller chunks cost more at their ends than they evened out.)
-// Measured, single tokens, 32 / 8 heads of 128, groups of 64: 64 sequences up to 8192 (421 MB) 104 us, 4.0 TB/s over the call, 5.3
-// while tiles stream; bound by issue slots (58 % busy) and the dependent steps of a tile with three warps per scheduler.
+// Measured, single tokens, 32 / 8 heads of 128, groups of 64: 64 sequences up to 8192 (421 MB) 104 us, 4.0 TB/s; bound by issue slots (58 % busy) and the dependent steps of a tile with three warps per scheduler.
 #include <algorithm>
 
 #include "kv4_attention.h"
@@ -132,6 +131,7 @@ __device__ __forceinline__ void StoreOut(const AttnArgs& a, int bf16, int64_t at
 }
 
 // PAGE16: pages hold a multiple of 16 tokens, so a tile lies in one page.
+// (The comparisons here and below are of before steps were scaled, which costs each side 1 to 3 %.)
 // At least so many blocks share an SM (registers).  head_dim 64 with 4 and with 5 (spills): 35, 47 us for 24 sequences of 3000 with
 // 5 tokens each; with 3 and with 4 where a tile of rows has 16 (12 tokens each): 50, 52.
 template <int DIM, int GROUP, int NT> constexpr int kShareSm = DIM == 64 ? (NT == 1 ? 4 : 3) : DIM == 128 ? (NT == 1 ? 3 : 2) : 2;

@@ -74,7 +74,8 @@ class Kv4Cache:
 
     def __init__(self, k_codes, k_params, v_codes, v_params, status=None):
         self.dev = K.device_of(k_codes, k_params, v_codes, v_params, status)
-        _status(status)
+        if status is not None:
+            _status(status)
         self.status = status
         cs, ps, ct, pt = k_codes.shape, k_params.shape, k_codes.stride(), k_params.stride()
         if len(cs) != 4 or len(ps) != 5 or k_codes.dtype != torch.uint8 or k_params.dtype != torch.float16:
@@ -130,7 +131,7 @@ class Kv4Cache:
     def append(self, k, v, slots, *, positions=None, inv_freq=None, interleaved=False, mscale=1.0, status=None):
         """Writes k, v [tokens, kv_heads, head_dim] (strided views are fine) into rows slots[t] = page * page_size + offset; -1
         skips a token; the other slots of a call must differ.  With positions and inv_freq the keys are rotated on the way."""
-        K.device_of(self.k_codes, k, v, slots, positions, inv_freq, status)
+        K.device_of(self._tensors[0], k, v, slots, positions, inv_freq, status)
         if (positions is None) != (inv_freq is None):
             raise ValueError("positions and inv_freq go together")
         n, kp, vp = self._kv(k, v, "append")
@@ -144,7 +145,7 @@ class Kv4Cache:
 
     def gather(self, slots, dtype=torch.bfloat16, *, out_k=None, out_v=None, status=None):
         """-> (k, v) [len(slots), kv_heads, head_dim]: the values that rows `slots` stand for, zeros for slot -1."""
-        K.device_of(self.k_codes, slots, out_k, out_v, status)
+        K.device_of(self._tensors[0], slots, out_k, out_v, status)
         sp = K._vector(slots, "slots", K._INDEX_DT)
         tokens = slots.shape[0]
         k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=slots.device) if out_k is None else out_k
@@ -165,7 +166,7 @@ class Kv4Cache:
         bound saves work.  -> out, whose rows behind the last sequence stay as they were (uninitialised without `out`).
         workspace: a dense uint8 tensor to use instead of a fresh one, at least as large as a refusal asks for; calls that may
         run at the same time need different ones."""
-        K.device_of(self.k_codes, q, block_table, kept, q_starts, out, status, workspace)
+        K.device_of(self._tensors[0], q, block_table, kept, q_starts, out, status, workspace)
         qp = K._rows(q, "q")
         kp = K._vector(kept, "kept", _INT32)
         seqs = kept.shape[0]
