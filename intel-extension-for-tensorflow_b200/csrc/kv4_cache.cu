@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t Quantize8(const float (&x)[8], int lanes, __
   const float lof = __half2float(lo);
   __half step = __float2half_rn(fmaxf((mx - lof) / 15.f, 0.f));
   float stepf = __half2float(step);
-  if (!(fmaf(15.f, stepf, lof) < kPastHalf)) {   // rare; NaN comes here too
+  if (!(fabsf(fmaf(15.f, stepf, lof)) < kPastHalf)) {   // rare; NaN and infinities come here too
     step = __ushort_as_half(uint16_t(__half_as_ushort(step) - 1));
     stepf = __half2float(step);
     if (!isfinite(lof) || !(fmaf(15.f, stepf, lof) < kPastHalf)) {

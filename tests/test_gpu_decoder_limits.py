@@ -513,3 +513,16 @@ def test_small_steps_on_a_large_common_value(kv4, dim, group, new):
     r = B.attention(cache, q, table, [n], [0, new], scale=scale)
     # keys off by 2^-21 where they are two halves, fp32 sums of 16 products at a time: 2^-19 of the sum of magnitudes in all
     B.check(out, r, score=r["dots"] * 2.0 ** -19, context=(dim, group, new))
+
+
+@pytest.mark.parametrize("value", [-math.inf, math.inf, math.nan, -70000.0, 70000.0, -65520.0, 65520.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_group_of_one_value_that_is_no_half_is_stored_as_nan(kv4, dtype, value):
+    cache = kv4.Kv4Cache.allocate(1, 16, 1, 128, 64)
+    x = randn(1, 3, 1, 128, dtype=dtype)
+    x[1, 0, 64:] = value
+    cache.append(x, x, ints([0, 1, 2]))
+    for y in cache.gather(ints([0, 1, 2]), torch.float32):
+        bad = torch.zeros_like(y, dtype=torch.bool)
+        bad[1, 0, 64:] = True
+        assert torch.equal(torch.isnan(y), bad) and torch.isfinite(y[~bad]).all()
