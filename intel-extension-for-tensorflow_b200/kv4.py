@@ -68,7 +68,7 @@ class Kv4Cache:
     """The cache's four tensors: codes uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16
     [pages, kv_heads, page_size, head_dim / group, 2], for keys and for values.  The first three dimensions may have any
     strides (a token-major cache is passed as its transpose(1, 2)); keys and values share them.  The object holds no state
-    besides the tensors, which are its own for good (k_codes, k_params, v_codes, v_params; read-only attributes, as are the sizes):
+    besides the tensors, which are its own for good (k_codes, k_params, v_codes, v_params; read-only attributes, as are the sizes and status):
     which page belongs to which sequence is the caller's block table.  status: one int32 (zero) on the same device for what calls
     without a status word of their own report; without it (a cache that allocate did not make) such calls skip in silence."""
 
@@ -76,7 +76,7 @@ class Kv4Cache:
         self.dev = K.device_of(k_codes, k_params, v_codes, v_params, status)
         if status is not None:
             _status(status)
-        self.status = status
+        self._own = status
         cs, ps, ct, pt = k_codes.shape, k_params.shape, k_codes.stride(), k_params.stride()
         if len(cs) != 4 or len(ps) != 5 or k_codes.dtype != torch.uint8 or k_params.dtype != torch.float16:
             raise ValueError("codes must be uint8 [pages, kv_heads, page_size, head_dim / 2] and params float16 [.., head_dim / group, 2]")
@@ -93,6 +93,7 @@ class Kv4Cache:
         self._strides = (ct[0], ct[1], ct[2], pt[0] // 2, pt[1] // 2, pt[2] // 2)
 
     k_codes, k_params, v_codes, v_params = (property(lambda self, i=i: self._tensors[i]) for i in range(4))
+    status = property(lambda self: self._own)
     num_pages, page_size, kv_heads, head_dim, group = (property(lambda self, i=i: self._sizes[i]) for i in range(5))
 
     def _cache(self):
@@ -141,7 +142,7 @@ class Kv4Cache:
             pos, pdt = K._vector(positions, "positions", K._INDEX_DT, n), K._INDEX_DT[positions.dtype]
             freq, rot = K._vector(inv_freq, "inv_freq", K._FLOAT64), 2 * inv_freq.shape[0]
         K.launch(L.load().itexb_kv4_append, L.pack_kv4_append(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, pos, freq, pdt, rot,
-                                                              int(interleaved), mscale, _status(status, self.status)), self.dev)
+                                                              int(interleaved), mscale, _status(status, self._own)), self.dev)
 
     def gather(self, slots, dtype=torch.bfloat16, *, out_k=None, out_v=None, status=None):
         """-> (k, v) [len(slots), kv_heads, head_dim]: the values that rows `slots` stand for, zeros for slot -1."""
@@ -153,7 +154,7 @@ class Kv4Cache:
         n, kp, vp = self._kv(k, v, "gather")
         if n != tokens:
             raise ValueError("gather: %d rows for %d slots" % (n, tokens))
-        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status, self.status)),
+        K.launch(L.load().itexb_kv4_gather, L.pack_kv4_gather(*self._cache(), n, K._REAL_DT[k.dtype], K._INDEX_DT[slots.dtype], *kp, *vp, sp, _status(status, self._own)),
                  self.dev)
         return k, v
 
@@ -192,7 +193,7 @@ class Kv4Cache:
         else:
             op = K._rows(out, "out", q)
         args = (*self._cache(), K._REAL_DT[q.dtype], seqs, heads, int(causal), window, max_new, max_kept, dim ** -0.5 if scale is None else scale,
-                rows, *qp, *op, block_table.data_ptr(), tst[0], cols, kp, sp, _status(status, self.status))
+                rows, *qp, *op, block_table.data_ptr(), tst[0], cols, kp, sp, _status(status, self._own))
         lib = L.load()
         if workspace is None:
             need = lib.itexb_kv4_attention_workspace_bytes(L.pack_kv4_attention(*args, 0, 0))

@@ -47,7 +47,7 @@ def test_by_parts_stretches_pairs_by_their_turns(mods, trained, base):
             assert plain / factor < f[i].item() < plain
 
 
-@pytest.mark.parametrize("name", ["k_codes", "k_params", "v_codes", "v_params", "num_pages", "page_size", "kv_heads", "head_dim", "group"])
+@pytest.mark.parametrize("name", ["k_codes", "k_params", "v_codes", "v_params", "num_pages", "page_size", "kv_heads", "head_dim", "group", "status"])
 def test_a_cache_keeps_its_tensors_and_sizes(mods, name):
     cache = object.__new__(mods[3].Kv4Cache)
     with pytest.raises(AttributeError):
